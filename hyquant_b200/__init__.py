@@ -24,6 +24,9 @@ from .decode_d_stage import (  # noqa: F401
     quantize_per_token, quantize_per_token_into,
 )
 from .d_stage_kv_cache import DStageKVCache, DStageLayerCache, QuantizedKVCache  # noqa: F401
+from .paged_kv import (  # noqa: F401
+    PagedKVCache, PageStep, page_advance, paged_append, paged_attention, paged_pages, paged_read,
+)
 from .sage_unified import (  # noqa: F401
     full_attention_fp16_triton, hybrid_prefill, sage_fp8_attention, sage_unified_attention, sage_vertical_attention_v2,
 )
@@ -36,6 +39,7 @@ __all__ = [
     "fused_d_stage_decode", "DStageKVCache", "DStageLayerCache", "create_cache_for_mode",
     "compute_vertical_indices", "quantize_per_token", "dequantize_per_token", "lse_merge",
     "sage_vertical_attention_v2", "sage_unified_attention", "sage_fp8_attention", "full_attention_fp16_triton",
+    "PagedKVCache", "PageStep", "page_advance", "paged_append", "paged_attention", "paged_pages", "paged_read",
     "install_as_src", "HyQuantError",
 ]
 

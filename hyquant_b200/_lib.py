@@ -32,6 +32,7 @@ EXPORTS = [
     "hq_prefill_quant_workspace_bytes", "hq_prefill_quant", "hq_prefill_quant_blocks", "hq_per_block_int8",
     "hq_prefill_vertical_sort", "hq_prefill_vertical_prepare", "hq_prefill_vertical_prepare_rows", "hq_prefill_transpose_v", "hq_prefill_quant_v_fp8", "hq_prefill_vertical_gather_v_fp8",
     "hq_prefill_hybrid", "hq_tc_peak",
+    "hq_page_advance", "hq_paged_append", "hq_paged_read", "hq_paged_attention_workspace_bytes", "hq_paged_attention",
     "hq_peer_exchange_bytes", "hq_peer_slot", "hq_peer_recv_slot", "hq_peer_exchange_merge", "hq_peer_status",
     "hq_peer_buffer_create", "hq_peer_buffer_open", "hq_peer_buffer_close", "hq_peer_buffer_destroy",
 ]
@@ -93,6 +94,18 @@ class PeerExchangeArgs(C.Structure):
     ]
 
 
+class PagedAttentionArgs(C.Structure):
+    """Mirror of ``hq_paged_attention_args``."""
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("R", C.c_int32), ("T", C.c_int32), ("H_Q", C.c_int32), ("H_KV", C.c_int32),
+        ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_pages", C.c_int32), ("max_q_len", C.c_int32),
+        ("dtype", C.c_int32), ("sm_scale", C.c_float), ("reserved", C.c_int32), ("num_pages", C.c_int64),
+        ("q", C.c_void_p), ("q_st", C.c_int64), ("q_sh", C.c_int64), ("pages", C.c_void_p),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("kv_lens", C.c_void_p), ("cu_q", C.c_void_p),
+        ("out", C.c_void_p), ("o_st", C.c_int64), ("o_sh", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -133,6 +146,11 @@ def _declare(lib):
     lib.hq_prefill_quant_v_fp8.argtypes = [vp, i64, i64, i64, i32, i32, i32, vp, vp, vp, vp]
     lib.hq_prefill_vertical_gather_v_fp8.argtypes = [vp, i32, i32, i32, i32, i32, vp, i64, i64, i64, vp, vp, vp]
     lib.hq_prefill_hybrid.argtypes = [C.POINTER(PrefillArgs), vp]
+    lib.hq_page_advance.argtypes = [vp, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.hq_paged_append.argtypes = [vp, vp, i32, i64, i64, i64, i64, i32, i32, vp, vp, i64, i32, vp]
+    lib.hq_paged_read.argtypes = [vp, i64, i32, vp, i32, i32, i32, vp, vp, vp]
+    lib.hq_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionArgs), C.POINTER(i64)]
+    lib.hq_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs), vp]
     lib.hq_tc_peak.argtypes = [i32, i32, vp, C.POINTER(C.c_int), vp]
     lib.hq_peer_exchange_bytes.argtypes = [i32, i32, C.POINTER(i64)]
     lib.hq_peer_slot.argtypes = [vp, i32, i32, C.c_uint32, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]

@@ -1,0 +1,93 @@
+// The paged 4-bit cache: layout, row quantiser and address arithmetic shared by its kernels.
+//
+// A page holds `page` tokens (16, 32, 64 or 128) of every kv head; a head's part of it is a run of blocks of sixteen
+// tokens, and a block lies in one piece:
+//   16 x 64 bytes K codes | 16 x 64 bytes V codes | 16 bf16 K scales | 16 bf16 V scales      = 2112 bytes
+// so that any run of tokens inside a page is one contiguous range: attention fetches it with one request, whatever the
+// page size.  Codes are two's-complement nibbles, even channel in the low one (as hq_quant_pack at 4 bits).
+//
+// Row quantiser: scale = max|x| / 7 rounded UP to bf16, within [2^-17, 9344]; code = rint(x / scale), half to even, clamped
+// to +-7.  A value code * scale then has at most 3 + 8 significant bits, a lowest bit of 2^-24 or more and a magnitude of 65408
+// at most: it IS an fp16 number, and the tensor core's 16-bit operands hold the cache without another rounding (with an
+// 11-bit scale the product is rounded: 1e-4 of a value, half of what fp16 outputs are rounded by).  The price is a step up to
+// 2^-7 wider, 0.3 % on average.  Larger values and infinities saturate; a NaN takes the lowest code and does not count for
+// the scale.
+#pragma once
+#include "hq_common.cuh"
+
+namespace hq {
+namespace paged {
+
+constexpr int kTok = HQ_PAGED_BLOCK;                    // tokens of a block
+constexpr int kBlockBytes = HQ_PAGED_BLOCK_BYTES;
+constexpr int kVOff = kTok * 64, kKsOff = 2 * kTok * 64, kVsOff = kKsOff + 2 * kTok;
+static_assert(kVsOff + 2 * kTok == kBlockBytes && kBlockBytes % 16 == 0, "block layout");
+
+inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ float scale_of(float amax) {
+  const float s = fminf(fmaxf(__fdiv_rn(amax, 7.0f), 0x1p-17f), 9344.0f);
+  return __uint_as_float((__float_as_uint(s) + 0xFFFFu) & 0xFFFF0000u);
+}
+
+// Eight lanes hold one row, sixteen channels each (all 32 lanes call).  Returns the row's scale; the lane's codes in channel order.
+// The common lane multiplies by the rounded reciprocal and corrects the product once by its remainder, which leaves it on the
+// IEEE quotient's side of every half-integer h (h * scale has 12 bits at most, so it and the remainder are exact: the argument
+// at quant_row16 holds with fewer bits), and adds 1.5 * 2^23, which rounds to the integer, ties to even.  Lanes that hold a NaN, and
+// rows whose scale is saturated, divide and clamp.
+__device__ __forceinline__ float quant_row(const float (&v)[16], uint32_t (&code)[2]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) top = fmax3_abs_nan(top, v[i], v[i + 1]);
+  bool rare = top != top;
+  if (rare) {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) top = fmax3_abs(top, v[i], v[i + 1]);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float s = scale_of(top);
+  rare |= !(top <= 65408.0f);
+  const float rcp = __frcp_rn(s);
+  constexpr uint32_t kOnes = 0x11111111u, kTop = 0x88888888u, kMagic = 0x4B400000u;
+  const float2 rcp2 = make_float2(rcp, rcp), ns2 = make_float2(-s, -s), magic2 = make_float2(12582912.f, 12582912.f);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    uint32_t c = kTop - kMagic * kOnes;              // + 8 per digit: no borrows between digits
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 x = make_float2(v[8 * w + i], v[8 * w + i + 1]);
+      const float2 t = fmul2(x, rcp2);
+      const float2 r = fadd2(ffma2(ffma2(t, ns2, x), rcp2, t), magic2);
+      c += __float_as_uint(r.x) << (4 * i);
+      c += __float_as_uint(r.y) << (4 * i + 4);
+    }
+    code[w] = c ^ kTop;
+  }
+  if (__builtin_expect(rare, 0)) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q = fminf(fmaxf(rintf(__fdiv_rn(v[8 * w + i], s)), -7.f), 7.f);      // a NaN becomes -7
+        c |= ((uint32_t)__float2int_rn(q) & 15u) << (4 * i);
+      }
+      code[w] = c;
+    }
+  }
+  return s;
+}
+
+// first byte of the sixteen-token block of `slot` (page * page_size + position in the page) of head `h`
+__device__ __forceinline__ int64_t block_offset(int64_t slot, int h, int H, int page_shift) {
+  const int64_t page = slot >> page_shift;
+  const int blocks = 1 << (page_shift - 4), in_page = (int)(slot & ((1 << page_shift) - 1));
+  return ((page * H + h) * blocks + (in_page >> 4)) * kBlockBytes;
+}
+#endif
+
+}  // namespace paged
+}  // namespace hq

@@ -1,0 +1,273 @@
+"""Paged 4-bit KV cache: requests of different lengths that come and go share a pool of pages, and attention of their new
+tokens - one each, drafts, prompt chunks - reads the pages as they lie.  The four-segment cache
+(:mod:`hyquant_b200.d_stage_kv_cache`) serves one batch of equal lengths; this one serves a ragged batch, with every
+token in 4 bits from the start (no counterpart in the reference).
+
+One layer's pool is ``pages`` uint8 ``[num_pages, H_KV, page_size // 16, 2112]`` (:func:`paged_pages`); a block of sixteen
+tokens is 16 x 64 bytes of K codes, 16 x 64 bytes of V codes, 16 bf16 K scales and 16 bf16 V scales.  A row's scale is
+max|x| / 7 rounded up to bf16, within [2^-17, 9344], and its codes are clamp(rint(x / scale), -7, 7), packed as
+:func:`hyquant_b200.quantize_per_token` packs four bits.  Every value code * scale is an fp16 number: attention works on the
+cache's values without rounding them again.  Values beyond +-65408 saturate; a NaN takes code -7.
+
+A step is: :func:`page_advance` (block tables, slots, positions - once for all layers), then per layer :func:`paged_append`
+and :func:`paged_attention`.  All of it stays on the device, allocates only its outputs (and attention its scratch) and
+can be captured in a CUDA graph.  :class:`PagedKVCache` keeps the state of a whole model.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import HyQuantError, PagedAttentionArgs
+
+BLOCK = 16                  # tokens of a block
+BLOCK_BYTES = 2112
+PAGE_SIZES = (16, 32, 64, 128)
+STATUS = {1: "too few free pages", 2: "a request longer than its table row", 4: "more new tokens than max_tokens",
+          8: "arguments that do not fit the state"}
+
+_I32, _I64 = torch.int32, torch.int64
+
+
+class PageStep(NamedTuple):
+    """What :func:`page_advance` gives.  ``slots`` int64 [max_tokens] (-1 behind the last token), ``positions`` int32 [max_tokens],
+    ``cu_q`` int32 [R + 1]; ``kv_lens``, ``held`` int32 [R] and ``free_count`` int32 [1] are the state after the step;
+    ``status`` int32 [1] is 0 unless the step was refused (:data:`STATUS`)."""
+    kv_lens: torch.Tensor
+    held: torch.Tensor
+    free_count: torch.Tensor
+    cu_q: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    status: torch.Tensor
+
+
+def _call(fn, dev, *args) -> int:
+    """One library call on the current stream of ``dev``, which need not be the current device."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return fn(*args, _lib.stream_ptr(dev))
+    return fn(*args, _lib.stream_ptr(dev))
+
+
+def paged_pages(num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda") -> torch.Tensor:
+    """An empty pool of one layer."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    return torch.zeros(num_pages, num_kv_heads, page_size // BLOCK, BLOCK_BYTES, dtype=torch.uint8, device=device)
+
+
+def _pool(pages: torch.Tensor) -> Tuple[int, int, int]:
+    """(num_pages, H_KV, page_size) of a pool."""
+    _lib.require_cuda(pages, "pages")
+    shape = pages.shape
+    if pages.dtype != torch.uint8 or len(shape) != 4 or shape[3] != BLOCK_BYTES or not pages.is_contiguous():
+        raise HyQuantError(f"pages must be contiguous uint8 [num_pages, H_KV, page_size // {BLOCK}, {BLOCK_BYTES}]")
+    page_size = shape[2] * BLOCK
+    if page_size not in PAGE_SIZES:
+        raise HyQuantError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    return shape[0], shape[1], page_size
+
+
+def _vector(t: torch.Tensor, n: Optional[int], dtype, device, name: str) -> int:
+    """Address of a contiguous one-dimensional tensor."""
+    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != device or not t.is_contiguous():
+        raise HyQuantError(f"{name} must be contiguous {dtype} [{'n' if n is None else n}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _table(page_table: torch.Tensor, R: int, device) -> Tuple[int, int, int]:
+    """(address, row stride, columns) of a block table."""
+    if page_table.dtype != _I32 or page_table.dim() != 2 or page_table.shape[0] != R or page_table.device != device:
+        raise HyQuantError(f"page_table must be int32 [{R}, max_pages] on {device}")
+    cols = page_table.shape[1]
+    if cols > 1 and page_table.stride(1) != 1:
+        raise HyQuantError("page_table rows must be contiguous")
+    return page_table.data_ptr(), page_table.stride(0) if R > 1 else max(cols, 1), cols
+
+
+def page_advance(kv_lens: torch.Tensor, held: torch.Tensor, add: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, *, page_size: int, max_tokens: int, keep: Optional[torch.Tensor] = None,
+                 in_place: bool = False) -> PageStep:
+    """Block tables, slots and positions of one step, on the device (:class:`PageStep`).
+
+    Request r keeps its first ``keep[r]`` cached tokens (default all of ``kv_lens[r]``; fewer drops rejected drafts, 0 ends
+    the request) and takes ``add[r]`` new ones (0 is allowed).  Pages it no longer needs go onto the stack
+    ``free_pages[:free_count]`` in request and page order, then missing ones are taken from its top.  ``page_table`` int32
+    [R, max_pages] and ``free_pages`` change in place; ``held`` int32 [R] says how many pages a row holds.  ``max_tokens`` is
+    the length of ``slots`` and ``positions``, at least the sum of ``add``.  ``in_place`` writes the new ``kv_lens``, ``held`` and
+    ``free_count`` over the old.
+
+    A step that cannot be done changes nothing and sets ``status``; its ``cu_q`` is 0 throughout and its slots -1, so that appending
+    and attention do nothing with it."""
+    _lib.require_cuda(kv_lens, "kv_lens")
+    dev, R = kv_lens.device, kv_lens.shape[0]
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if max_tokens < 0:
+        raise ValueError(f"max_tokens must be >= 0, got {max_tokens}")
+    lens_p, held_p, add_p = _vector(kv_lens, R, _I32, dev, "kv_lens"), _vector(held, R, _I32, dev, "held"), _vector(add, R, _I32, dev, "add")
+    keep_p = None if keep is None else _vector(keep, R, _I32, dev, "keep")
+    free_p, count_p = _vector(free_pages, None, _I32, dev, "free_pages"), _vector(free_count, 1, _I32, dev, "free_count")
+    table_p, stride, cols = _table(page_table, R, dev)
+    # one allocation: cu_q, positions, status, and the new state unless it goes over the old
+    ints = torch.empty(R + 2 + max_tokens + (0 if in_place else 2 * R + 1), dtype=_I32, device=dev)
+    slots = torch.empty(max_tokens, dtype=_I64, device=dev)
+    cu_q, positions, status, rest = ints.split_with_sizes((R + 1, max_tokens, 1, ints.shape[0] - R - 2 - max_tokens))
+    if in_place:
+        lens2, held2, count2 = kv_lens, held, free_count
+    else:
+        lens2, held2, count2 = rest.split_with_sizes((R, R, 1))
+    base = ints.data_ptr()
+    rc = _call(_lib.lib().hq_page_advance, dev, lens_p, held_p, add_p, keep_p, R, table_p, stride, cols, free_p, free_pages.shape[0], count_p,
+               page_size, max_tokens, lens2.data_ptr(), held2.data_ptr(), count2.data_ptr(), base, slots.data_ptr(), base + 4 * (R + 1),
+               base + 4 * (R + 1 + max_tokens))
+    if rc != 0:
+        _lib.check(rc, "hq_page_advance")
+    return PageStep(lens2, held2, count2, cu_q, slots, positions, status)
+
+
+def paged_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise rows ``k``, ``v`` [T, H_KV, 128] (bf16, fp16 or fp32, views are fine) into their slots of ``pages``.  Slots that are -1
+    or outside the pool are skipped; the others of one call are distinct."""
+    num_pages, H, page_size = _pool(pages)
+    T, dev = slots.shape[0], pages.device
+    if k.shape != (T, H, 128) or v.shape != (T, H, 128) or k.dtype != v.dtype or k.device != dev or v.device != dev:
+        raise HyQuantError(f"k and v must be [{T}, {H}, 128] of one dtype on {dev}, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    code = _lib.dtype_code(k.dtype)
+    slots_p = _vector(slots, T, _I64, dev, "slots")
+    k, v = _rows(k), _rows(v)
+    rc = _call(_lib.lib().hq_paged_append, dev, k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), T, H,
+               slots_p, pages.data_ptr(), num_pages, page_size)
+    if rc != 0:
+        _lib.check(rc, "hq_paged_append")
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x with rows of 128 that the kernels read in 16-byte pieces; a copy if it has none."""
+    st, sh, sd = x.stride()
+    return x if sd == 1 and not (st | sh) & 7 and not x.data_ptr() & 15 else x.contiguous()
+
+
+def paged_read(pages: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cache's values of ``slots`` as rows (k, v) [T, H_KV, 128] (fp16 and fp32 hold them exactly); zeros for slots outside the pool."""
+    num_pages, H, page_size = _pool(pages)
+    code = _lib.dtype_code(dtype)
+    T, dev = slots.shape[0], pages.device
+    slots_p = _vector(slots, T, _I64, dev, "slots")
+    k = torch.empty(T, H, 128, dtype=dtype, device=dev)
+    v = torch.empty(T, H, 128, dtype=dtype, device=dev)
+    rc = _call(_lib.lib().hq_paged_read, dev, pages.data_ptr(), num_pages, page_size, slots_p, T, H, code, k.data_ptr(), v.data_ptr())
+    if rc != 0:
+        _lib.check(rc, "hq_paged_read")
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor, *,
+                    cu_q: Optional[torch.Tensor] = None, max_q_len: int = 1, sm_scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of new tokens ``q`` [T, H_Q, 128] (bf16 or fp16) over the cache, which holds them already -> [T, H_Q, 128].
+
+    Request r has the rows ``cu_q[r] .. cu_q[r + 1]`` of ``q`` (without ``cu_q``: row r, one each) and ``kv_lens[r]`` cached tokens
+    with them; its token i of n sees the first ``kv_lens[r] - n + i + 1`` of them, and gets zeros if there is none.
+    ``max_q_len`` is the most tokens of a request (tokens beyond it are not computed).  ``sm_scale`` is 128 ** -0.5 by default.
+    Rows of ``out`` behind the last token stay as they are (without ``out`` they are not initialised)."""
+    num_pages, H, page_size = _pool(pages)
+    dev = pages.device
+    if q.dim() != 3 or q.shape[2] != 128 or q.device != dev:
+        raise HyQuantError(f"q must be [T, H_Q, 128] on {dev}, got {tuple(q.shape)} on {q.device}")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise HyQuantError(f"q must be bf16 or fp16, got {q.dtype}")
+    T, H_Q, _ = q.shape
+    if kv_lens.dim() != 1:
+        raise HyQuantError("kv_lens must be int32 [R]")
+    R = kv_lens.shape[0]
+    lens_p = _vector(kv_lens, R, _I32, dev, "kv_lens")
+    table_p, stride, cols = _table(page_table, R, dev)
+    if cu_q is None:
+        if T != R or max_q_len != 1:
+            raise HyQuantError(f"without cu_q every request has one token: q has {T} rows, kv_lens {R}, max_q_len {max_q_len}")
+        cu_p = None
+    else:
+        cu_p = _vector(cu_q, R + 1, _I32, dev, "cu_q")
+        if max_q_len < 1:
+            raise ValueError(f"max_q_len must be >= 1, got {max_q_len}")
+    q = _rows(q)
+    if out is None:
+        out = torch.empty(T, H_Q, 128, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+        raise HyQuantError(f"out must be {tuple(q.shape)} {q.dtype} on {dev} with contiguous rows")
+    a = PagedAttentionArgs(C.sizeof(PagedAttentionArgs), R, T, H_Q, H, 128, page_size, cols, max_q_len, _lib.dtype_code(q.dtype),
+                           128 ** -0.5 if sm_scale is None else sm_scale, 0, num_pages, q.data_ptr(), q.stride(0), q.stride(1),
+                           pages.data_ptr(), table_p, stride, lens_p, cu_p, out.data_ptr(), out.stride(0), out.stride(1), None, 0)
+    lib, n = _lib.lib(), C.c_int64()
+    ref = C.byref(a)
+    rc = lib.hq_paged_attention_workspace_bytes(ref, C.byref(n))
+    if rc == 0:
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+        rc = _call(lib.hq_paged_attention, dev, ref)
+    if rc != 0:
+        _lib.check(rc, "hq_paged_attention")
+    return out
+
+
+class PagedKVCache:
+    """State of a model's paged cache: a pool of pages per layer, one block table, stack of free pages and set of lengths for
+    all layers.  ``advance`` once per step, then ``append`` and ``attention`` per layer; buffers keep their addresses, so that a
+    whole step can be captured in a CUDA graph (``add`` and ``keep`` are read on the device).
+
+    Requests live in ``max_requests`` rows; a row of length 0 is free.  ``kv_lens`` are the cached tokens of each row."""
+
+    def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, *, max_requests: int, max_pages_per_request: int,
+                 page_size: int = 64, device="cuda"):
+        if min(num_layers, num_pages, num_kv_heads, max_requests, max_pages_per_request) < 1:
+            raise ValueError("sizes of a paged cache must be positive")
+        self.page_size = page_size
+        self.pages = [paged_pages(num_pages, num_kv_heads, page_size, device) for _ in range(num_layers)]
+        dev = self.pages[0].device
+        self.page_table = torch.full((max_requests, max_pages_per_request), -1, dtype=_I32, device=dev)
+        self.kv_lens = torch.zeros(max_requests, dtype=_I32, device=dev)
+        self.held = torch.zeros(max_requests, dtype=_I32, device=dev)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=_I32, device=dev)      # page 0 on top
+        self.free_count = torch.full((1,), num_pages, dtype=_I32, device=dev)
+        self.step: Optional[PageStep] = None
+
+    def __len__(self):
+        return len(self.pages)
+
+    def advance(self, add: torch.Tensor, *, max_tokens: int, keep: Optional[torch.Tensor] = None) -> PageStep:
+        """Next step: ``add`` [max_requests] new tokens, ``keep`` tokens of the cached ones (:func:`page_advance`)."""
+        self.step = page_advance(self.kv_lens, self.held, add, self.page_table, self.free_pages, self.free_count,
+                                 page_size=self.page_size, max_tokens=max_tokens, keep=keep, in_place=True)
+        return self.step
+
+    def check(self) -> None:
+        """Raise if the last step was refused (reads the status: waits for the device)."""
+        why = 0 if self.step is None else int(self.step.status.item())
+        if why:
+            raise HyQuantError("the step was refused: " + ", ".join(text for bit, text in STATUS.items() if why & bit))
+
+    def _step(self) -> PageStep:
+        if self.step is None:
+            raise HyQuantError("advance() comes before append(), attention() and read()")
+        return self.step
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's rows of one layer, [max_tokens, H_KV, 128] (:func:`paged_append`)."""
+        paged_append(self.pages[layer], k, v, self._step().slots)
+
+    def attention(self, layer: int, q: torch.Tensor, *, max_q_len: int, sm_scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The step's tokens of one layer, [max_tokens, H_Q, 128] (:func:`paged_attention`)."""
+        return paged_attention(q, self.pages[layer], self.page_table, self.kv_lens, cu_q=self._step().cu_q, max_q_len=max_q_len,
+                               sm_scale=sm_scale, out=out)
+
+    def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+        """Rows of one layer by slot (:func:`paged_read`)."""
+        return paged_read(self.pages[layer], slots, dtype)

@@ -445,6 +445,69 @@ int hq_prefill_vertical_gather_v_fp8(const int32_t* vidx_asc, int B, int H_Q, in
                                      void* stream);
 
 /* --------------------------------------------------------------------------
+ * Paged 4-bit cache (no counterpart in the reference, whose cache is one batch of equal lengths): requests of different
+ * lengths share a pool of pages.  One layer's pool is
+ *   pages  uint8 [num_pages, H_KV, page_size / 16, HQ_PAGED_BLOCK_BYTES], 16-byte aligned, page_size 16, 32, 64 or 128;
+ * a block of sixteen tokens is 16 x 64 bytes of K codes, 16 x 64 bytes of V codes, 16 bf16 K scales, 16 bf16 V scales.
+ * scale = max|x| / 7 rounded up to bf16, within [2^-17, 9344]; code = clamp(rint(x / scale), -7, 7), nibbles as hq_quant_pack
+ * (even channel low).  Every value code * scale is an fp16 number.  Larger values saturate, a NaN takes code -7.
+ * A slot is page * page_size + position in the page; the layers of a model share tables and slots, each with a pool of its own.
+ */
+#define HQ_PAGED_BLOCK 16
+#define HQ_PAGED_BLOCK_BYTES 2112
+
+/* One step's bookkeeping for R requests (R <= 8192), on the device: request r keeps its first keep[r] tokens (null: all of
+ * kv_lens[r]) and takes add[r] new ones.  With target = keep + add and need = ceil(target / page_size): pages of a table row beyond need go back
+ * onto the stack free_pages[0 .. free_count) in request and page order, then missing ones are taken from its top in request
+ * and page order.  Token t of the step, the i-th new one of request r, gets position keep[r] + i and slot
+ * page_table[r, position / page_size] * page_size + position % page_size; cu_q is the running sum of add.  slots / positions of the T entries
+ * behind the last token are -1 / 0.  page_table and free_pages change in place (only entries beyond held / at and beyond the
+ * count), the others go to *_out, which may be the inputs.
+ *   kv_lens, held (pages in the row), add, keep  int32 [R]; page_table int32 [R, max_pages] with row stride table_stride;
+ *   free_pages int32 [free_cap]; free_count int32 [1]; cu_q int32 [R + 1]; slots int64 [T]; positions int32 [T]
+ *   status int32 [1]: 0, or why nothing was changed (cu_q is then 0 throughout, slots -1): bit 0 too few free pages, bit 1 a
+ *   request longer than max_pages, bit 2 more than T new tokens, bit 3 arguments that do not fit (keep > kv_lens, a negative
+ *   number, held outside [ceil(kv_lens / page_size), max_pages], a full stack).  The word is written by every call. */
+int hq_page_advance(const int32_t* kv_lens, const int32_t* held, const int32_t* add, const int32_t* keep, int R,
+                    int32_t* page_table, int64_t table_stride, int max_pages, int32_t* free_pages, int free_cap,
+                    const int32_t* free_count, int page_size, int T, int32_t* kv_lens_out, int32_t* held_out,
+                    int32_t* free_count_out, int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* status, void* stream);
+
+/* T rows of K and V, [T, H_KV, 128] in dtype (bf16, fp16, fp32; rows 16-byte aligned, strides in elements, multiples of 8),
+ * quantised into their slots.  A slot outside [0, num_pages * page_size) is skipped (padding is -1); the slots of a call are
+ * distinct. */
+int hq_paged_append(const void* k, const void* v, int dtype, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int T, int H_KV,
+                    const int64_t* slots, void* pages, int64_t num_pages, int page_size, void* stream);
+
+/* The values of T slots as rows [T, H_KV, 128] in dtype, contiguous, 16-byte aligned (bf16 rounds, fp16 and fp32 are exact);
+ * a slot outside the pool gives zeros. */
+int hq_paged_read(const void* pages, int64_t num_pages, int page_size, const int64_t* slots, int T, int H_KV, int dtype,
+                  void* k, void* v, void* stream);
+
+/* Attention of T new tokens over the cache, which holds them already.  Request r has the tokens cu_q[r] .. cu_q[r + 1]
+ * (null: token r) and kv_lens[r] cached tokens with them; its token i of n sees keys 0 .. kv_lens[r] - n + i:
+ *   out[t, h] = sum_j softmax_j(sm_scale q[t, h] . k_j) v_j;   a token that sees no key gets zeros.
+ * max_q_len: no request has more tokens (those beyond are not computed).  Rows of out behind the last token are not written.
+ * Lengths past the table and pages outside the pool are treated as absent keys. */
+typedef struct hq_paged_attention_args {
+  int32_t struct_bytes;
+  int32_t R, T, H_Q, H_KV, head_dim;          /* H_Q / H_KV 1..16, head_dim 128 */
+  int32_t page_size, max_pages, max_q_len;
+  int32_t dtype;                              /* of q and out: HQ_BF16 or HQ_F16 */
+  float   sm_scale;                           /* >= 0 */
+  int32_t reserved;
+  int64_t num_pages;
+  const void* q; int64_t q_st, q_sh;          /* [T, H_Q, 128]: strides in elements, multiples of 8; 16-byte aligned */
+  const void* pages;
+  const int32_t* page_table; int64_t table_stride;
+  const int32_t* kv_lens; const int32_t* cu_q;
+  void* out; int64_t o_st, o_sh;
+  void* workspace; int64_t workspace_bytes;   /* hq_paged_attention_workspace_bytes; contents do not matter, 16-byte aligned */
+} hq_paged_attention_args;
+int hq_paged_attention_workspace_bytes(const hq_paged_attention_args* args, int64_t* bytes);
+int hq_paged_attention(const hq_paged_attention_args* args, void* stream);
+
+/* --------------------------------------------------------------------------
  * Tensor-pipe peak probe (no counterpart in the reference): runs tcgen05.mma products of `kind` (0 = kind::i8,
  * 1 = kind::f8f6f4 on e4m3, 2 = kind::f16 on bf16) back to back on every SM, operands resident in shared memory,
  * accumulators in tensor memory.  One launch does sms * steps products of 128 x 256 x K (K = 128 for the 8-bit kinds,

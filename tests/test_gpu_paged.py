@@ -1,0 +1,479 @@
+"""The paged 4-bit cache on the GPU against plain forms in 64 bits."""
+
+import random
+
+import pytest
+import torch
+
+import hyquant_b200 as hq
+from tests import paged_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------------------------------------- block tables and slot maps
+
+class State:
+    def __init__(self, R, page, max_pages, num_pages):
+        self.page, self.max_pages, self.room = page, max_pages, num_pages
+        self.book = plain.Book([[] for _ in range(R)], [0] * R, list(range(num_pages)), page)
+        self.wide = torch.full((R, max_pages + 5), -7, dtype=torch.int32, device=DEV)
+        self.table = self.wide[:, :max_pages]                               # a row stride of its own
+        self.lens, self.held = ints([0] * R), ints([0] * R)
+        self.free, self.count = ints(list(range(num_pages))), ints([num_pages])
+
+    def step(self, add, keep, T, in_place):
+        got = hq.page_advance(self.lens, self.held, ints(add), self.table, self.free, self.count, page_size=self.page, max_tokens=T,
+                              keep=None if keep is None else ints(keep), in_place=in_place)
+        cu, slots, pos, why = self.book.advance(add, keep, max_pages=self.max_pages, max_tokens=T, room=self.room)
+        assert int(got.status) == why
+        assert got.cu_q.tolist() == cu and got.slots.tolist() == slots and got.positions.tolist() == pos
+        assert got.kv_lens.tolist() == self.book.lens and got.held.tolist() == [len(r) for r in self.book.rows]
+        assert int(got.free_count) == len(self.book.free)
+        assert self.free[:len(self.book.free)].tolist() == self.book.free
+        table = self.table.tolist()
+        assert all(table[r][:len(row)] == row for r, row in enumerate(self.book.rows))
+        assert (self.wide[:, self.max_pages:] == -7).all()
+        self.lens, self.held, self.count = got.kv_lens, got.held, got.free_count
+        return why
+
+
+@pytest.mark.parametrize("R,page,most,T", [(1, 16, 40, 40), (3, 32, 1, 3), (64, 64, 1, 80), (65, 16, 200, 4096), (1024, 128, 3, 2048),
+                                           (1025, 16, 5, 6000), (4000, 32, 9, 40000), (8192, 16, 1, 8192)])
+def test_advance_steps(R, page, most, T):
+    rng = random.Random(R * page + most)
+    s = State(R, page, 64, 70000 if R > 1000 else 40 * R)
+    ok = 0
+    for step in range(7):
+        add, left = [], T
+        for r in range(R):
+            a = min(left, rng.choice([0, 1, 1, rng.randint(0, most)]))
+            left -= a
+            add.append(a)
+        keep = None if step % 3 == 0 else [0 if rng.random() < 0.1 else max(0, n - rng.randint(0, 20)) for n in s.book.lens]
+        ok += s.step(add, keep, T, step % 2 == 1) == 0
+    assert ok >= 5
+
+
+def test_advance_refuses_and_changes_nothing():
+    s = State(3, 16, 4, 6)
+    assert s.step([40, 10, 1], None, 60, False) == 0                         # 3 + 1 + 1 pages of 6
+    before = s.wide.clone(), s.free.clone()
+    assert s.step([0, 0, 16 * 4], None, 64, True) == 2                       # five pages in a row of four
+    assert s.step([0, 0, 16 * 3 - 1], None, 64, False) == 1                  # two more pages, one is free
+    assert s.step([0, 10, 10], None, 19, True) == 4
+    assert s.step([0, 1, 0], [40, 11, 1], 4, False) == 8                     # keeps more than there is
+    assert s.step([0, -1, 0], None, 4, False) == 8
+    assert s.step([1, 1, 1], [-1, 10, 1], 4, True) == 8
+    assert s.step([2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1], None, 4, True) == 2
+    assert torch.equal(s.wide, before[0]) and torch.equal(s.free, before[1])
+    assert s.step([0, 0, 0], [0, 10, 1], 0, True) == 0                       # the first request ends
+    assert s.step([30, 0, 33], None, 63, True) == 0                          # and its pages are taken again
+
+
+def test_advance_state_that_does_not_fit():
+    z = ints([0])
+    for lens, held, count, free in (([17], [1], 1, 4), ([0], [3], 1, 4), ([0], [-1], 1, 4), ([0], [0], -1, 4), ([0], [1], 4, 4), ([-1], [0], 1, 4)):
+        got = hq.page_advance(ints(lens), ints(held), z, ints([[5, 6]]), ints([0] * free), ints([count]), page_size=16, max_tokens=2)
+        assert int(got.status) == 8 and got.slots.tolist() == [-1, -1] and got.cu_q.tolist() == [0, 0]
+        assert got.kv_lens.tolist() == lens and got.held.tolist() == held and int(got.free_count) == count
+
+
+def test_advance_pages_pass_from_one_request_to_another_in_one_step():
+    s = State(4, 16, 8, 8)
+    assert s.step([64, 64, 0, 0], None, 128, True) == 0
+    assert s.step([0, 3, 64, 0], [0, 61, 0, 0], 70, True) == 0
+
+
+# ---------------------------------------------------------------------------------------------- rows in, rows out
+
+def special_rows(dtype):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(24, 128, generator=g, dtype=torch.float64)
+    x[0] = 0.0
+    x[1] *= 1e-7                                                            # below the smallest scale
+    x[2] *= 1e4
+    x[3, 5], x[4, 7], x[5, 9] = float("inf"), float("-inf"), float("nan")
+    x[6] = float("nan")
+    x[7] = torch.arange(128) % 15 * 0.5 - 3.5                               # scale 0.5: quotients on integers
+    x[7, 0] = 3.5
+    x[8] = (torch.arange(128) % 15 * 0.5 - 3.5) * 0.5                       # and on half-integers
+    x[8, 0] = 3.5
+    x[9] = 7.0 * 2.0 ** -17
+    x[10] *= 2.0 ** -20 if dtype != torch.float16 else 2.0 ** -13
+    x[11] = 65504.0 if dtype == torch.float16 else 70000.0
+    x[12] = -65408.0
+    x[13, 3], x[13, 4] = float("inf"), float("nan")
+    x[14] *= 3e38 / x[14].abs().max() if dtype != torch.float16 else 1.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,H,page", [(1, 1, 16), (24, 3, 32), (257, 8, 64), (1000, 2, 128)])
+def test_append_and_read(T, H, page, dtype):
+    g = torch.Generator(device=DEV).manual_seed(T + H)
+    num = -(-T // page) + 3
+    fused = torch.randn(T, H + 1, 2, 128, generator=g, device=DEV).to(dtype)     # rows of K and V lie between one another
+    if T >= 24:
+        fused[:24, 0, 0] = special_rows(dtype).to(DEV)
+        fused[:24, H - 1, 1] = special_rows(dtype).flip(0).to(DEV)
+    k, v = fused[:, :H, 0], fused[:, :H, 1]
+    slots = torch.randperm(num * page, generator=g, device=DEV)[:T].contiguous()
+    if T > 10:
+        slots[3], slots[7], slots[9] = -1, num * page, -(1 << 40)
+    pages = torch.randint(0, 256, (num, H, page // 16, 2112), generator=g, device=DEV, dtype=torch.uint8)
+    want = pages.clone()
+    inside = torch.where(slots < num * page, slots, -1)
+    plain.store(want, inside, k, v)
+    hq.paged_append(pages, k, v, slots)
+    assert torch.equal(pages, want)
+    pages.view(torch.bfloat16)[..., 1024:][~torch.isfinite(pages.view(torch.bfloat16)[..., 1024:])] = 1.0
+    for out in (torch.bfloat16, torch.float16, torch.float32):
+        got = hq.paged_read(pages, slots, out)
+        for a, b in zip(got, plain.values(pages, inside.clamp(min=0))):
+            b = torch.where((inside >= 0)[:, None, None], b, 0.0)
+            assert torch.equal(a, b.to(torch.float32).to(out))              # code * scale has 11 bits at most
+
+
+def test_values_are_fp16_numbers():
+    """Every scale of the format times every code, and that the row's largest value is kept to the last code."""
+    bits = torch.arange(0x3700, 0x4612 + 1, dtype=torch.int32).to(torch.int16)
+    s = bits.view(torch.bfloat16).double()
+    assert s[0] == 2.0 ** -17 and s[-1] == 9344.0
+    v = s[:, None] * torch.arange(-7, 8)
+    assert torch.equal(v, v.to(torch.float16).double())
+    x = torch.rand(4096, 1, 128, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    x = x * torch.logspace(-5, 4, 4096, device=DEV)[:, None, None]
+    pages = hq.paged_pages(32, 1, 128)
+    slots = torch.arange(4096, device=DEV)
+    hq.paged_append(pages, x, x, slots)
+    k, _ = hq.paged_read(pages, slots, torch.float32)
+    top = x.amax(-1)
+    assert ((k - x).abs().amax(-1) <= top / 14 * (1 + 2.0 ** -7) + 2.0 ** -18).all()
+
+
+def test_rows_that_need_a_copy():
+    x = torch.randn(5, 2, 129, device=DEV).to(torch.bfloat16)[..., 1:]
+    pages, want = hq.paged_pages(2, 2, 16), hq.paged_pages(2, 2, 16)
+    slots = torch.arange(5, device=DEV)
+    hq.paged_append(pages, x, x.transpose(0, 1).contiguous().transpose(0, 1), slots)
+    plain.store(want, slots, x, x)
+    assert torch.equal(pages, want)
+
+
+# ---------------------------------------------------------------------------------------------- attention
+
+def make(lens, new, hq_heads, kv_heads, page, dtype, seed, extra_cols=2, behind=0, nan_holes=True):
+    """Inputs of a call: pages out of order, every row that no request holds full of NaN scales."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    need = [-(-L // page) for L in lens]
+    num = sum(need) + 3
+    pages = torch.randint(0, 256, (num, kv_heads, page // 16, 2112), generator=g, device=DEV, dtype=torch.uint8)
+    if nan_holes:
+        pages.view(torch.bfloat16)[..., 1024:] = float("nan")
+    order = torch.randperm(num, generator=g, device=DEV).tolist()
+    table = torch.full((len(lens), max(need) + extra_cols), 2 ** 30, dtype=torch.int32, device=DEV)
+    at = 0
+    for r, (L, n) in enumerate(zip(lens, need)):
+        table[r, :n] = ints(order[at:at + n])
+        at += n
+        if L:
+            j = torch.arange(L, device=DEV)
+            slots = table[r, j // page].long() * page + j % page
+            k = torch.randn(L, kv_heads, 128, generator=g, device=DEV)
+            k[..., 3] += 4.0
+            plain.store(pages, slots, k.to(dtype), torch.randn(L, kv_heads, 128, generator=g, device=DEV).to(dtype))
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1] + behind, hq_heads, 128, generator=g, device=DEV).to(dtype)
+    return q, pages, table, cu
+
+
+def verify(got, q, pages, table, lens, cu, sm_scale=None):
+    want, tol = plain.attention(q, pages, table, lens, cu, sm_scale)
+    T = cu[-1]
+    off = (got[:T].double() - want[:T]).abs()
+    assert torch.isfinite(got[:T]).all()
+    assert (off <= tol[:T]).all(), f"{(off - tol[:T]).max():.3e} beyond the tolerance, off by {off.max():.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("lens", [[1], [17], [16, 0, 33, 1, 128], [129, 31, 500, 64, 15, 2, 255, 1000]])
+def test_one_token_each(lens, page, dtype):
+    new = [1] * len(lens)
+    q, pages, table, cu = make(lens, new, 8, 2, page, dtype, seed=page)
+    verify(hq.paged_attention(q, pages, table, ints(lens)), q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (2, 1), (6, 2), (5, 1), (7, 1), (8, 1), (18, 2), (11, 1), (16, 1), (32, 2), (4, 4)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 1, 0], [5, 3, 130], [300, 1, 20]])
+def test_head_groups(heads, new):
+    lens = [700, 129, 333]
+    q, pages, table, cu = make(lens, new, *heads, 32, torch.bfloat16, seed=heads[0])
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("lens,new", [([1], [1]), ([5, 70, 0, 64], [5, 3, 0, 64]), ([10, 3, 0, 200], [12, 5, 4, 2]), ([130, 257, 1], [129, 1, 1]),
+                                      ([1000, 64, 777, 2, 128], [7, 64, 333, 1, 65]), ([513], [513])])
+def test_several_tokens(lens, new, page, dtype):
+    """Chunks from one token to the whole prompt, requests without tokens, more new tokens than cached ones (rows that see nothing)."""
+    q, pages, table, cu = make(lens, new, 8, 2, page, dtype, seed=page + len(lens))
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("lens,new,heads", [([40000], [1], (8, 1)), ([9000, 1, 20000, 300], [1, 1, 1, 1], (32, 8)), ([20000, 500], [2, 2], (32, 2)),
+                                            ([12000, 5000], [40, 1], (32, 8)), ([6000], [1500], (8, 2)), ([30000, 8], [4, 4], (8, 2))])
+def test_long(lens, new, heads):
+    q, pages, table, cu = make(lens, new, *heads, 64, torch.bfloat16, seed=9)
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_requests(new):
+    rng = random.Random(4)
+    lens = [rng.choice([0, 1, rng.randint(1, 90), rng.randint(1, 900)]) + new for _ in range(700)]
+    q, pages, table, cu = make(lens, [new] * 700, 4, 1, 16, torch.float16, seed=2)
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=new)
+    verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+def test_scores_far_apart(new):
+    """Large queries and scales: references that move, scores that vanish, values near the end of the format."""
+    lens = [900, 450]
+    for scale, sm in ((30.0, None), (1e-3, None), (1.0, 0.0), (100.0, 1.0), (1.0, 3.0)):
+        q, pages, table, cu = make(lens, new, 8, 2, 32, torch.bfloat16, seed=11)
+        q = (q.float() * scale).to(torch.bfloat16)
+        got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new), sm_scale=sm)
+        verify(got, q, pages, table, lens, cu, sm)
+
+
+@pytest.mark.parametrize("new", [[1], [70]])
+@pytest.mark.parametrize("grow", [False, True])
+def test_scales_of_very_different_size(new, grow):
+    """Rows of V from 2^-12 to the format's end, the large ones first or last; a heavy key with a tiny value."""
+    L = 600
+    q, pages, table, cu = make([L], new, 4, 1, 64, torch.float16, seed=3)
+    j = torch.arange(L, device=DEV)
+    slots = table[0, j // 64].long() * 64 + j % 64
+    k = torch.randn(L, 1, 128, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    v = torch.randn(L, 1, 128, device=DEV, generator=torch.Generator(DEV).manual_seed(2))
+    size = torch.logspace(-12, 9, L, base=2.0, device=DEV)
+    v = v * (size if grow else size.flip(0))[:, None, None]
+    k[0], v[0] = 6.0 * q[0, 0].float(), 1e-4
+    plain.store(pages, slots, k, v)
+    got = hq.paged_attention(q, pages, table, ints([L]), cu_q=ints(cu), max_q_len=max(new))
+    verify(got, q, pages, table, [L], cu)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 90, 1]])
+def test_pages_outside_the_pool_and_lengths_past_the_table(new):
+    lens = [300, 200, 150]
+    q, pages, table, cu = make(lens, new, 8, 2, 32, torch.bfloat16, seed=21, extra_cols=0)
+    table[0, 2], table[0, 9], table[1, 0], table[2, 4] = -1, pages.shape[0], -2 ** 31, 2 ** 31 - 1
+    verify(hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new)), q, pages, table, lens, cu)
+    lens = [table.shape[1] * 32 + 77, 200, 2 ** 31 - 1]                     # past the table: what it holds is there
+    table[2, 5:] = 2 ** 30
+    verify(hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new)), q, pages, table, lens, cu)
+    out = hq.paged_attention(q, pages, torch.full_like(table, -1), ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    assert (out == 0).all()                                                 # no key at all
+    out = hq.paged_attention(q, pages, table, ints([0, -5, 0]), cu_q=ints(cu), max_q_len=max(new))
+    assert (out == 0).all()
+    out = hq.paged_attention(q, pages, table[:, :0], ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [30, 90]])
+def test_strides_and_rows_behind_the_last_token(new):
+    lens = [250, 131]
+    q, pages, table, cu = make(lens, new, 8, 2, 64, torch.float16, seed=31, behind=5)
+    T = q.shape[0]
+    fused = torch.zeros(T, 12, 160, dtype=q.dtype, device=DEV)
+    fused[:, 2:10, 8:136] = q
+    room = torch.full((T, 9, 136), 7.0, dtype=q.dtype, device=DEV)
+    got = hq.paged_attention(fused[:, 2:10, 8:136], pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new), out=room[:, :8, :128])
+    verify(got, q, pages, table, lens, cu)
+    assert (room[cu[-1]:] == 7).all() and (room[:, 8] == 7).all() and (room[..., 128:] == 7).all()
+    odd = torch.zeros(T, 8, 129, dtype=q.dtype, device=DEV)                  # rows that need a copy
+    odd[..., 1:] = q
+    wide = torch.zeros(2, 40, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    again = hq.paged_attention(odd[..., 1:], pages, wide[:, :table.shape[1]], ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    assert torch.equal(again[:cu[-1]], got[:cu[-1]])
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 3, 2], [90, 3, 200]])
+def test_starts_that_are_no_starts(new):
+    """Row offsets outside q or that fall: nothing outside is read or written, requests that fit are right."""
+    lens = [250, 131, 300]
+    q, pages, table, cu = make(lens, new, 8, 2, 64, torch.bfloat16, seed=33)
+    room = torch.full((q.shape[0] + 2, 8, 128), 7.0, dtype=q.dtype, device=DEV)
+    for bad in ([-5, 1, 0, 10 ** 9], [3, 2, 1, 0], [2 ** 31 - 1] * 4, [-2 ** 31, 2 ** 31 - 1, 0, 1]):
+        hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(bad), max_q_len=max(new), out=room[1:-1])
+    assert (room[0] == 7).all() and (room[-1] == 7).all()
+
+
+def test_offsets_past_32_bits():
+    """A pool of 6 GB whose last pages are the ones in use."""
+    page, H = 128, 8
+    num = 6 * 2 ** 30 // (H * page // 16 * 2112)
+    pages = torch.empty(num, H, page // 16, 2112, dtype=torch.uint8, device=DEV)
+    L = 300
+    table = ints([[num - 1, num - 3, num - 2], [0, num // 2, num - 4]])
+    g = torch.Generator(DEV).manual_seed(6)
+    k, v = (torch.randn(2 * L, H, 128, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    j = torch.arange(L, device=DEV)
+    slots = torch.cat([table[r, j // page].long() * page + j % page for r in (0, 1)])
+    hq.paged_append(pages, k, v, slots)
+    for a, x in zip(hq.paged_read(pages, slots, torch.float32), (k, v)):
+        c, s = plain.quantise(x)
+        assert torch.equal(a.double(), c * s)
+    for new in ([1, 1], [20, 150]):
+        cu = [0, new[0], sum(new)]
+        q = torch.randn(cu[-1], 32, 128, generator=g, device=DEV).to(torch.bfloat16)
+        verify(hq.paged_attention(q, pages, table, ints([L, L]), cu_q=ints(cu), max_q_len=max(new)), q, pages, table, [L, L], cu)
+
+
+# ---------------------------------------------------------------------------------------------- as they are used together
+
+def test_other_streams_give_the_same():
+    lens, new = [3000, 200, 9000], [1, 1, 1]
+    q, pages, table, cu = make(lens, new, 32, 8, 64, torch.bfloat16, seed=41)
+    lens_t = ints(lens)
+    want = hq.paged_attention(q, pages, table, lens_t)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(hq.paged_attention(q, pages, table, lens_t))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def serve(cache, steps, kv_heads, heads, layers, seed, run):
+    """Drives `run(add, keep, k, v, q, max_q)` -> outputs per layer over a made-up life of requests, and checks every step."""
+    rng, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    R, T = cache.kv_lens.shape[0], 48
+    rows = [[None] * R for _ in range(layers)]                               # cached (k, v) per layer and request, as given
+    for step in range(steps):
+        lens = [0 if rows[0][r] is None else rows[0][r][0].shape[0] for r in range(R)]
+        keep = [0 if rng.random() < 0.15 else max(0, n - rng.choice([0, 0, 2])) for n in lens]
+        add, left = [], T
+        for r in range(R):
+            a = min(left, rng.choice([1, 1, 1, 0, 4, 20]) if step else rng.randint(0, 12))
+            left -= a
+            add.append(a)
+        k, v = (torch.randn(layers, T, kv_heads, 128, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+        q = torch.randn(layers, T, heads, 128, generator=g, device=DEV).to(torch.bfloat16)
+        got = run(ints(add), ints(keep), k, v, q)
+        cache.check()
+        at = 0
+        cu = [0]
+        for r in range(R):
+            for layer in range(layers):
+                old = rows[layer][r]
+                fresh = (k[layer, at:at + add[r]], v[layer, at:at + add[r]])
+                rows[layer][r] = fresh if old is None else tuple(torch.cat((o[:keep[r]], f)) for o, f in zip(old, fresh))
+            at += add[r]
+            cu.append(at)
+        # a cache of its own for the check: one page list per request, rows quantised by the plain form
+        for layer in range(layers):
+            lens = [rows[layer][r][0].shape[0] for r in range(R)]
+            assert cache.kv_lens.tolist() == lens
+            need = [-(-n // 16) for n in lens]
+            pages = torch.zeros(sum(need) + 1, kv_heads, 1, 2112, dtype=torch.uint8, device=DEV)
+            table = torch.zeros(R, max(need) + 1, dtype=torch.int32, device=DEV)
+            base = 0
+            for r in range(R):
+                table[r, :need[r]] = torch.arange(base, base + need[r], device=DEV)
+                if lens[r]:
+                    plain.store(pages, base * 16 + torch.arange(lens[r], device=DEV), *rows[layer][r])
+                base += need[r]
+            verify(got[layer], q[layer], pages, table, lens, cu)
+
+
+def test_cache_serves_requests_that_come_and_go():
+    cache = hq.PagedKVCache(2, 120, 2, max_requests=5, max_pages_per_request=40, page_size=16)
+
+    def run(add, keep, k, v, q):
+        cache.advance(add, keep=keep, max_tokens=48)
+        out = []
+        for layer in range(2):
+            cache.append(layer, k[layer], v[layer])
+            out.append(cache.attention(layer, q[layer], max_q_len=20))
+        return out
+    serve(cache, 12, 2, 8, 2, 5, run)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (4, 4)])
+def test_step_in_a_cuda_graph(heads, kv_heads):
+    """A whole step captured once, replayed with other lengths; eager calls of the same cache between the replays."""
+    cache = hq.PagedKVCache(2, 200, kv_heads, max_requests=6, max_pages_per_request=40, page_size=16)
+    add, keep = ints([0] * 6), ints([0] * 6)
+    k, v = (torch.zeros(2, 48, kv_heads, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = torch.zeros(2, 48, heads, 128, dtype=torch.bfloat16, device=DEV)
+    outs = []
+
+    def step():
+        outs.clear()
+        cache.advance(add, keep=keep, max_tokens=48)
+        for layer in range(2):
+            cache.append(layer, k[layer], v[layer])
+            outs.append(cache.attention(layer, q[layer], max_q_len=20))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()                                                              # nothing is added: a warm-up that changes nothing
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+
+    def run(add2, keep2, k2, v2, q2):
+        for a, b in ((add, add2), (keep, keep2), (k, k2), (v, v2), (q, q2)):
+            a.copy_(b)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        eager = hq.paged_attention(q[0], cache.pages[0], cache.page_table, cache.kv_lens, cu_q=cache.step.cu_q, max_q_len=20)
+        n = int(cache.step.cu_q[-1])
+        assert torch.equal(eager[:n], got[0][:n])
+        return got
+    serve(cache, 8, kv_heads, heads, 2, 6, run)
+
+
+def test_two_graphs_and_an_eager_call_at_once():
+    """Graphs of one cache replayed on streams of their own while eager calls run: none uses another's scratch."""
+    lens, new = [20000, 300, 9000, 40], [1, 1, 1, 1]
+    q, pages, table, cu = make(lens, new, 32, 2, 64, torch.bfloat16, seed=43)
+    lens_t, cu3 = ints(lens), ints([0, 3, 6, 9, 12])
+    q3 = q.repeat_interleave(3, 0).contiguous()
+    want, want3 = hq.paged_attention(q, pages, table, lens_t), hq.paged_attention(q3, pages, table, lens_t, cu_q=cu3, max_q_len=40)
+    graphs, outs = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append((hq.paged_attention(q, pages, table, lens_t), hq.paged_attention(q3, pages, table, lens_t, cu_q=cu3, max_q_len=40)))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        again = hq.paged_attention(q, pages, table, lens_t), hq.paged_attention(q3, pages, table, lens_t, cu_q=cu3, max_q_len=40)
+    torch.cuda.synchronize()
+    for a, b in (*outs, again):
+        assert torch.equal(a, want) and torch.equal(b, want3)

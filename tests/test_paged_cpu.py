@@ -1,0 +1,127 @@
+"""The paged cache's checks of arguments, and its entry points in the C ABI; nothing here reaches a GPU."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import hyquant_b200 as hq
+from hyquant_b200 import _lib
+from hyquant_b200 import paged_kv
+
+FAKE = 1 << 20
+
+
+def attention_args(**fields):
+    """Arguments that pass every check; the addresses are made up.  T is 0: a call that passes returns before a launch."""
+    a = _lib.PagedAttentionArgs()
+    a.struct_bytes = C.sizeof(a)
+    a.R, a.T, a.H_Q, a.H_KV, a.head_dim, a.page_size, a.max_pages, a.max_q_len = 2, 5, 8, 2, 128, 64, 10, 4
+    a.dtype, a.sm_scale, a.num_pages = _lib.HQ_BF16, 0.1, 20
+    for name in ("q", "pages", "page_table", "kv_lens", "cu_q", "out", "workspace"):
+        setattr(a, name, FAKE)
+    a.q_st = a.o_st = 1024
+    a.q_sh = a.o_sh = 128
+    a.table_stride, a.workspace_bytes = 10, 1 << 40
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("fields,code,text", [
+    (dict(struct_bytes=8), -1, b"struct_bytes"), (dict(R=-1), -1, b"size"), (dict(T=-1), -1, b"size"), (dict(H_Q=0), -1, b"size"),
+    (dict(H_KV=0), -1, b"size"), (dict(max_q_len=0), -1, b"size"), (dict(num_pages=-1), -1, b"size"), (dict(max_pages=-1), -1, b"size"),
+    (dict(head_dim=64), -2, b"head_dim"), (dict(H_Q=9), -2, b"heads"), (dict(H_Q=34), -2, b"heads"), (dict(page_size=48), -2, b"page_size"),
+    (dict(page_size=256), -2, b"page_size"), (dict(max_pages=1 << 28, table_stride=1 << 28), -2, b"tables"), (dict(dtype=2), -2, b"dtype"),
+    (dict(sm_scale=-1.0), -1, b"sm_scale"), (dict(sm_scale=float("nan")), -1, b"sm_scale"), (dict(sm_scale=float("inf")), -1, b"sm_scale"),
+    (dict(cu_q=None), -1, b"cu_q"), (dict(q=None), -1, b"null"), (dict(out=None), -1, b"null"), (dict(kv_lens=None), -1, b"null"),
+    (dict(page_table=None), -1, b"null"), (dict(pages=None), -1, b"null"), (dict(table_stride=9), -1, b"overlap"),
+    (dict(q=FAKE + 8), -3, b"aligned"), (dict(out=FAKE + 2), -3, b"aligned"), (dict(pages=FAKE + 4), -3, b"aligned"),
+    (dict(q_st=1028), -3, b"aligned"), (dict(o_sh=129), -3, b"aligned"),
+])
+def test_attention_refusals(fields, code, text):
+    lib, n = _lib.lib(), C.c_int64()
+    a = attention_args(**fields)
+    assert lib.hq_paged_attention(C.byref(a), None) == code and text in lib.hq_last_error()
+    assert lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n)) == code
+
+
+def test_attention_null_block_and_nothing_to_do():
+    lib, n = _lib.lib(), C.c_int64(-1)
+    assert lib.hq_paged_attention(None, None) == -1
+    assert lib.hq_paged_attention_workspace_bytes(None, C.byref(n)) == -1
+    assert lib.hq_paged_attention_workspace_bytes(C.byref(attention_args()), None) == -1
+    for fields in (dict(T=0), dict(R=0), dict(T=0, q=None, out=None, pages=None)):
+        assert lib.hq_paged_attention(C.byref(attention_args(**fields)), None) == 0
+    assert lib.hq_paged_attention_workspace_bytes(C.byref(attention_args()), C.byref(n)) == 0 and n.value >= 0
+
+
+def advance(**fields):
+    a = dict(kv_lens=FAKE, held=FAKE, add=FAKE, keep=None, R=3, table=FAKE, stride=10, max_pages=10, free=FAKE, cap=9, count=FAKE, page=16, T=4,
+             lens2=FAKE, held2=FAKE, count2=FAKE, cu=FAKE, slots=FAKE, pos=FAKE, status=FAKE)
+    a.update(fields)
+    return _lib.lib().hq_page_advance(*a.values(), None)
+
+
+@pytest.mark.parametrize("fields,code", [
+    (dict(R=-1), -1), (dict(T=-1), -1), (dict(cap=-1), -1), (dict(max_pages=-1), -1), (dict(R=8193), -2), (dict(page=8), -2), (dict(page=0), -2),
+    (dict(kv_lens=None), -1), (dict(add=None), -1), (dict(slots=None), -1), (dict(cu=None), -1), (dict(status=None), -1), (dict(table=None), -1),
+    (dict(free=None), -1), (dict(stride=9), -1), (dict(R=8192, max_pages=1 << 20, stride=1 << 20), -2)])
+def test_advance_refusals(fields, code):
+    assert advance(**fields) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(T=-1), -1), (dict(H=0), -1), (dict(page=17), -2), (dict(dtype=3), -2), (dict(k=None), -1), (dict(slots=None), -1), (dict(pages=None), -1),
+    (dict(k=FAKE + 8), -3), (dict(k_st=1020), -3), (dict(v_sh=4), -3), (dict(pages=FAKE + 8), -3), (dict(slots=FAKE + 4), -3), (dict(T=1 << 30, H=2), -2)])
+def test_append_refusals(change, code):
+    a = dict(k=FAKE, v=FAKE, dtype=0, k_st=1024, k_sh=128, v_st=1024, v_sh=128, T=4, H=8, slots=FAKE, pages=FAKE, num=10, page=64)
+    a.update(change)
+    assert _lib.lib().hq_paged_append(*a.values(), None) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(T=-1), -1), (dict(H=0), -1), (dict(page=0), -2), (dict(dtype=-1), -2), (dict(k=None), -1), (dict(v=FAKE + 2), -3), (dict(slots=None), -1),
+    (dict(num=-1), -1)])
+def test_read_refusals(change, code):
+    a = dict(pages=FAKE, num=10, page=64, slots=FAKE, T=4, H=8, dtype=0, k=FAKE, v=FAKE)
+    a.update(change)
+    assert _lib.lib().hq_paged_read(*a.values(), None) == code
+
+
+def test_nothing_to_do_touches_nothing():
+    lib = _lib.lib()
+    assert lib.hq_paged_append(None, None, 0, 0, 0, 0, 0, 0, 8, None, None, 10, 64, None) == 0
+    assert lib.hq_paged_append(FAKE, FAKE, 0, 1024, 128, 1024, 128, 4, 8, FAKE, None, 0, 64, None) == 0
+    assert lib.hq_paged_read(None, 10, 64, None, 0, 8, 0, None, None, None) == 0
+
+
+def test_python_refusals():
+    with pytest.raises(ValueError):
+        hq.paged_pages(4, 2, 48, device="cpu")
+    pages = hq.paged_pages(4, 2, 64, device="cpu")
+    assert pages.shape == (4, 2, 4, 2112) and pages.dtype == torch.uint8
+    i32 = torch.zeros(1, dtype=torch.int32)
+    x = torch.zeros(1, 2, 128)
+    with pytest.raises(hq.HyQuantError):                                    # no CPU path
+        hq.paged_attention(torch.zeros(1, 4, 128, dtype=torch.bfloat16), pages, torch.zeros(1, 4, dtype=torch.int32), i32)
+    with pytest.raises(hq.HyQuantError):
+        hq.paged_append(pages, x, x, torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(hq.HyQuantError):
+        hq.paged_read(pages, torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(hq.HyQuantError):
+        hq.page_advance(i32, i32, i32, torch.zeros(1, 4, dtype=torch.int32), i32, i32, page_size=64, max_tokens=1)
+    with pytest.raises(ValueError):
+        hq.PagedKVCache(0, 4, 2, max_requests=1, max_pages_per_request=4, device="cpu")
+    with pytest.raises(ValueError):
+        hq.PagedKVCache(1, 4, 2, max_requests=1, max_pages_per_request=4, page_size=20, device="cpu")
+    cache = hq.PagedKVCache(3, 4, 2, max_requests=2, max_pages_per_request=4, device="cpu")
+    assert len(cache) == 3 and cache.free_pages.tolist() == [3, 2, 1, 0] and int(cache.free_count) == 4
+    cache.check()                                                           # no step yet: nothing to report
+    with pytest.raises(hq.HyQuantError):
+        cache.append(0, x, x)
+
+
+def test_format_constants():
+    assert paged_kv.BLOCK_BYTES == 2 * paged_kv.BLOCK * 64 + 2 * paged_kv.BLOCK * 2
+    assert [f[0] for f in _lib.PagedAttentionArgs._fields_][-2:] == ["workspace", "workspace_bytes"] and C.sizeof(_lib.PagedAttentionArgs) == 160
