@@ -23,6 +23,22 @@ constexpr int kBlockBytes = HQ_PAGED_BLOCK_BYTES;
 constexpr int kVOff = kTok * 64, kKsOff = 2 * kTok * 64, kVsOff = kKsOff + 2 * kTok;
 static_assert(kVsOff + 2 * kTok == kBlockBytes && kBlockBytes % 16 == 0, "block layout");
 
+struct AttnParams {
+  int R, T, H_Q, H_KV, G, page_shift, max_pages, max_q_len;
+  float sml;                                   // sm_scale * log2(e)
+  int dtype;
+  int64_t num_pages;
+  const void* q; int64_t q_st, q_sh;
+  const uint8_t* pages;
+  const int* table; int64_t table_stride;
+  const int* kv_lens; const int* cu_q;
+  void* out; int64_t o_st, o_sh;
+  float* ws;
+};
+
+int64_t decode_workspace(const AttnParams& p);                 // bytes; hq_paged_decode.cu
+int decode_launch(const AttnParams& p, cudaStream_t st);
+
 inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
 
 #if defined(__CUDACC__)
@@ -79,6 +95,23 @@ __device__ __forceinline__ float quant_row(const float (&v)[16], uint32_t (&code
     }
   }
   return s;
+}
+
+// Request r of a call: its first row of q, its rows, its cached tokens, and those before its first new one.  Starts outside q and
+// lengths past the table are cut, so that no address is formed from them.
+struct Request { int q0, nq, len, past; };
+__device__ __forceinline__ Request request_of(const AttnParams& p, int r) {
+  Request x;
+  int n = 1;
+  x.q0 = r;
+  if (p.cu_q) {
+    x.q0 = min(max(__ldg(p.cu_q + r), 0), p.T);
+    n = max(min(max(__ldg(p.cu_q + r + 1), 0), p.T) - x.q0, 0);
+  }
+  x.nq = min(n, p.max_q_len);
+  x.len = max(0, min(__ldg(p.kv_lens + r), p.max_pages << p.page_shift));
+  x.past = x.len - n;
+  return x;
 }
 
 // first byte of the sixteen-token block of `slot` (page * page_size + position in the page) of head `h`

@@ -4,28 +4,15 @@
 namespace hq {
 namespace paged {
 
-struct AttnParams {
-  int R, T, H_Q, H_KV, G, page_shift, max_pages, max_q_len;
-  float sml;                                   // sm_scale * log2(e)
-  int64_t num_pages;
-  const void* q; int64_t q_st, q_sh;
-  const uint8_t* pages;
-  const int* table; int64_t table_stride;
-  const int* kv_lens; const int* cu_q;
-  void* out; int64_t o_st, o_sh;
-  int dtype;
-};
-
 // One block per new token and kv head; 128 threads.  Keys in tiles of 32: four threads a key for the scores, then a thread per
 // channel for the values.
 __global__ void __launch_bounds__(128)
 attn_simple_kernel(const AttnParams p) {
   __shared__ float sq[16][128], sp[16][32], smx[16], sl[16], sal[16];
   const int r = blockIdx.z, h = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
-  const int q0 = p.cu_q ? min(max(p.cu_q[r], 0), p.T) : r, q1 = p.cu_q ? min(max(p.cu_q[r + 1], 0), p.T) : r + 1;
-  if (i >= q1 - q0) return;
-  const int64_t cap = (int64_t)p.max_pages << p.page_shift;
-  const int n_keys = (int)max((int64_t)0, min((int64_t)p.kv_lens[r], cap) - (q1 - q0) + i + 1);
+  const Request rq = request_of(p, r);
+  if (i >= rq.nq) return;
+  const int q0 = rq.q0, n_keys = max(0, min(rq.len, rq.past + i + 1));
   const int t = q0 + i, G = p.G;
   for (int x = tid; x < G * 128; x += 128) {
     const int64_t at = t * p.q_st + (h * G + x / 128) * p.q_sh + x % 128;
@@ -107,6 +94,7 @@ static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a->dtype == HQ_BF16 || a->dtype == HQ_F16, HQ_ERR_UNSUPPORTED, "hq_paged_attention: dtype %d (bf16 and fp16 are built)", a->dtype);
   HQ_REQUIRE(a->sm_scale >= 0.f && a->sm_scale < 1e30f, HQ_ERR_INVALID, "hq_paged_attention: sm_scale must be finite and not negative");
   HQ_REQUIRE(a->cu_q || (a->R == a->T && a->max_q_len == 1), HQ_ERR_INVALID, "hq_paged_attention: without cu_q every request has one token");
+  HQ_REQUIRE((int64_t)a->R * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %d requests of %d kv heads", a->R, a->H_KV);
   if (a->R == 0 || a->T == 0) return HQ_OK;
   HQ_REQUIRE(a->q && a->out && a->kv_lens && (a->page_table || a->max_pages == 0) && (a->pages || a->num_pages == 0), HQ_ERR_INVALID,
              "hq_paged_attention: null pointer");
@@ -117,6 +105,20 @@ static int check(const hq_paged_attention_args* a) {
   return HQ_OK;
 }
 
+static AttnParams params_of(const hq_paged_attention_args* a) {
+  AttnParams p{};
+  p.R = a->R; p.T = a->T; p.H_Q = a->H_Q; p.H_KV = a->H_KV; p.G = a->H_Q / a->H_KV;
+  p.page_shift = shift_of(a->page_size); p.max_pages = a->max_pages; p.max_q_len = a->max_q_len;
+  p.sml = a->sm_scale * 1.44269504f;
+  p.num_pages = a->num_pages;
+  p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh; p.pages = (const uint8_t*)a->pages;
+  p.table = a->page_table; p.table_stride = a->table_stride; p.kv_lens = a->kv_lens; p.cu_q = a->cu_q;
+  p.ws = (float*)a->workspace;
+  p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh; p.dtype = a->dtype;
+  return p;
+}
+static bool few_rows(const AttnParams& p) { return (int64_t)p.max_q_len * p.G <= 16; }
+
 }  // namespace paged
 }  // namespace hq
 
@@ -124,7 +126,8 @@ extern "C" int hq_paged_attention_workspace_bytes(const hq_paged_attention_args*
   using namespace hq;
   if (int rc = paged::check(a)) return rc;
   HQ_REQUIRE(bytes, HQ_ERR_INVALID, "hq_paged_attention_workspace_bytes: null pointer");
-  *bytes = 0;
+  const paged::AttnParams p = paged::params_of(a);
+  *bytes = paged::few_rows(p) && a->R > 0 && a->T > 0 ? paged::decode_workspace(p) : 0;
   return HQ_OK;
 }
 
@@ -133,14 +136,13 @@ extern "C" int hq_paged_attention(const hq_paged_attention_args* a, void* stream
   using namespace hq::paged;
   if (int rc = check(a)) return rc;
   if (a->R == 0 || a->T == 0) return HQ_OK;
-  AttnParams p{};
-  p.R = a->R; p.T = a->T; p.H_Q = a->H_Q; p.H_KV = a->H_KV; p.G = a->H_Q / a->H_KV;
-  p.page_shift = shift_of(a->page_size); p.max_pages = a->max_pages; p.max_q_len = a->max_q_len;
-  p.sml = a->sm_scale * 1.44269504f;
-  p.num_pages = a->num_pages;
-  p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh; p.pages = (const uint8_t*)a->pages;
-  p.table = a->page_table; p.table_stride = a->table_stride; p.kv_lens = a->kv_lens; p.cu_q = a->cu_q;
-  p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh; p.dtype = a->dtype;
+  const AttnParams p = params_of(a);
+  if (few_rows(p)) {
+    HQ_REQUIRE(a->workspace && a->workspace_bytes >= decode_workspace(p), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
+               (long long)a->workspace_bytes, (long long)decode_workspace(p));
+    HQ_REQUIRE(aligned16(a->workspace), HQ_ERR_ALIGNMENT, "hq_paged_attention: the workspace must be 16-byte aligned");
+    return decode_launch(p, (cudaStream_t)stream);
+  }
   HQ_REQUIRE(a->R <= 65535 && a->H_KV <= 65535, HQ_ERR_UNSUPPORTED, "hq_paged_attention: too many requests");
   attn_simple_kernel<<<dim3(a->max_q_len, a->H_KV, a->R), 128, 0, (cudaStream_t)stream>>>(p);
   HQ_CUDA(cudaGetLastError());

@@ -1,0 +1,594 @@
+// Attention of a few new tokens per request over the paged 4-bit cache: calls whose new tokens times query heads per kv head
+// fit 16 rows (one token at every group size, drafts of a few).
+//
+// HBM-bound: 132 bytes a cached token and kv head, read once; at 6.5 TB/s an SM has some 100 clocks for 32 tokens.
+//
+// Work split.  A kv head of a request is a run of units of 32 tokens and one closing unit, so that heads without tokens cost
+// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one of 16 warps per SM, and a block's
+// part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
+// barrier inside, and a run that lies within one warp's part is written out by that warp.  Runs that several warps share are
+// merged through shared memory at the block's end, runs that several blocks share by the merge kernel.  Everything goes by
+// position, nothing by arrival: results do not depend on timing, and no counter has to be zero beforehand.
+//
+// Per warp a ring of three units in shared memory, each one bulk copy (two for pages of sixteen tokens).  Products on mma.sync
+// m16n8k16 in fp16: S^T = K Q^T, tokens on M and the rows (token, head of the group) on N, then O^T = V^T P^T.  Codes enter as fp16
+// subnormals (one logic operation for two of them): the nibble + 8 as mantissa bits is (code + 8) 2^-24, or 2^-20 for a nibble four
+// bits up.  The power of two goes into the query operand and the epilogue, the 8 into the accumulators' start (K) and the row sum
+// of P (V, one more product against ones).  Queries are scaled by a power of two of their own so that fp16 holds them
+// exactly.  P v_scale is rounded to fp16, 11 bits against bf16's 8: relative to the largest v_scale so far, whose power of two moves like
+// the maximum does.
+#include "hq_paged.cuh"
+
+namespace hq {
+namespace paged {
+
+constexpr int kUnit = 32, kUnitBytes = 2 * kBlockBytes, kSlots = 3;
+constexpr int kRowPad = 132;                    // floats of a row of a piece
+constexpr float kLazy = 4.0f;                   // the reference moves when a score passes it by 2^4
+constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9) <= 2^13: fp16's range above and below is used
+__host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 16 : 12; }
+__host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// nibbles 0..3 of each 16-bit half as fp16 subnormals: (code + 8) 2^-24 for 0 and 2, 2^-20 for 1 and 3
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&h)[4]) {
+  const uint32_t w8 = w >> 8;
+  h[0] = lop3_and_xor(w, 0x000F000Fu, 0x00080008u);
+  h[1] = lop3_and_xor(w, 0x00F000F0u, 0x00800080u);
+  h[2] = lop3_and_xor(w8, 0x000F000Fu, 0x00080008u);
+  h[3] = lop3_and_xor(w8, 0x00F000F0u, 0x00800080u);
+}
+__device__ __forceinline__ float over_g(float v, bool max) {      // over the eight lanes with the same lane % 4
+#pragma unroll
+  for (int o = 4; o <= 16; o <<= 1) {
+    const float x = __shfl_xor_sync(0xffffffffu, v, o);
+    v = max ? fmaxf(v, x) : v + x;
+  }
+  return v;
+}
+__device__ __forceinline__ float bf16_bits(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+
+// A place in the row of runs.  pos = first + u; u == units is the closing unit.
+struct Walk {
+  int r, h, u, units;
+  Request q;
+};
+__device__ __forceinline__ int units_of(const Request& x) { return x.nq > 0 ? (x.len + kUnit - 1) / kUnit : -1; }     // -1: no run at all
+__device__ __forceinline__ void next_run(const AttnParams& p, Walk& w) {
+  w.u = 0;
+  if (++w.h < p.H_KV) return;
+  w.h = 0;
+  do {
+    if (++w.r >= p.R) return;
+    w.q = request_of(p, w.r);
+    w.units = units_of(w.q);
+  } while (w.units < 0);
+}
+
+// Workspace: pieces of runs that begin before a warp's part and end in it; two pieces per block; what the merge kernel has to
+// do for each block.
+struct Merge { int q0, nq, h, first, go, unused[3]; };
+template <int NT> __host__ __device__ inline int64_t ws_block_pieces(int blocks) { return (int64_t)blocks * warps_of(NT) * piece_floats(NT); }
+template <int NT> __host__ __device__ inline int64_t ws_merge(int blocks) { return ws_block_pieces<NT>(blocks) + (int64_t)blocks * 2 * piece_floats(NT); }
+
+__device__ __forceinline__ void store_row4(const AttnParams& p, int64_t at, float4 v, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;                // a row that saw no key: 0
+  v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+  uint2 o;
+  if (p.dtype == HQ_BF16) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    o = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  } else {
+    __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    o = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = o;
+}
+__device__ __forceinline__ int64_t out_row(const AttnParams& p, const Request& q, int h, int n) {
+  return (int64_t)(q.q0 + n / p.G) * p.o_st + (int64_t)(h * p.G + n % p.G) * p.o_sh;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(warps_of(NT) * 32, 1)
+decode_kernel(const AttnParams p) {
+  constexpr int kWarps = warps_of(NT), kThreads = kWarps * 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t bars[kWarps * kSlots];
+  __shared__ int s_live[kWarps * kSlots];                    // which of a unit's two blocks lie in the pool
+  __shared__ long long s_part[kThreads + 1], s_warp[kWarps];
+  __shared__ int s_seg[32], s_q0[32], s_nq[32];              // run (r * H_KV + h) of a warp's first and last piece, or -1; its request
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  if (tid < kWarps * kSlots) { mbar_init(bars + tid, 1); fence_mbar_init(); }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- where this warp's part lies
+  const int per = (p.R + kThreads - 1) / kThreads;
+  long long mine = 0;
+  for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += (long long)p.H_KV * (units_of(request_of(p, r)) + 1);
+  long long x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kWarps; ++w) { if (w < warp) before += s_warp[w]; total += s_warp[w]; }
+  s_part[tid + 1] = before + x;
+  if (tid == 0) s_part[0] = 0;
+  __syncthreads();
+  // a block has at least one unit for every warp: fewer blocks take part in short calls
+  const int blocks = (int)max(1ll, min((long long)gridDim.x, total / kWarps)), block = blockIdx.x;
+  Merge* todo = reinterpret_cast<Merge*>(p.ws + ws_merge<NT>(gridDim.x)) + block;
+  if (block >= blocks) { if (tid == 0) todo->go = 0; return; }
+  const long long b0 = total * block / blocks, b1 = total * (block + 1) / blocks;
+  const long long w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
+  int left = (int)(w1 - w0);
+  // the run at position w0
+  Walk c{0, 0, 0, -1, Request{0, 0, 0, 0}};
+  auto locate = [&](long long pos, Walk& w) {
+    int lo = 0, hi = kThreads;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= pos) lo = mid; else hi = mid; }
+    long long at = s_part[lo];
+    w.r = lo * per;
+    for (;; ++w.r) {
+      w.q = request_of(p, w.r);
+      w.units = units_of(w.q);
+      const long long n = (long long)p.H_KV * (w.units + 1);
+      if (pos < at + n) break;
+      at += n;
+    }
+    const int in = (int)((pos - at) / (w.units + 1));
+    w.h = in;
+    w.u = (int)(pos - at - (long long)in * (w.units + 1));
+  };
+  if (left > 0) locate(w0, c);
+  const int start_u = c.u;                                   // the part begins inside a run if start_u > 0
+
+  // ---- the ring
+  uint8_t* ring = smem + warp * (kSlots * kUnitBytes);
+  uint64_t* bar = bars + warp * kSlots;
+  int* live = s_live + warp * kSlots;
+  Walk f = c;                                                // the unit that is fetched next
+  int f_left = left, f_slot = 0;
+  int tab_r = -1, tab_u = 0, pg0 = -1, pg1 = -1;             // pages of 32 units of request tab_r, a unit per lane
+  auto fetch = [&]() {                                       // the next unit that is there; all lanes
+    while (f_left > 0 && f.u >= f.units) { --f_left; next_run(p, f); }
+    if (f_left <= 0) return;
+    if (f.r != tab_r || f.u - tab_u >= 32 || f.u < tab_u) {
+      tab_r = f.r; tab_u = f.u;
+      const int64_t tok = ((int64_t)tab_u + lane) * kUnit;
+      const int* row = p.table + (int64_t)f.r * p.table_stride;
+      pg0 = tok < f.q.len ? __ldg(row + (tok >> p.page_shift)) : -1;
+      pg1 = tok + kTok < f.q.len ? __ldg(row + ((tok + kTok) >> p.page_shift)) : -1;
+    }
+    const int a = __shfl_sync(0xffffffffu, pg0, f.u - tab_u), b = __shfl_sync(0xffffffffu, pg1, f.u - tab_u);
+    if (lane == 0) {
+      const int64_t tok = (int64_t)f.u * kUnit, in = tok & ((1 << p.page_shift) - 1);
+      const bool la = a >= 0 && a < p.num_pages, lb = b >= 0 && b < p.num_pages;
+      live[f_slot] = (la ? 1 : 0) | (lb ? 2 : 0);
+      uint8_t* dst = ring + f_slot * kUnitBytes;
+      mbar_expect_tx(bar + f_slot, ((la ? 1 : 0) + (lb ? 1 : 0)) * kBlockBytes);
+      const uint8_t* src = p.pages + block_offset(((int64_t)a << p.page_shift) + in, f.h, p.H_KV, p.page_shift);
+      if (la && lb && p.page_shift > 4) bulk_g2s(dst, src, kUnitBytes, bar + f_slot);
+      else {
+        if (la) bulk_g2s(dst, src, kBlockBytes, bar + f_slot);
+        if (lb) bulk_g2s(dst + kBlockBytes, p.page_shift > 4 ? src + kBlockBytes
+                                                              : p.pages + block_offset((int64_t)b << p.page_shift, f.h, p.H_KV, p.page_shift),
+                         kBlockBytes, bar + f_slot);
+      }
+    }
+    if (++f_slot == kSlots) f_slot = 0;
+    ++f.u; --f_left;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kSlots; ++i) fetch();
+
+  // ---- the state of the run in hand
+  uint32_t qf[NT][16];                                       // query operand: word w, nibble k at 4 w + k
+  float2 fac[NT], start[NT];                                 // factor of a score, start of the accumulators: columns 2 t4, 2 t4 + 1
+  float2 m[NT], l[NT];
+  float O[NT][8][4], Ls[NT][4];
+  int vexp = 0;                                              // V scales are taken relative to 2^vexp
+  int lim0 = 0;                                              // keys that the run's first token sees
+  int lim[NT][2];
+  auto open = [&]() {
+    const int rows = c.q.nq * p.G;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int n = 8 * nt + g;
+      uint4 raw[4];
+      const bool there = n < rows;
+      const int64_t at = (int64_t)(c.q.q0 + n / p.G) * p.q_st + (int64_t)(c.h * p.G + n % p.G) * p.q_sh + 32 * t4;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        raw[w] = there ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at) + w) : make_uint4(0u, 0u, 0u, 0u);
+      float top = 0.f;
+      auto value = [&](int w, int i) {                       // channel 32 t4 + 8 w + i
+        const uint32_t u = i < 2 ? raw[w].x : i < 4 ? raw[w].y : i < 6 ? raw[w].z : raw[w].w;
+        if (p.dtype == HQ_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half((unsigned short)(i & 1 ? u >> 16 : u & 0xFFFFu)));
+      };
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(value(w, i)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the largest magnitude to [2^13, 2^14): below it fp16 has 37 bits
+      const int ex = (int)(__float_as_uint(top) >> 23);      // 0: zero or below the normal numbers, 255: infinite
+      const int up = ex == 255 ? 0 : 140 - max(ex, 14);      // at most 2^126, a normal number
+      const float scale = __uint_as_float((uint32_t)(127 + up) << 23);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float s = k & 1 ? scale * 0.0625f : scale;
+          const __half2 hh = __floats2half2_rn(value(w, k) * s, value(w, k + 4) * s);
+          qf[nt][4 * w + k] = *reinterpret_cast<const uint32_t*>(&hh);
+          const float2 back = __half22float2(hh);
+          sum += (back.x + back.y) * (k & 1 ? 16.f : 1.f);
+        }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float back = p.sml * __uint_as_float((uint32_t)min(127 + 24 - up, 255) << 23);       // sml 2^24 / scale
+      const float first = -8.f * 0x1p-24f * sum;
+      fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
+      start[nt] = make_float2(__shfl_sync(0xffffffffu, first, 8 * t4), __shfl_sync(0xffffffffu, first, 8 * t4 + 4));
+      m[nt] = make_float2(-INFINITY, -INFINITY);
+      l[nt] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) lim[nt][j] = c.q.past + 1 + min((8 * nt + 2 * t4 + j) / p.G, c.q.nq - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ls[nt][i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[nt][mt][i] = 0.f;
+    }
+    lim0 = c.q.past + 1;
+    vexp = -1000;
+  };
+  // what the row is at the end: the 8 of the codes taken off, the powers of two put back
+  auto close = [&](auto&& row) {
+    const float back = vexp == -1000 ? 0.f : ldexpf(1.f, vexp);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float ls[2] = {over_g(l[nt].x, false), over_g(l[nt].y, false)};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float4 v[4];
+        const float eight = 8.f * Ls[nt][j];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          v[q4].x = (O[nt][2 * q4][j] * 0x1p24f - eight) * back;
+          v[q4].y = (O[nt][2 * q4 + 1][j] * 0x1p20f - eight) * back;
+          v[q4].z = (O[nt][2 * q4][2 + j] * 0x1p24f - eight) * back;
+          v[q4].w = (O[nt][2 * q4 + 1][2 + j] * 0x1p20f - eight) * back;
+        }
+        row(8 * nt + 2 * t4 + j, v, j ? m[nt].y : m[nt].x, ls[j]);
+      }
+    }
+  };
+  auto to_piece = [&](float* piece) {
+    close([&](int n, const float4 (&v)[4], float mm, float ll) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = v[q4];
+      if (g == 0) { piece[8 * NT * kRowPad + n] = mm; piece[8 * NT * kRowPad + 8 * NT + n] = ll; }
+    });
+  };
+  auto to_out = [&]() {
+    const int rows = c.q.nq * p.G;
+    close([&](int n, const float4 (&v)[4], float, float ll) {
+      if (n < rows) {
+        const int64_t at = out_row(p, c.q, c.h, n) + 16 * g;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) store_row4(p, at + 4 * q4, v[q4], ll);
+      }
+    });
+  };
+
+  int slot = 0;
+  uint32_t parity = 0;
+  const int tau = (g >> 1) + 4 * (g & 1);                    // token of score row g (and + 8): the four tokens of a V fragment's
+                                                             // load are neighbours then, on both halves of the banks
+  auto unit = [&]() {
+    const bool ok = mbar_wait_bounded(bar + slot, parity);
+    const uint8_t* u0 = ring + slot * kUnitBytes;
+    const int there = live[slot];
+    float S[NT][2][4];
+    float ks[2][2], vs[2][2];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const uint8_t* b = u0 + cb * kBlockBytes;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) { S[nt][cb][0] = S[nt][cb][2] = start[nt].x; S[nt][cb][1] = S[nt][cb][3] = start[nt].y; }
+      const uint4 ka = *reinterpret_cast<const uint4*>(b + tau * 64 + 16 * t4), kb = *reinterpret_cast<const uint4*>(b + (tau + 8) * 64 + 16 * t4);
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t ha[4], hb[4];
+        nibbles(wa[w], ha);
+        nibbles(wb[w], hb);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(S[nt][cb], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * w], qf[nt][4 * w + 1]);
+          mma16816(S[nt][cb], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * w + 2], qf[nt][4 * w + 3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ks[cb][i] = bf16_bits(*reinterpret_cast<const uint16_t*>(b + kKsOff + 2 * (tau + 8 * i)));
+        vs[cb][i] = bf16_bits(*reinterpret_cast<const uint16_t*>(b + kVsOff + 2 * (tau + 8 * i)));
+      }
+    }
+    // scores in powers of two
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float2 y = fmul2(make_float2(S[nt][cb][2 * i], S[nt][cb][2 * i + 1]), make_float2(ks[cb][i], ks[cb][i]));
+          y = fmul2(y, fac[nt]);
+          S[nt][cb][2 * i] = y.x; S[nt][cb][2 * i + 1] = y.y;
+        }
+    const int tok0 = c.u * kUnit;
+    if (__builtin_expect(tok0 + kUnit > lim0 || there != 3, 0)) {        // keys behind a row's last one, pages that are not there
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int tok = tok0 + 16 * cb + tau + 8 * i;
+          const bool here = (there >> cb) & 1;
+          if (!here || tok >= c.q.len) vs[cb][i] = 0.f;                  // what lies there may be anything, NaN too
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (!here || tok >= lim[nt][j]) S[nt][cb][2 * i + j] = -INFINITY;
+        }
+    }
+    // the references: the maximum of a row, the largest V scale
+    bool move = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float x0 = fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2]));
+      const float x1 = fmaxf(fmaxf(S[nt][0][1], S[nt][0][3]), fmaxf(S[nt][1][1], S[nt][1][3]));
+      move |= x0 > m[nt].x + kLazy || x1 > m[nt].y + kLazy;
+    }
+    const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
+    move |= (int)(__float_as_uint(vtop) >> 23) - 127 > vexp && vtop > 0.f;
+    if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
+      const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 127;
+      const int nv = max(vexp, e);
+      const float vscale = vexp == -1000 ? 0.f : ldexpf(1.f, max(vexp - nv, -200));
+      vexp = nv;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float x0 = over_g(fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2])), true);
+        const float x1 = over_g(fmaxf(fmaxf(S[nt][0][1], S[nt][0][3]), fmaxf(S[nt][1][1], S[nt][1][3])), true);
+        const float2 nm = make_float2(fmaxf(m[nt].x, x0), fmaxf(m[nt].y, x1));
+        const float2 al = make_float2(m[nt].x == -INFINITY ? 0.f : ex2f(m[nt].x - nm.x), m[nt].y == -INFINITY ? 0.f : ex2f(m[nt].y - nm.y));
+        m[nt] = nm;
+        l[nt] = fmul2(l[nt], al);
+        const float2 av = make_float2(al.x * vscale, al.y * vscale);
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) { O[nt][mt][0] *= av.x; O[nt][mt][1] *= av.y; O[nt][mt][2] *= av.x; O[nt][mt][3] *= av.y; }
+        Ls[nt][0] *= av.x; Ls[nt][1] *= av.y; Ls[nt][2] *= av.x; Ls[nt][3] *= av.y;
+      }
+    }
+    const float vback = __uint_as_float((uint32_t)(127 - max(vexp, -126)) << 23);        // 2^-vexp
+    uint32_t P[NT][2][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 nm = make_float2(m[nt].x == -INFINITY ? 0.f : kShift - m[nt].x, m[nt].y == -INFINITY ? 0.f : kShift - m[nt].y);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 y = fadd2(make_float2(S[nt][cb][2 * i], S[nt][cb][2 * i + 1]), nm);
+          const float2 e = make_float2(ex2f(y.x), ex2f(y.y));
+          l[nt] = fadd2(l[nt], e);
+          const float sv = vs[cb][i] * vback;
+          const float2 pv = fmul2(e, make_float2(sv, sv));
+          const __half2 hh = __floats2half2_rn(pv.x, pv.y);
+          P[nt][cb][i] = movmatrix(*reinterpret_cast<const uint32_t*>(&hh));
+        }
+    }
+    if (!ok) {                                               // a copy that never came: the rows are NaN
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l[nt] = make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000));
+    }
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const uint8_t* b = u0 + cb * kBlockBytes + kVOff + 8 * g;
+      const uint2 v0 = *reinterpret_cast<const uint2*>(b + t4 * 64), v1 = *reinterpret_cast<const uint2*>(b + (t4 + 4) * 64);
+      const uint2 v2 = *reinterpret_cast<const uint2*>(b + (t4 + 8) * 64), v3 = *reinterpret_cast<const uint2*>(b + (t4 + 12) * 64);
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {                       // channels 16 g + 4 q4 .. + 3: a 16-bit half of each token's word
+        const uint32_t sel = q4 & 1 ? 0x7632u : 0x5410u;
+        uint32_t ha[4], hb[4];
+        nibbles(prmt(q4 < 2 ? v0.x : v0.y, q4 < 2 ? v1.x : v1.y, sel), ha);
+        nibbles(prmt(q4 < 2 ? v2.x : v2.y, q4 < 2 ? v3.x : v3.y, sel), hb);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(O[nt][2 * q4], ha[0], ha[2], hb[0], hb[2], P[nt][cb][0], P[nt][cb][1]);
+          mma16816(O[nt][2 * q4 + 1], ha[1], ha[3], hb[1], hb[3], P[nt][cb][0], P[nt][cb][1]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816(Ls[nt], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, P[nt][cb][0], P[nt][cb][1]);
+    }
+    __syncwarp();
+    if (++slot == kSlots) { slot = 0; parity ^= 1u; }
+  };
+
+  float* first_piece = p.ws + (int64_t)(block * kWarps + warp) * piece_floats(NT);
+  if (tid < 32) s_seg[tid] = -1;
+  __syncthreads();
+  auto mark = [&](int i) {
+    if (lane == 0) { s_seg[2 * warp + i] = c.r * p.H_KV + c.h; s_q0[2 * warp + i] = c.q.q0; s_nq[2 * warp + i] = c.q.nq; }
+  };
+  bool inside = start_u > 0;                                 // the run in hand began before this part
+  if (left > 0) {
+    open();
+#pragma unroll 1
+    while (true) {
+      if (c.u < c.units) {
+        unit();
+        fetch();
+        ++c.u; --left;
+      } else {                                               // the run ends here
+        if (inside) { to_piece(first_piece); mark(0); }
+        else to_out();
+        inside = false;
+        --left;
+        if (left > 0) { next_run(p, c); open(); }
+        else { c.u = -1; }
+      }
+      if (left == 0) break;
+    }
+    if (c.u != -1) {                                         // and goes on in the next part: its piece into the ring, which is empty
+      to_piece(reinterpret_cast<float*>(ring));
+      mark(1);
+    }
+  }
+  if (tid == 0) todo->go = 0;
+  __syncthreads();
+
+  // ---- runs that several warps share: pieces in order are the warps' first and last ones, a lane each; neighbours of the same
+  // run are a group.  A warp takes a row of a group at a time.
+  const int seg = s_seg[lane];
+  const uint32_t valid = __ballot_sync(0xffffffffu, seg >= 0);
+  if (valid == 0) return;
+  const uint32_t below = valid & ((1u << lane) - 1u);
+  const int prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : 0);
+  const uint32_t heads = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0u || prev != seg));
+  const bool from_before = __shfl_sync(0xffffffffu, start_u, 0) > 0;      // of warp 0 only
+  __shared__ int s_before;
+  __shared__ long long s_start;
+  if (tid == 0) { s_before = from_before; s_start = b0 - start_u; }
+  __syncthreads();
+  int item = 0;
+  for (uint32_t rest = heads; rest; rest &= rest - 1) {
+    const int head = __ffs(rest) - 1;
+    const uint32_t later = rest & (rest - 1);
+    const uint32_t group = valid & ~((1u << head) - 1u) & (later ? (later & (0u - later)) - 1u : 0xffffffffu);
+    const int id = s_seg[head], q0 = s_q0[head], nq = s_nq[head], rows = nq * p.G, r = id / p.H_KV, h = id - r * p.H_KV;
+    const bool began_before = head == __ffs(valid) - 1 && s_before, ends = ((31 - __clz(group)) & 1) == 0;
+    float* to = p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block + (began_before ? 0 : 1)) * piece_floats(NT);
+    if (began_before && ends && tid == 0) {
+      int first = (int)(s_start * blocks / total);
+      while (total * first / blocks > s_start) --first;
+      while (total * (first + 1) / blocks <= s_start) ++first;
+      *todo = Merge{q0, nq, h, first, 1, {0, 0, 0}};
+    }
+    for (int n = 0; n < rows; ++n, ++item) {
+      if (item % kWarps != warp) continue;
+      auto piece = [&](int i) -> const float* {
+        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes)) : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
+      };
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t x = group; x; x &= x - 1) M = fmaxf(M, piece(__ffs(x) - 1)[8 * NT * kRowPad + n]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      for (uint32_t x = group; x; x &= x - 1) {
+        const float* from = piece(__ffs(x) - 1);
+        const float w = ex2f(from[8 * NT * kRowPad + n] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(from + n * kRowPad + 4 * lane);
+        L += w * from[8 * NT * kRowPad + 8 * NT + n];
+        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+      }
+      if (!began_before && ends) store_row4(p, out_row(p, Request{q0, nq, 0, 0}, h, n) + 4 * lane, acc, L);
+      else {
+        *reinterpret_cast<float4*>(to + n * kRowPad + 4 * lane) = acc;
+        if (lane == 0) { to[8 * NT * kRowPad + n] = M; to[8 * NT * kRowPad + 8 * NT + n] = L; }
+      }
+    }
+  }
+}
+
+// Runs that several blocks share.  Block (b, n) merges row n of the run that ends in block b of the decode kernel: eight warps take
+// its pieces in turn, then each other's sums.
+template <int NT>
+__global__ void __launch_bounds__(256)
+merge_kernel(const AttnParams p, int grid) {
+  __shared__ float s_m[8], s_l[8], s_acc[8][128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int b = blockIdx.x, n = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Merge todo = reinterpret_cast<const Merge*>(p.ws + ws_merge<NT>(grid))[b];
+  if (!todo.go || n >= todo.nq * p.G) return;
+  const float* base = p.ws + ws_block_pieces<NT>(grid);
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = todo.first + warp; i <= b; i += 8) {
+    const float* x = base + (int64_t)(2 * i + (i == todo.first ? 1 : 0)) * piece_floats(NT);
+    const float m = x[8 * NT * kRowPad + n], l = x[8 * NT * kRowPad + 8 * NT + n];
+    const float4 v = *reinterpret_cast<const float4*>(x + n * kRowPad + 4 * lane);
+    const float nm = fmaxf(M, m), ref = nm == -INFINITY ? 0.f : nm, wo = ex2f(M - ref), w = ex2f(m - ref);
+    L = L * wo + l * w;
+    acc.x = acc.x * wo + v.x * w; acc.y = acc.y * wo + v.y * w; acc.z = acc.z * wo + v.z * w; acc.w = acc.w * wo + v.w * w;
+    M = nm;
+  }
+  if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
+  *reinterpret_cast<float4*>(&s_acc[warp][4 * lane]) = acc;
+  __syncthreads();
+  if (warp) return;
+  M = s_m[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) M = fmaxf(M, s_m[i]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  L = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = ex2f(s_m[i] - ref);
+    const float4 v = *reinterpret_cast<const float4*>(&s_acc[i][4 * lane]);
+    L += w * s_l[i];
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+  }
+  store_row4(p, out_row(p, Request{todo.q0, todo.nq, 0, 0}, todo.h, n) + 4 * lane, acc, L);
+}
+
+static int tiles_of(const AttnParams& p) { return p.max_q_len * p.G <= 8 ? 1 : 2; }
+
+int64_t decode_workspace(const AttnParams& p) {
+  const int grid = sm_count();
+  return tiles_of(p) == 1 ? ws_merge<1>(grid) * 4 + grid * (int64_t)sizeof(Merge) : ws_merge<2>(grid) * 4 + grid * (int64_t)sizeof(Merge);
+}
+
+template <int NT>
+static int launch(const AttnParams& p, cudaStream_t st) {
+  const int grid = sm_count(), smem = warps_of(NT) * kSlots * kUnitBytes;
+  static thread_local int attr_dev = -1;
+  int dev = 0;
+  HQ_CUDA(cudaGetDevice(&dev));
+  if (attr_dev != dev) {
+    HQ_CUDA(cudaFuncSetAttribute(decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_dev = dev;
+  }
+  cudaLaunchAttribute after{};
+  after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  after.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(warps_of(NT) * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.attrs = &after; cfg.numAttrs = 1;
+  HQ_CUDA(cudaLaunchKernelEx(&cfg, decode_kernel<NT>, p));
+  cfg.gridDim = dim3(grid, p.max_q_len * p.G); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 0;
+  HQ_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel<NT>, p, grid));
+  return HQ_OK;
+}
+
+int decode_launch(const AttnParams& p, cudaStream_t st) { return tiles_of(p) == 1 ? launch<1>(p, st) : launch<2>(p, st); }
+
+}  // namespace paged
+}  // namespace hq

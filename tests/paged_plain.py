@@ -89,6 +89,12 @@ def values(pages, slots):
     return out
 
 
+def scales(pages, slots):
+    """The V scales float64 [T, H] of the slots."""
+    P = pages.shape[2] * BLOCK
+    return pages.view(torch.bfloat16)[..., 1040:1056][slots // P, :, slots % P // BLOCK, slots % BLOCK].double()
+
+
 def attention(q, pages, table, lens, cu, sm_scale=None):
     """(out, tolerance) float64 [T, H_Q, 128]; rows behind the last token are NaN.  Pages outside the pool hold absent keys.
 
@@ -97,7 +103,10 @@ def attention(q, pages, table, lens, cu, sm_scale=None):
     row sums and the quotient, and half a step of the output's type.  Terms that vanish: P~ is held as the fp16 number nearest to
     2^9 p v_scale / (a power of two that is less than four times the largest v_scale), p = 1 at the reference or above it at the
     maximum, so that a term is off by half of fp16's smallest step, 2^-25, at most: 2^-34 of 4 v_scale, or 2^-32 max|v| with
-    codes up to 7, against a row sum of at least 1; exponentials below the normal 32-bit numbers (2^-126) are far less."""
+    codes up to 7, against a row sum of at least 1; exponentials below the normal 32-bit numbers (2^-126) are far less.  Products of V:
+    the short form adds p (code + 8) v_scale and takes 8 p v_scale off again; its codes are fp16 numbers below the normal ones,
+    (code + 8) 2^-24, whose exponent field is that of 2^-14.  The tensor core lines products up by these fields and keeps 24
+    bits: the last one is 2^-37, or 2^-13 of a code, so that a product is off by 2^-13 p v_scale at most."""
     T, HQ, _ = q.shape
     num, H, blocks, _ = pages.shape
     P, G = blocks * BLOCK, HQ // H
@@ -116,6 +125,7 @@ def attention(q, pages, table, lens, cu, sm_scale=None):
         page = table[r, j // P].long()
         live = (page >= 0) & (page < num)
         k, v = values(pages, torch.where(live, page * P + j % P, 0))
+        vs = torch.where(live[:, None], scales(pages, torch.where(live, page * P + j % P, 0)), 0.0).unsqueeze(-1)
         for h in range(H):
             kk, vv = k[:, h], torch.where(live[:, None], v[:, h], 0.0)
             kk = torch.where(live[:, None], kk, 0.0)
@@ -132,5 +142,5 @@ def attention(q, pages, table, lens, cu, sm_scale=None):
             out[t0:t0 + n, h * G:h * G + G] = o
             tol[t0:t0 + n, h * G:h * G + G] = torch.finfo(q.dtype).eps / 2 * o.abs() * 1.01 + \
                 (2.0 ** -11 + 2 * delta + 2.0 ** -16) * (p @ vv.abs()) + \
-                2.0 ** -32 * L * vv.abs().max() / l.clamp(min=1.0) + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+                2.0 ** -13 * (p @ vs[:, h]) + 2.0 ** -32 * L * vv.abs().max() / l.clamp(min=1.0) + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
     return out, tol
