@@ -95,6 +95,7 @@ static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a->sm_scale >= 0.f && a->sm_scale < 1e30f, HQ_ERR_INVALID, "hq_paged_attention: sm_scale must be finite and not negative");
   HQ_REQUIRE(a->cu_q || (a->R == a->T && a->max_q_len == 1), HQ_ERR_INVALID, "hq_paged_attention: without cu_q every request has one token");
   HQ_REQUIRE((int64_t)a->R * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %d requests of %d kv heads", a->R, a->H_KV);
+  HQ_REQUIRE(a->num_pages * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %lld pages of %d kv heads", (long long)a->num_pages, a->H_KV);
   if (a->R == 0 || a->T == 0) return HQ_OK;
   HQ_REQUIRE(a->q && a->out && a->kv_lens && (a->page_table || a->max_pages == 0) && (a->pages || a->num_pages == 0), HQ_ERR_INVALID,
              "hq_paged_attention: null pointer");

@@ -24,8 +24,7 @@ namespace paged {
 
 constexpr int kUnit = 32, kUnitBytes = 2 * kBlockBytes, kSlots = 3;
 constexpr int kRowPad = 132;                    // floats of a row of a piece
-constexpr float kLazy = 4.0f;                   // the reference moves when a score passes it by 2^4
-constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9) <= 2^13: fp16's range above and below is used
+constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9): at most 2^10 when a reference is set, 2^15 before it moves
 __host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 16 : 12; }
 __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
 
@@ -38,13 +37,27 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// nibbles 0..3 of each 16-bit half as fp16 subnormals: (code + 8) 2^-24 for 0 and 2, 2^-20 for 1 and 3
-__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&h)[4]) {
+__device__ __forceinline__ void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float2 c) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y));
+}
+// nibbles 0..3 of each 16-bit half as fp16 subnormals: (code + 8) 2^-24 for 0 and 2, 2^-20 for 1 and 3.  The masks stay in registers:
+// as constants they are loaded again beside every use.
+struct Masks { uint32_t lo, hi, lo8, hi8; };
+__device__ __forceinline__ Masks masks() {
+  Masks k;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(k.lo));
+  asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(k.hi));
+  asm volatile("mov.b32 %0, 0x00080008;" : "=r"(k.lo8));
+  asm volatile("mov.b32 %0, 0x00800080;" : "=r"(k.hi8));
+  return k;
+}
+__device__ __forceinline__ void nibbles(const Masks& k, uint32_t w, uint32_t (&h)[4]) {
   const uint32_t w8 = w >> 8;
-  h[0] = lop3_and_xor(w, 0x000F000Fu, 0x00080008u);
-  h[1] = lop3_and_xor(w, 0x00F000F0u, 0x00800080u);
-  h[2] = lop3_and_xor(w8, 0x000F000Fu, 0x00080008u);
-  h[3] = lop3_and_xor(w8, 0x00F000F0u, 0x00800080u);
+  h[0] = lop3_and_xor(w, k.lo, k.lo8);
+  h[1] = lop3_and_xor(w, k.hi, k.hi8);
+  h[2] = lop3_and_xor(w8, k.lo, k.lo8);
+  h[3] = lop3_and_xor(w8, k.hi, k.hi8);
 }
 __device__ __forceinline__ float over_g(float v, bool max) {      // over the eight lanes with the same lane % 4
 #pragma unroll
@@ -156,6 +169,7 @@ decode_kernel(const AttnParams p) {
   uint8_t* ring = smem + warp * (kSlots * kUnitBytes);
   uint64_t* bar = bars + warp * kSlots;
   int* live = s_live + warp * kSlots;
+  const int num_pages = (int)p.num_pages, page_bytes = kBlockBytes << (p.page_shift - 4), blocks_mask = (1 << (p.page_shift - 4)) - 1;
   Walk f = c;                                                // the unit that is fetched next
   int f_left = left, f_slot = 0;
   int tab_r = -1, tab_u = 0, pg0 = -1, pg1 = -1;             // pages of 32 units of request tab_r, a unit per lane
@@ -171,18 +185,16 @@ decode_kernel(const AttnParams p) {
     }
     const int a = __shfl_sync(0xffffffffu, pg0, f.u - tab_u), b = __shfl_sync(0xffffffffu, pg1, f.u - tab_u);
     if (lane == 0) {
-      const int64_t tok = (int64_t)f.u * kUnit, in = tok & ((1 << p.page_shift) - 1);
-      const bool la = a >= 0 && a < p.num_pages, lb = b >= 0 && b < p.num_pages;
+      const bool la = (uint32_t)a < (uint32_t)num_pages, lb = (uint32_t)b < (uint32_t)num_pages;
       live[f_slot] = (la ? 1 : 0) | (lb ? 2 : 0);
       uint8_t* dst = ring + f_slot * kUnitBytes;
+      const uint8_t* src = p.pages + (int64_t)(a * p.H_KV + f.h) * page_bytes + ((f.u << 1) & blocks_mask) * kBlockBytes;
       mbar_expect_tx(bar + f_slot, ((la ? 1 : 0) + (lb ? 1 : 0)) * kBlockBytes);
-      const uint8_t* src = p.pages + block_offset(((int64_t)a << p.page_shift) + in, f.h, p.H_KV, p.page_shift);
       if (la && lb && p.page_shift > 4) bulk_g2s(dst, src, kUnitBytes, bar + f_slot);
       else {
         if (la) bulk_g2s(dst, src, kBlockBytes, bar + f_slot);
-        if (lb) bulk_g2s(dst + kBlockBytes, p.page_shift > 4 ? src + kBlockBytes
-                                                              : p.pages + block_offset((int64_t)b << p.page_shift, f.h, p.H_KV, p.page_shift),
-                         kBlockBytes, bar + f_slot);
+        if (lb) bulk_g2s(dst + kBlockBytes, p.page_shift > 4 ? src + kBlockBytes : p.pages + (int64_t)(b * p.H_KV + f.h) * page_bytes, kBlockBytes,
+                         bar + f_slot);
       }
     }
     if (++f_slot == kSlots) f_slot = 0;
@@ -194,7 +206,9 @@ decode_kernel(const AttnParams p) {
   // ---- the state of the run in hand
   uint32_t qf[NT][16];                                       // query operand: word w, nibble k at 4 w + k
   float2 fac[NT], start[NT];                                 // factor of a score, start of the accumulators: columns 2 t4, 2 t4 + 1
-  float2 m[NT], l[NT];
+  float2 m[NT], l[NT], shift[NT];                            // shift = kShift - m
+  float vback = 1.f;                                         // 2^-vexp
+  const Masks km = masks();
   float O[NT][8][4], Ls[NT][4];
   int vexp = 0;                                              // V scales are taken relative to 2^vexp
   int lim0 = 0;                                              // keys that the run's first token sees
@@ -244,6 +258,7 @@ decode_kernel(const AttnParams p) {
       fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
       start[nt] = make_float2(__shfl_sync(0xffffffffu, first, 8 * t4), __shfl_sync(0xffffffffu, first, 8 * t4 + 4));
       m[nt] = make_float2(-INFINITY, -INFINITY);
+      shift[nt] = make_float2(INFINITY, INFINITY);
       l[nt] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < 2; ++j) lim[nt][j] = c.q.past + 1 + min((8 * nt + 2 * t4 + j) / p.G, c.q.nq - 1);
@@ -256,6 +271,7 @@ decode_kernel(const AttnParams p) {
     }
     lim0 = c.q.past + 1;
     vexp = -1000;
+    vback = 1.f;
   };
   // what the row is at the end: the 8 of the codes taken off, the powers of two put back
   auto close = [&](auto&& row) {
@@ -309,18 +325,17 @@ decode_kernel(const AttnParams p) {
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb) {
       const uint8_t* b = u0 + cb * kBlockBytes;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) { S[nt][cb][0] = S[nt][cb][2] = start[nt].x; S[nt][cb][1] = S[nt][cb][3] = start[nt].y; }
       const uint4 ka = *reinterpret_cast<const uint4*>(b + tau * 64 + 16 * t4), kb = *reinterpret_cast<const uint4*>(b + (tau + 8) * 64 + 16 * t4);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t ha[4], hb[4];
-        nibbles(wa[w], ha);
-        nibbles(wb[w], hb);
+        nibbles(km, wa[w], ha);
+        nibbles(km, wb[w], hb);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma16816(S[nt][cb], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * w], qf[nt][4 * w + 1]);
+          if (w == 0) mma16816_from(S[nt][cb], ha[0], hb[0], ha[1], hb[1], qf[nt][0], qf[nt][1], start[nt]);
+          else mma16816(S[nt][cb], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * w], qf[nt][4 * w + 1]);
           mma16816(S[nt][cb], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * w + 2], qf[nt][4 * w + 3]);
         }
       }
@@ -357,21 +372,40 @@ decode_kernel(const AttnParams p) {
               if (!here || tok >= lim[nt][j]) S[nt][cb][2 * i + j] = -INFINITY;
         }
     }
-    // the references: the maximum of a row, the largest V scale
-    bool move = false;
+    // P against the references as they stand: a row's reference maximum, the power of two of the V scales.  Nothing is compared
+    // beforehand: a term that fp16 could not hold shows in the sum of the terms (so does a row's first unit, whose shift is infinite);
+    // only then the maxima are taken, the references move and the unit's P is formed again.
+    uint32_t P[NT][2][2];
+    float2 le[NT];
+    auto form = [&]() {
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float x0 = fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2]));
-      const float x1 = fmaxf(fmaxf(S[nt][0][1], S[nt][0][3]), fmaxf(S[nt][1][1], S[nt][1][3]));
-      move |= x0 > m[nt].x + kLazy || x1 > m[nt].y + kLazy;
-    }
-    const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
-    move |= (int)(__float_as_uint(vtop) >> 23) - 127 > vexp && vtop > 0.f;
-    if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
+      for (int nt = 0; nt < NT; ++nt) {
+        le[nt] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 y = fadd2(make_float2(S[nt][cb][2 * i], S[nt][cb][2 * i + 1]), shift[nt]);
+            const float2 e = make_float2(ex2f(y.x), ex2f(y.y));
+            le[nt] = fadd2(le[nt], e);
+            const float sv = vs[cb][i] * vback;
+            const float2 pv = fmul2(e, make_float2(sv, sv));
+            sum = fadd2(sum, pv);
+            const __half2 hh = __floats2half2_rn(pv.x, pv.y);
+            P[nt][cb][i] = *reinterpret_cast<const uint32_t*>(&hh);
+          }
+      }
+      return sum.x + sum.y;
+    };
+    const float sum = form();
+    if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 32768.f)), 0)) {
+      const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
       const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 127;
       const int nv = max(vexp, e);
       const float vscale = vexp == -1000 ? 0.f : ldexpf(1.f, max(vexp - nv, -200));
       vexp = nv;
+      vback = __uint_as_float((uint32_t)(127 - max(vexp, -126)) << 23);                 // 2^-vexp
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float x0 = over_g(fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2])), true);
@@ -384,25 +418,20 @@ decode_kernel(const AttnParams p) {
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) { O[nt][mt][0] *= av.x; O[nt][mt][1] *= av.y; O[nt][mt][2] *= av.x; O[nt][mt][3] *= av.y; }
         Ls[nt][0] *= av.x; Ls[nt][1] *= av.y; Ls[nt][2] *= av.x; Ls[nt][3] *= av.y;
+        shift[nt] = make_float2(nm.x == -INFINITY ? 0.f : kShift - nm.x, nm.y == -INFINITY ? 0.f : kShift - nm.y);
+      }
+      form();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {                      // a row without a key so far: its next unit comes here again
+        if (m[nt].x == -INFINITY) shift[nt].x = INFINITY;
+        if (m[nt].y == -INFINITY) shift[nt].y = INFINITY;
       }
     }
-    const float vback = __uint_as_float((uint32_t)(127 - max(vexp, -126)) << 23);        // 2^-vexp
-    uint32_t P[NT][2][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float2 nm = make_float2(m[nt].x == -INFINITY ? 0.f : kShift - m[nt].x, m[nt].y == -INFINITY ? 0.f : kShift - m[nt].y);
+      l[nt] = fadd2(l[nt], le[nt]);
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 y = fadd2(make_float2(S[nt][cb][2 * i], S[nt][cb][2 * i + 1]), nm);
-          const float2 e = make_float2(ex2f(y.x), ex2f(y.y));
-          l[nt] = fadd2(l[nt], e);
-          const float sv = vs[cb][i] * vback;
-          const float2 pv = fmul2(e, make_float2(sv, sv));
-          const __half2 hh = __floats2half2_rn(pv.x, pv.y);
-          P[nt][cb][i] = movmatrix(*reinterpret_cast<const uint32_t*>(&hh));
-        }
+      for (int cb = 0; cb < 2; ++cb) { P[nt][cb][0] = movmatrix(P[nt][cb][0]); P[nt][cb][1] = movmatrix(P[nt][cb][1]); }
     }
     if (!ok) {                                               // a copy that never came: the rows are NaN
 #pragma unroll
@@ -417,8 +446,8 @@ decode_kernel(const AttnParams p) {
       for (int q4 = 0; q4 < 4; ++q4) {                       // channels 16 g + 4 q4 .. + 3: a 16-bit half of each token's word
         const uint32_t sel = q4 & 1 ? 0x7632u : 0x5410u;
         uint32_t ha[4], hb[4];
-        nibbles(prmt(q4 < 2 ? v0.x : v0.y, q4 < 2 ? v1.x : v1.y, sel), ha);
-        nibbles(prmt(q4 < 2 ? v2.x : v2.y, q4 < 2 ? v3.x : v3.y, sel), hb);
+        nibbles(km, prmt(q4 < 2 ? v0.x : v0.y, q4 < 2 ? v1.x : v1.y, sel), ha);
+        nibbles(km, prmt(q4 < 2 ? v2.x : v2.y, q4 < 2 ? v3.x : v3.y, sel), hb);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mma16816(O[nt][2 * q4], ha[0], ha[2], hb[0], hb[2], P[nt][cb][0], P[nt][cb][1]);
