@@ -38,6 +38,8 @@ struct AttnParams {
 
 int64_t decode_workspace(const AttnParams& p);                 // bytes; hq_paged_decode.cu
 int decode_launch(const AttnParams& p, cudaStream_t st);
+int64_t tile_workspace(const AttnParams& p);                   // hq_paged_tile.cu
+int tile_launch(const AttnParams& p, cudaStream_t st);
 
 inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
 

@@ -1,81 +1,9 @@
-// Attention over the paged 4-bit cache.
+// Attention over the paged 4-bit cache: the entry points.  Calls whose new tokens times query heads per kv head fit 16 rows go to the
+// split kernel on mma.sync (hq_paged_decode.cu), longer ones to the tile kernel on tcgen05 (hq_paged_tile.cu).
 #include "hq_paged.cuh"
 
 namespace hq {
 namespace paged {
-
-// One block per new token and kv head; 128 threads.  Keys in tiles of 32: four threads a key for the scores, then a thread per
-// channel for the values.
-__global__ void __launch_bounds__(128)
-attn_simple_kernel(const AttnParams p) {
-  __shared__ float sq[16][128], sp[16][32], smx[16], sl[16], sal[16];
-  const int r = blockIdx.z, h = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
-  const Request rq = request_of(p, r);
-  if (i >= rq.nq) return;
-  const int q0 = rq.q0, n_keys = max(0, min(rq.len, rq.past + i + 1));
-  const int t = q0 + i, G = p.G;
-  for (int x = tid; x < G * 128; x += 128) {
-    const int64_t at = t * p.q_st + (h * G + x / 128) * p.q_sh + x % 128;
-    sq[x / 128][x % 128] = (p.dtype == HQ_BF16 ? __bfloat162float(((const __nv_bfloat16*)p.q)[at]) : __half2float(((const __half*)p.q)[at])) * p.sml;
-  }
-  if (tid < 16) { smx[tid] = -INFINITY; sl[tid] = 0.f; }
-  __syncthreads();
-  float acc[16];
-#pragma unroll
-  for (int g = 0; g < 16; ++g) acc[g] = 0.f;
-  for (int j0 = 0; j0 < n_keys; j0 += 32) {
-    const int jj = tid >> 2, part = tid & 3, j = j0 + jj;
-    const int page = j < n_keys ? p.table[r * p.table_stride + (j >> p.page_shift)] : -1;
-    const bool live = page >= 0 && page < p.num_pages;
-    float kx[32];
-    if (live) {
-      const int64_t slot = ((int64_t)page << p.page_shift) + (j & ((1 << p.page_shift) - 1));
-      const uint8_t* b = p.pages + block_offset(slot, h, p.H_KV, p.page_shift);
-      const float s = __uint_as_float((uint32_t)((const uint16_t*)(b + kKsOff))[j & 15] << 16);
-      const uint4 c = *reinterpret_cast<const uint4*>(b + (j & 15) * 64 + part * 16);
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-      for (int x = 0; x < 32; ++x) kx[x] = (float)((int)(w[x >> 3] << (28 - 4 * (x & 7))) >> 28) * s;
-    }
-    for (int g = 0; g < G; ++g) {
-      float d = 0.f;
-      if (live)
-#pragma unroll
-        for (int x = 0; x < 32; ++x) d += kx[x] * sq[g][part * 32 + x];
-      d += __shfl_xor_sync(0xffffffffu, d, 1);
-      d += __shfl_xor_sync(0xffffffffu, d, 2);
-      if (part == 0) sp[g][jj] = live ? d : -INFINITY;
-    }
-    __syncthreads();
-    if (tid < G) {
-      float m = smx[tid];
-      for (int x = 0; x < 32; ++x) m = fmaxf(m, sp[tid][x]);
-      const float mu = m == -INFINITY ? 0.f : m;
-      const float alpha = ex2f(smx[tid] - mu);
-      float l = sl[tid] * alpha;
-      for (int x = 0; x < 32; ++x) { const float e = ex2f(sp[tid][x] - mu); sp[tid][x] = e; l += e; }
-      sal[tid] = alpha; smx[tid] = m; sl[tid] = l;
-    }
-    __syncthreads();
-    for (int g = 0; g < G; ++g) acc[g] *= sal[g];
-    for (int x = 0; x < 32 && j0 + x < n_keys; ++x) {
-      const int pg = p.table[r * p.table_stride + ((j0 + x) >> p.page_shift)];
-      if (pg < 0 || pg >= p.num_pages) continue;
-      const int64_t slot = ((int64_t)pg << p.page_shift) + ((j0 + x) & ((1 << p.page_shift) - 1));
-      const uint8_t* b = p.pages + block_offset(slot, h, p.H_KV, p.page_shift);
-      const int row = (j0 + x) & 15;
-      const float s = __uint_as_float((uint32_t)((const uint16_t*)(b + kVsOff))[row] << 16);
-      const int c = b[kVOff + row * 64 + (tid >> 1)];
-      const float vv = (float)((int)((uint32_t)c << (tid & 1 ? 24 : 28)) >> 28) * s;
-      for (int g = 0; g < G; ++g) acc[g] += sp[g][x] * vv;
-    }
-    __syncthreads();
-  }
-  for (int g = 0; g < G; ++g) {
-    const float l = sl[g], o = l > 0.f ? acc[g] / l : 0.f;
-    store_out(p.out, t * p.o_st + (h * G + g) * p.o_sh + tid, o, p.dtype);
-  }
-}
 
 static int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
 
@@ -119,6 +47,7 @@ static AttnParams params_of(const hq_paged_attention_args* a) {
   return p;
 }
 static bool few_rows(const AttnParams& p) { return (int64_t)p.max_q_len * p.G <= 16; }
+static int64_t workspace_of(const AttnParams& p) { return few_rows(p) ? decode_workspace(p) : tile_workspace(p); }
 
 }  // namespace paged
 }  // namespace hq
@@ -128,7 +57,7 @@ extern "C" int hq_paged_attention_workspace_bytes(const hq_paged_attention_args*
   if (int rc = paged::check(a)) return rc;
   HQ_REQUIRE(bytes, HQ_ERR_INVALID, "hq_paged_attention_workspace_bytes: null pointer");
   const paged::AttnParams p = paged::params_of(a);
-  *bytes = paged::few_rows(p) && a->R > 0 && a->T > 0 ? paged::decode_workspace(p) : 0;
+  *bytes = a->R > 0 && a->T > 0 ? paged::workspace_of(p) : 0;
   return HQ_OK;
 }
 
@@ -138,14 +67,8 @@ extern "C" int hq_paged_attention(const hq_paged_attention_args* a, void* stream
   if (int rc = check(a)) return rc;
   if (a->R == 0 || a->T == 0) return HQ_OK;
   const AttnParams p = params_of(a);
-  if (few_rows(p)) {
-    HQ_REQUIRE(a->workspace && a->workspace_bytes >= decode_workspace(p), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
-               (long long)a->workspace_bytes, (long long)decode_workspace(p));
-    HQ_REQUIRE(aligned16(a->workspace), HQ_ERR_ALIGNMENT, "hq_paged_attention: the workspace must be 16-byte aligned");
-    return decode_launch(p, (cudaStream_t)stream);
-  }
-  HQ_REQUIRE(a->R <= 65535 && a->H_KV <= 65535, HQ_ERR_UNSUPPORTED, "hq_paged_attention: too many requests");
-  attn_simple_kernel<<<dim3(a->max_q_len, a->H_KV, a->R), 128, 0, (cudaStream_t)stream>>>(p);
-  HQ_CUDA(cudaGetLastError());
-  return HQ_OK;
+  HQ_REQUIRE(a->workspace && a->workspace_bytes >= workspace_of(p), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
+             (long long)a->workspace_bytes, (long long)workspace_of(p));
+  HQ_REQUIRE(aligned16(a->workspace), HQ_ERR_ALIGNMENT, "hq_paged_attention: the workspace must be 16-byte aligned");
+  return few_rows(p) ? decode_launch(p, (cudaStream_t)stream) : tile_launch(p, (cudaStream_t)stream);
 }
