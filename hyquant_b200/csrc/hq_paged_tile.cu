@@ -5,12 +5,13 @@
 // group size - in two halves of 128; keys come in tiles of 64.  Bound by the tensor pipe and the exponentials, which take about the
 // same time: 8.4 MFLOP and 16384 exponentials a tile pair, some 1024 clocks of an SM each at their nominal rates.
 //
-// One block per SM, 12 warps (168 registers a thread):
+// One block per SM, 15 warps:
 //   0-3, 4-7   softmax of the two halves, a thread per row; they also load the queries and write the results
-//   8, 9       the cache: codes arrive by cp.async some tiles ahead, become fp16 values (exact: the format sees to that) and are
-//              written as the swizzled operand tiles that both halves read: 64 keys are unpacked once for 256 rows
-//   10, 11     issue the products of a half each: S = Q K^T into one of two buffers of 64 columns, O += P V with P (fp16, over the
+//   8-11       the cache: codes become fp16 values (exact: the format sees to that) in the swizzled operand tiles that both halves
+//              read, so that 64 keys are unpacked once for 256 rows; two warps take the even tiles, two the odd ones
+//   12, 13     issue the products of a half each: S = Q K^T into one of two buffers of 64 columns, O += P V with P (fp16, over the
 //              buffer just read) from tensor memory and V's rows as they lie.  Q K^T of tile t + 2 follows P V of tile t.
+//   14         fetches the codes: a tile is four blocks of sixteen tokens, a bulk copy each, some tiles ahead
 // Channels stand in the order in which the unpacking produces them (0 4 1 5 2 6 3 7 in every eight), in Q, K and V alike; the rows that
 // are written put them back.
 //
@@ -23,20 +24,20 @@
 namespace hq {
 namespace paged {
 
-constexpr int kTileThreads = 384, kRows = 256, kKeys = 64;
-constexpr int kUnpack = 2, kGroups = 8 / kUnpack;      // warps that unpack; groups of eight keys of a tile each takes: w, w + kUnpack, ..
+constexpr int kTileThreads = 480, kRows = 256, kKeys = 64;
+constexpr int kIssue = 12, kFetch = 14;          // first issuing warp; the fetching one
 constexpr int kStages = 3;                       // K tiles, and V tiles, in shared memory
-constexpr int kAhead = 4;                        // tiles of codes under way, the one that is unpacked among them
-constexpr int kCodeBytes = kGroups * (512 + 512 + 32) + 16;      // one warp's part of a tile: K codes, V codes, scales, row counts
+constexpr int kAhead = 4;                        // tiles of codes in shared memory
+constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
 constexpr int kItemCost = 2;                     // what a query tile costs beside its key tiles, in key tiles
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
 constexpr uint32_t kTPolls = 400000u;
 
 struct TileSmem {
-  static constexpr int Q = 0, K = 65536, V = K + kStages * 16384, Codes = V + kStages * 16384, Bar = Codes + kUnpack * kAhead * kCodeBytes,
-                       Bad = Bar + 256, Total = Bad + 32;
+  static constexpr int Q = 0, K = 65536, V = K + kStages * 16384, Codes = V + kStages * 16384, Bar = Codes + kAhead * kCodeBytes,
+                       Rows = Bar + 320, Bad = Rows + 4 * kAhead, Total = Bad + 16;
 };
-static_assert(kGroups == 4 && kUnpack == 2 && TileSmem::Bar % 16 == 0 && TileSmem::Total + 1024 <= 227 * 1024, "shared memory");
+static_assert(TileSmem::Bar % 16 == 0 && TileSmem::Total + 1024 <= 227 * 1024, "shared memory");
 
 struct TileMerge { int q0, rows, h, qt, first, go, unused[2]; };
 
@@ -100,8 +101,7 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 struct SlowState { float m, l; bool ok; };
 
 // A tile that needs masks or a new reference: the scores are read again, the maximum taken, O rescaled where a row's reference
-// moves (where the maximum passes it by `slack`), P formed.  `lim`: keys of the tile that the row sees; bad: eight-key groups that are
-// not there.
+// moves (where the maximum passes it by `slack`), P formed.  `lim`: keys of the tile that the row sees; bad: blocks of sixteen keys that are not there.
 __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, int lim, uint32_t bad, float slack, float m, float l,
                                             uint64_t* pv_bar, uint32_t pv_parity, volatile int* abort_flag) {
   SlowState out{m, l, true};
@@ -112,7 +112,7 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
   float mx = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 64; ++c) {
-    x[c] = (c < lim && !((bad >> (c >> 3)) & 1u)) ? x[c] * f : -INFINITY;
+    x[c] = (c < lim && !((bad >> (c >> 4)) & 1u)) ? x[c] * f : -INFINITY;
     mx = fmaxf(mx, x[c]);
   }
   const bool grow = mx > m + slack;
@@ -174,10 +174,6 @@ __device__ __forceinline__ uint4 values8_any(uint32_t w, __half2 s) {
   return make_uint4(val(x0), val(x1), val(x2), val(x3));
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
 template <bool kBf16>
 __global__ void __launch_bounds__(kTileThreads, 1)
 tile_kernel(const AttnParams p, int piece_rows) {
@@ -189,7 +185,9 @@ tile_kernel(const AttnParams p, int piece_rows) {
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
   uint64_t* v_empty = v_full + kStages;
-  uint64_t* s_full = v_empty + kStages;          // [half][2]
+  uint64_t* c_full = v_empty + kStages;          // [kAhead]
+  uint64_t* c_empty = c_full + kAhead;
+  uint64_t* s_full = c_empty + kAhead;           // [half][2]
   uint64_t* p_ready = s_full + 4;
   uint64_t* pv_done = p_ready + 4;
   uint64_t* drained = pv_done + 4;               // [half]
@@ -198,10 +196,11 @@ tile_kernel(const AttnParams p, int piece_rows) {
   __shared__ long long s_part[kTileThreads + 1], s_warp[kTileThreads / 32];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
-  if (warp == 10) {
+  if (warp == kIssue) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 128); mbar_init(drained + i, 1); }
-      for (int i = 0; i < kStages; ++i) { mbar_init(k_full + i, kUnpack); mbar_init(k_empty + i, 2); mbar_init(v_full + i, kUnpack); mbar_init(v_empty + i, 2); }
+      for (int i = 0; i < kStages; ++i) { mbar_init(k_full + i, 2); mbar_init(k_empty + i, 2); mbar_init(v_full + i, 2); mbar_init(v_empty + i, 2); }
+      for (int i = 0; i < kAhead; ++i) { mbar_init(c_full + i, 1); mbar_init(c_empty + i, 2); }
       for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_ready + i, 128); mbar_init(pv_done + i, 1); }
       *abort_flag = 0;
       fence_mbar_init();
@@ -266,9 +265,46 @@ tile_kernel(const AttnParams p, int piece_rows) {
     pc.it = it;
   }
 
-  if (warp >= 10) {
+  int* key_rows = reinterpret_cast<int*>(smem + TileSmem::Rows);           // [kAhead] keys of a tile that are there, the last ones missing
+  uint8_t* bads = smem + TileSmem::Bad;                                    // [16] blocks of a tile whose page is not there
+  if (warp == kFetch) {
+    // ------------------------------------------------------------ codes
+    const int num_pages = (int)p.num_pages, page_bytes = kBlockBytes << (p.page_shift - 4), blocks_mask = (1 << (p.page_shift - 4)) - 1;
+    int tab_r = -1, tab_t = 0, pg = -1;          // pages of eight tiles of request tab_r: lane 4 i + b, block b of tile tab_t + i
+    int stage = 0;
+    uint32_t par = 1u, tile = 0;                 // empty barriers: the first round passes
+    bool ok = true;
+    while (ok && pc.take(p)) {
+#pragma unroll 1
+      for (int t = pc.t0; t < pc.t1; ++t, ++tile) {
+        if (pc.it.r != tab_r || t < tab_t || t >= tab_t + 8) {
+          tab_r = pc.it.r; tab_t = t;
+          const int64_t tok = ((int64_t)t + (lane >> 2)) * kKeys + kTok * (lane & 3);
+          pg = tok < pc.it.q.len ? __ldg(p.table + (int64_t)tab_r * p.table_stride + (tok >> p.page_shift)) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, pg, 4 * (t - tab_t) + (lane & 3)), tok = t * kKeys + kTok * (lane & 3);
+        const bool in = tok < pc.it.q.len && lane < 4, there = in && (uint32_t)page < (uint32_t)num_pages;
+        const uint32_t have = __ballot_sync(0xffffffffu, there), gone = __ballot_sync(0xffffffffu, in && !there);
+        ok = wait_warp(c_empty + stage, par, abort_flag);
+        if (!ok) break;
+        if (lane == 0) {
+          key_rows[stage] = min(kKeys, pc.it.q.len - t * kKeys) | (int)(gone << 16);
+          bads[tile & 15u] = (uint8_t)gone;
+          mbar_expect_tx(c_full + stage, __popc(have) * kBlockBytes);
+        }
+        __syncwarp();
+        if (there)
+          bulk_g2s(smem + TileSmem::Codes + stage * kCodeBytes + lane * kBlockBytes,
+                   p.pages + (int64_t)(page * p.H_KV + pc.it.h) * page_bytes + ((tok >> 4) & blocks_mask) * kBlockBytes, kBlockBytes, c_full + stage);
+        if (++stage == kAhead) { stage = 0; par ^= 1u; }
+      }
+      pc.done(p);
+    }
+    // a block must not end with copies under way, also where it gives up: wait for the last load of every slot
+    for (int i = 0; i < kAhead; ++i) mbar_wait_bounded(c_full + i, i < stage ? par ^ 1u : par, kTPolls);
+  } else if (warp >= kIssue) {
     // ------------------------------------------------------------ products of one half
-    const int half = warp - 10;
+    const int half = warp - kIssue;
     const uint32_t idesc_qk = tc::make_idesc(1, 0, 0, 128, kKeys), idesc_pv = tc::make_idesc(1, 0, 0, 128, 128) | tc::kBMnMajor;
     const uint64_t dQ = tc::smem_desc_k128(smem + TileSmem::Q + half * 32768, 0);
     const uint64_t dK = tc::smem_desc_k128(smem + TileSmem::K, 0), dV = tc::smem_desc_mn128(smem + TileSmem::V, 8192);
@@ -335,100 +371,70 @@ tile_kernel(const AttnParams p, int piece_rows) {
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(drained + half, 0, kTPolls)) || !ok) *abort_flag = 1;
   } else if (warp >= 8) {
     // ------------------------------------------------------------ the cache: codes to operand tiles
-    const int w = warp - 8, rowl = lane & 7, quarter = lane >> 3;
-    uint8_t* codes = smem + TileSmem::Codes + w * (kAhead * kCodeBytes);
-    uint8_t* bads = smem + TileSmem::Bad;
-    const int num_pages = (int)p.num_pages, page_bytes = kBlockBytes << (p.page_shift - 4), blocks_mask = (1 << (p.page_shift - 4)) - 1;
-    Pieces f = pc;                               // what is asked for next
-    bool f_some = f.take(p);
-    while (f_some && f.t1 == f.t0) { f.done(p); f_some = f.take(p); }
-    int f_t = f_some ? f.t0 : 0, f_stage = 0;
-    constexpr int kWindow = 32 / kGroups;
-    int tab_r = -1, tab_t = 0, pg = -1;          // pages of kWindow tiles of request tab_r: lane kGroups i + g, the warp's group g of tile tab_t + i
-    auto ask = [&]() {
-      if (f_some) {
-        if (f.it.r != tab_r || f_t < tab_t || f_t >= tab_t + kWindow) {
-          tab_r = f.it.r; tab_t = f_t;
-          const int64_t tok = ((int64_t)tab_t + lane / kGroups) * kKeys + 8 * (w + kUnpack * (lane % kGroups));
-          pg = tok < f.it.q.len ? __ldg(p.table + (int64_t)tab_r * p.table_stride + (tok >> p.page_shift)) : -1;
-        }
-        uint8_t* st = codes + f_stage * kCodeBytes;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const int page = __shfl_sync(0xffffffffu, pg, kGroups * (f_t - tab_t) + g), tok = f_t * kKeys + 8 * (w + kUnpack * g);
-          const int rows = min(8, f.it.q.len - tok);          // <= 0: behind the last key
-          const bool there = (uint32_t)page < (uint32_t)num_pages && rows > 0;
-          const uint8_t* block = p.pages + (there ? (int64_t)(page * p.H_KV + f.it.h) * page_bytes + ((tok >> 4) & blocks_mask) * kBlockBytes : 0);
-          const uint8_t* src = block + (tok & 8) * 64 + rowl * 64 + quarter * 16;
-          cp_async16(st + g * 512 + lane * 16, src, there);
-          cp_async16(st + kGroups * 512 + g * 512 + lane * 16, src + kVOff, there);
-          if (lane < 2) cp_async16(st + kGroups * 1024 + g * 32 + lane * 16, block + (lane ? kVsOff : kKsOff) + 2 * (tok & 8), there);
-          if (lane == 0) reinterpret_cast<int*>(st + kGroups * 1056)[g] = there ? rows : rows > 0 ? -1 : 0;     // rows; -1: a page that is not there
-        }
-        if (++f_stage == kAhead) f_stage = 0;
-        if (++f_t == f.t1) {
-          do { f.done(p); f_some = f.take(p); } while (f_some && f.t1 == f.t0);
-          if (f_some) f_t = f.t0;
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll 1
-    for (int i = 0; i < kAhead - 1; ++i) ask();
-    int stage = 0, c_stage = 0;
-    uint32_t par = 1u, tile = 0;                 // empty barriers: the first round passes
+    // Lane: row lane / 4 of a group of eight keys, channels 32 (lane % 4) ..  A warp reads 512 bytes in one piece; the lanes of the
+    // upper channels take their words two apart, so that no two of eight lanes write to the same banks either.
+    const int team = warp & 1, wt = (warp - 8) >> 1, rowl = lane >> 2, quarter = lane & 3, turn = quarter & 2;
+    int n_all = 0;
+    while (pc.take(p)) { n_all += pc.t1 - pc.t0; pc.done(p); }
     bool ok = true;
-    while (ok && pc.take(p)) {
-      const int n = pc.t1 - pc.t0;
 #pragma unroll 1
-      for (int t = 0; t < n; ++t, ++tile) {
-        __syncwarp();                            // the part of the ring that is asked for has been read by all lanes
-        ask();
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-        __syncwarp();
-        const uint8_t* st = codes + c_stage * kCodeBytes;
-        const int4 rows = *reinterpret_cast<const int4*>(st + kGroups * 1056);
-        ok = wait_warp(k_empty + stage, par, abort_flag);
-        if (!ok) break;
-        if (lane == 0) bads[(tile & 7u) * kUnpack + w] = (uint8_t)((rows.x < 0 ? 1 : 0) | (rows.y < 0 ? 2 : 0) | (rows.z < 0 ? 4 : 0) | (rows.w < 0 ? 8 : 0));
-        auto unpack = [&](int which, uint8_t* tile_at) {
+    for (int tile = team; ok && tile < n_all; tile += 2) {
+      const int cs = tile % kAhead, ks = tile % kStages;
+      const uint32_t kpar = (uint32_t)(tile / kStages + 1) & 1u;
+      ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
+      if (!ok) break;
+      const uint8_t* st = smem + TileSmem::Codes + cs * kCodeBytes;
+      const int info = key_rows[cs], rows = info & 0xFFFF;
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            const uint4 c = *reinterpret_cast<const uint4*>(st + which * (kGroups * 512) + g * 512 + lane * 16);
-            const uint16_t sb = *reinterpret_cast<const uint16_t*>(st + kGroups * 1024 + g * 32 + which * 16 + 2 * rowl);
-            const float s = rowl < (g == 0 ? rows.x : g == 1 ? rows.y : g == 2 ? rows.z : rows.w) ? __uint_as_float((uint32_t)sb << 16) : 0.f;      // rows that are not there: zeros
-            const __half2 s2 = __float2half2_rn(s), s24 = __float2half2_rn(-24.f * s);
-            const bool any = __any_sync(0xffffffffu, s > 2048.f);
-            const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
-            const int row = 8 * (w + kUnpack * g) + rowl;
+      for (int kv = 0; kv < 2; ++kv) {
+        uint4 val[4][4];
+        {
+          uint4 c[4];
+          float s[4];
+          bool any = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int chunk = quarter * 4 + k;
-              *reinterpret_cast<uint4*>(tile_at + (chunk >> 3) * 8192 + row * 128 + (((chunk & 7) ^ rowl) << 4)) =
-                  __builtin_expect(any, 0) ? values8_any(cw[k], s2) : values8(cw[k], s2, s24);
+          for (int g = 0; g < 4; ++g) {          // keys 8 (wt + 2 g) .. + 7: block g, its half wt
+            const uint8_t* block = st + g * kBlockBytes;
+            c[g] = *reinterpret_cast<const uint4*>(block + kv * kVOff + wt * 512 + lane * 16);
+            const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * wt + rowl));
+            const bool live = kTok * g + 8 * wt + rowl < rows && !((info >> (16 + g)) & 1);
+            s[g] = live ? __uint_as_float((uint32_t)sb << 16) : 0.f;       // keys that are not there: zeros, whatever lies here
+            any |= s[g] > 2048.f;
+          }
+          const bool big = __any_sync(0xffffffffu, any);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t cw[4] = {turn ? c[g].z : c[g].x, turn ? c[g].w : c[g].y, turn ? c[g].x : c[g].z, turn ? c[g].y : c[g].w};
+            const __half2 s2 = __float2half2_rn(s[g]), s24 = __float2half2_rn(-24.f * s[g]);
+            if (__builtin_expect(big, 0)) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) val[g][k] = values8_any(cw[k], s2);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) val[g][k] = values8(cw[k], s2, s24);
             }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-        };
-        unpack(0, smem + TileSmem::K + stage * 16384);
-        if (lane == 0) tc::mbar_arrive(k_full + stage);
-        ok = wait_warp(v_empty + stage, par, abort_flag);
-        if (!ok) break;
-        unpack(1, smem + TileSmem::V + stage * 16384);
-        if (lane == 0) tc::mbar_arrive(v_full + stage);
-        if (++stage == kStages) { stage = 0; par ^= 1u; }
-        if (++c_stage == kAhead) c_stage = 0;
+        }
+        // the values are in registers before their place is free: from then on it takes sixteen stores
+        ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
+        uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384 + (quarter >> 1) * 8192 + (8 * wt + rowl) * 128;
+        if (ok)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(to + g * 2048 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
       }
-      pc.done(p);
+      if (!ok) break;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) { tc::mbar_arrive(c_empty + cs); tc::mbar_arrive(k_full + ks); tc::mbar_arrive(v_full + ks); }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ------------------------------------------------------------ softmax: a thread per row
     const int half = warp >> 2, wq = warp & 3, r = wq * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(wq * 32) << 16), tO = lane_base + 256u + 128u * half;
     uint8_t* sQ = smem + TileSmem::Q + half * 32768;
-    const uint8_t* bads = smem + TileSmem::Bad;
     uint32_t tile = 0, all = 0;                  // tiles of this half; of the block
     bool ok = true;
     while (pc.take(p)) {
@@ -483,7 +489,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
           if (!ok) break;
           tc::fence_after_sync();
           const uint32_t tS = lane_base + 128u * half + 64u * slot;
-          const uint32_t bad = *reinterpret_cast<const uint16_t*>(bads + ((all + t) & 7u) * kUnpack);
+          const uint32_t bad = bads[(all + t) & 15u];
           const int see = lim - (pc.t0 + t) * kKeys;
           const bool masks = __any_sync(0xffffffffu, see < kKeys || bad != 0u);
           bool need = false;
@@ -509,12 +515,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
             need = !(sum <= kTMost);
           }
           if (__builtin_expect(masks || __any_sync(0xffffffffu, need), 0)) {
-            uint32_t gone = 0;                   // byte w, bit g -> key group w + kUnpack g
-            if (bad) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) gone |= ((bad >> (8 * (j % kUnpack) + j / kUnpack)) & 1u) << j;
-            }
-            const SlowState x2 = slow_tile(tS, tO, f, see, gone, need ? 0.f : 4.f, m, l, t > 0 ? pv_done + 2 * half + (slot ^ 1u) : nullptr,
+            const SlowState x2 = slow_tile(tS, tO, f, see, bad, need ? 0.f : 4.f, m, l, t > 0 ? pv_done + 2 * half + (slot ^ 1u) : nullptr,
                                            ((tile - 1u) >> 1) & 1u, abort_flag);
             ok = x2.ok;
             if (!ok) break;
@@ -610,7 +611,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 10) tc::tmem_dealloc(tmem, 512);
+  if (warp == kIssue) tc::tmem_dealloc(tmem, 512);
 }
 
 // Query tiles that several blocks share: a warp a row, over the pieces of the blocks first .. b.
