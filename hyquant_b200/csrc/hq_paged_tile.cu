@@ -8,7 +8,7 @@
 // One block per SM, 15 warps:
 //   0-3, 4-7   softmax of the two halves, a thread per row; they also load the queries and write the results
 //   8-11       the cache: codes become fp16 values (exact: the format sees to that) in the swizzled operand tiles that both halves
-//              read, so that 64 keys are unpacked once for 256 rows; two warps take the even tiles, two the odd ones
+//              read, so that 64 keys are unpacked once for 256 rows
 //   12, 13     issue the products of a half each: S = Q K^T into one of two buffers of 64 columns, O += P V with P (fp16, over the
 //              buffer just read) from tensor memory and V's rows as they lie.  Q K^T of tile t + 2 follows P V of tile t.
 //   14         fetches the codes: a tile is four blocks of sixteen tokens, a bulk copy each, some tiles ahead
@@ -199,8 +199,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
   if (warp == kIssue) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 128); mbar_init(drained + i, 1); }
-      for (int i = 0; i < kStages; ++i) { mbar_init(k_full + i, 2); mbar_init(k_empty + i, 2); mbar_init(v_full + i, 2); mbar_init(v_empty + i, 2); }
-      for (int i = 0; i < kAhead; ++i) { mbar_init(c_full + i, 1); mbar_init(c_empty + i, 2); }
+      for (int i = 0; i < kStages; ++i) { mbar_init(k_full + i, 4); mbar_init(k_empty + i, 2); mbar_init(v_full + i, 4); mbar_init(v_empty + i, 2); }
+      for (int i = 0; i < kAhead; ++i) { mbar_init(c_full + i, 1); mbar_init(c_empty + i, 4); }
       for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_ready + i, 128); mbar_init(pv_done + i, 1); }
       *abort_flag = 0;
       fence_mbar_init();
@@ -373,37 +373,35 @@ tile_kernel(const AttnParams p, int piece_rows) {
     // ------------------------------------------------------------ the cache: codes to operand tiles
     // Lane: row lane / 4 of a group of eight keys, channels 32 (lane % 4) ..  A warp reads 512 bytes in one piece; the lanes of the
     // upper channels take their words two apart, so that no two of eight lanes write to the same banks either.
-    const int team = warp & 1, wt = (warp - 8) >> 1, rowl = lane >> 2, quarter = lane & 3, turn = quarter & 2;
+    const int w = warp - 8, rowl = lane >> 2, quarter = lane & 3, turn = quarter & 2;
     int n_all = 0;
     while (pc.take(p)) { n_all += pc.t1 - pc.t0; pc.done(p); }
+    int ks = 0;
+    uint32_t kpar = 1u;                          // empty barriers: the first round passes
     bool ok = true;
 #pragma unroll 1
-    for (int tile = team; ok && tile < n_all; tile += 2) {
-      const int cs = tile % kAhead, ks = tile % kStages;
-      const uint32_t kpar = (uint32_t)(tile / kStages + 1) & 1u;
+    for (int tile = 0; ok && tile < n_all; ++tile) {
+      const int cs = tile % kAhead;
       ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
       if (!ok) break;
-      const uint8_t* st = smem + TileSmem::Codes + cs * kCodeBytes;
-      const int info = key_rows[cs], rows = info & 0xFFFF;
+      const uint8_t* block = smem + TileSmem::Codes + cs * kCodeBytes + w * kBlockBytes;       // keys 16 w .. + 15
+      const int info = key_rows[cs], rows = ((info >> (16 + w)) & 1) ? 0 : (info & 0xFFFF) - kTok * w;
+      uint8_t* to = smem + TileSmem::K + ks * 16384 + (quarter >> 1) * 8192 + (kTok * w + rowl) * 128;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        uint4 val[4][4];
+        uint4 val[2][4];
         {
-          uint4 c[4];
-          float s[4];
-          bool any = false;
+          uint4 c[2];
+          float s[2];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {          // keys 8 (wt + 2 g) .. + 7: block g, its half wt
-            const uint8_t* block = st + g * kBlockBytes;
-            c[g] = *reinterpret_cast<const uint4*>(block + kv * kVOff + wt * 512 + lane * 16);
-            const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * wt + rowl));
-            const bool live = kTok * g + 8 * wt + rowl < rows && !((info >> (16 + g)) & 1);
-            s[g] = live ? __uint_as_float((uint32_t)sb << 16) : 0.f;       // keys that are not there: zeros, whatever lies here
-            any |= s[g] > 2048.f;
+          for (int g = 0; g < 2; ++g) {          // keys 16 w + 8 g .. + 7
+            c[g] = *reinterpret_cast<const uint4*>(block + kv * kVOff + g * 512 + lane * 16);
+            const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * g + rowl));
+            s[g] = 8 * g + rowl < rows ? __uint_as_float((uint32_t)sb << 16) : 0.f;        // keys that are not there: zeros, whatever lies here
           }
-          const bool big = __any_sync(0xffffffffu, any);
+          const bool big = __any_sync(0xffffffffu, s[0] > 2048.f || s[1] > 2048.f);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < 2; ++g) {
             const uint32_t cw[4] = {turn ? c[g].z : c[g].x, turn ? c[g].w : c[g].y, turn ? c[g].x : c[g].z, turn ? c[g].y : c[g].w};
             const __half2 s2 = __float2half2_rn(s[g]), s24 = __float2half2_rn(-24.f * s[g]);
             if (__builtin_expect(big, 0)) {
@@ -415,20 +413,23 @@ tile_kernel(const AttnParams p, int piece_rows) {
             }
           }
         }
-        // the values are in registers before their place is free: from then on it takes sixteen stores
+        // the values are in registers before their place is free: from then on it takes eight stores
         ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
-        uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384 + (quarter >> 1) * 8192 + (8 * wt + rowl) * 128;
-        if (ok)
+        if (ok) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
+          for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(to + g * 2048 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
+              *reinterpret_cast<uint4*>(to + kv * (TileSmem::V - TileSmem::K) + g * 1024 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (kv) tc::mbar_arrive(c_empty + cs);
+            tc::mbar_arrive((kv ? v_full : k_full) + ks);
+          }
+        }
       }
-      if (!ok) break;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) { tc::mbar_arrive(c_empty + cs); tc::mbar_arrive(k_full + ks); tc::mbar_arrive(v_full + ks); }
+      if (++ks == kStages) { ks = 0; kpar ^= 1u; }
     }
   } else {
     // ------------------------------------------------------------ softmax: a thread per row
