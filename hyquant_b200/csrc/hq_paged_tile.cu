@@ -2,18 +2,21 @@
 // tensor memory.
 //
 // A query tile is 256 rows of one kv head of one request - rows are (token, head of the group) pairs, one behind the other, whatever the
-// group size - in two halves of 128; keys come in tiles of 64.  Bound by the tensor pipe and the exponentials, which take about the
-// same time: 8.4 MFLOP and 16384 exponentials a tile pair, some 1024 clocks of an SM each at their nominal rates.
+// group size; keys come in tiles of 64.  The two halves of the softmax take 128 rows each, or, where a query tile has no more than
+// 128 rows, the same rows and every other key tile, and join their states at the end.  Bound by the tensor pipe and the exponentials,
+// which take about the same time: 8.4 MFLOP and 16384 exponentials a key tile of 256 rows, some 1024 clocks of an SM each at
+// their nominal rates.
 //
 // One block per SM, 15 warps:
 //   0-3, 4-7   softmax of the two halves, a thread per row; they also load the queries and write the results
 //   8-11       the cache: codes become fp16 values (exact: the format sees to that) in the swizzled operand tiles that both halves
 //              read, so that 64 keys are unpacked once for 256 rows
 //   12, 13     issue the products of a half each: S = Q K^T into one of two buffers of 64 columns, O += P V with P (fp16, over the
-//              buffer just read) from tensor memory and V's rows as they lie.  Q K^T of tile t + 2 follows P V of tile t.
+//              buffer just read) from tensor memory and V's rows as they lie.  Q K^T of the next tile but one follows P V.
 //   14         fetches the codes: a tile is four blocks of sixteen tokens, a bulk copy each, some tiles ahead
 // Channels stand in the order in which the unpacking produces them (0 4 1 5 2 6 3 7 in every eight), in Q, K and V alike; the rows that
-// are written put them back.
+// are written put them back.  What runs once per query tile is written as loops: straight-line code that is met cold costs more
+// for its instructions' way to the SM than for their execution (queries 6500 -> CLK1 clocks, results 10800 -> CLK2).
 //
 // All query tiles' keys in a row (requests, heads, query tiles) are cut evenly over the blocks, by position: lengths are only known
 // on the device, and no block is left with a long tile at the end.  A query tile that several blocks share leaves softmax states,
@@ -29,7 +32,7 @@ constexpr int kIssue = 12, kFetch = 14;          // first issuing warp; the fetc
 constexpr int kStages = 3;                       // K tiles, and V tiles, in shared memory
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
-constexpr int kItemCost = 2;                     // what a query tile costs beside its key tiles, in key tiles
+constexpr int kItemCost = 4;                     // positions that a query tile costs beside its key tiles
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
 constexpr uint32_t kTPolls = 400000u;
 
@@ -41,16 +44,18 @@ static_assert(TileSmem::Bar % 16 == 0 && TileSmem::Total + 1024 <= 227 * 1024, "
 
 struct TileMerge { int q0, rows, h, qt, first, go, unused[2]; };
 
-// A query tile and where in it a block's part begins
+// A query tile and where in it a block's part begins.  A key tile costs one position, or two where both halves work on it.
 struct Item {
-  int r, h, qt, n_qt, u, tiles;
+  int r, h, qt, n_qt, u, tiles, cost;
   Request q;
+  __device__ __forceinline__ int positions() const { return tiles * cost + kItemCost; }
 };
 __device__ __forceinline__ int query_tiles(const AttnParams& p, const Request& q) { return (q.nq * p.G + kRows - 1) / kRows; }
-__device__ __forceinline__ int key_tiles(const AttnParams& p, const Request& q, int qt) {
-  const int last = min(q.nq * p.G, (qt + 1) * kRows) - 1;
-  const int keys = min(q.len, q.past + 1 + last / p.G);
-  return keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
+__device__ __forceinline__ void size_item(const AttnParams& p, Item& x) {
+  const int rows = x.q.nq * p.G, last = min(rows, (x.qt + 1) * kRows) - 1;
+  const int keys = min(x.q.len, x.q.past + 1 + last / p.G);
+  x.tiles = keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
+  x.cost = rows - x.qt * kRows > 128 ? 2 : 1;
 }
 __device__ __forceinline__ void next_item(const AttnParams& p, Item& x) {
   x.u = 0;
@@ -65,7 +70,7 @@ __device__ __forceinline__ void next_item(const AttnParams& p, Item& x) {
       } while (x.n_qt == 0);
     }
   }
-  x.tiles = key_tiles(p, x.q, x.qt);
+  size_item(p, x);
 }
 // A block's part as pieces of query tiles: key tiles [t0, t1) of `it`
 struct Pieces {
@@ -75,23 +80,24 @@ struct Pieces {
   bool began, ends;                              // earlier, in another block; here
   __device__ __forceinline__ bool take(const AttnParams& p) {
     while (left > 0) {
-      const bool some = it.tiles > 0 ? it.u < it.tiles : it.u == 0;
-      if (some) {
-        began = it.u > 0;
-        t0 = it.u;
-        t1 = (int)min((long long)it.tiles, it.u + left);
-        ends = t1 == it.tiles;
-        return true;
-      }
+      const int to = (int)min((long long)it.tiles * it.cost, it.u + left);
+      t0 = (it.u + it.cost - 1) / it.cost;
+      t1 = (to + it.cost - 1) / it.cost;
+      began = it.u > 0;
+      ends = t1 == it.tiles;
+      if (t1 > t0 || (it.tiles == 0 && it.u == 0)) return true;
       done(p);
     }
     return false;
   }
   __device__ __forceinline__ void done(const AttnParams& p) {
-    left -= it.tiles + kItemCost - it.u;
+    left -= it.positions() - it.u;
     if (left > 0) next_item(p, it);
   }
+  __device__ __forceinline__ bool split() const { return it.cost == 1; }      // every other key tile to each half
 };
+// a / b for a >= 0, b > 0: 64-bit division only where it is needed
+__device__ __forceinline__ long long quotient(long long a, int b) { return (unsigned long long)a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
 
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
@@ -101,19 +107,28 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 struct SlowState { float m, l; bool ok; };
 
 // A tile that needs masks or a new reference: the scores are read again, the maximum taken, O rescaled where a row's reference
-// moves (where the maximum passes it by `slack`), P formed.  `lim`: keys of the tile that the row sees; bad: blocks of sixteen keys that are not there.
+// moves (where the maximum passes it by `slack`), P formed.  `lim`: keys of the tile that the row sees; bad: blocks of sixteen keys that are
+// not there.
 __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, int lim, uint32_t bad, float slack, float m, float l,
                                             uint64_t* pv_bar, uint32_t pv_parity, volatile int* abort_flag) {
   SlowState out{m, l, true};
-  float x[64];
-  tc::tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-  tc::tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
-  tc::tmem_wait_ld();
-  float mx = -INFINITY;
+  uint32_t see[2];
 #pragma unroll
-  for (int c = 0; c < 64; ++c) {
-    x[c] = (c < lim && !((bad >> (c >> 4)) & 1u)) ? x[c] * f : -INFINITY;
-    mx = fmaxf(mx, x[c]);
+  for (int c = 0; c < 2; ++c) {
+    const int n = lim - 32 * c;
+    see[c] = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+    if ((bad >> (2 * c)) & 1u) see[c] &= 0xFFFF0000u;
+    if ((bad >> (2 * c + 1)) & 1u) see[c] &= 0x0000FFFFu;
+  }
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    float x[32];
+    tc::tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+    tc::tmem_wait_ld();
+    const uint32_t mask = c ? see[1] : see[0];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (mask >> e) & 1u ? x[e] * f : -INFINITY);
   }
   const bool grow = mx > m + slack;
   if (__any_sync(0xffffffffu, grow)) {
@@ -121,7 +136,7 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
     if (pv_bar != nullptr) {                     // O must be quiescent
       if (!wait_warp(pv_bar, pv_parity, abort_flag)) { out.ok = false; return out; }
       tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 1
       for (int ch = 0; ch < 4; ++ch) {
         uint32_t o[32];
         tc::tmem_ld32(tO + ch * 32, o);
@@ -136,43 +151,46 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
     if (grow) out.m = mx;
   }
   const float shift = out.m == -INFINITY ? 0.f : kTShift - out.m;
-  uint32_t pk[32];
   float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {                  // P of columns 32 c .. lands in columns 16 c .., which have been read
+    float x[32];
+    tc::tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+    tc::tmem_wait_ld();
+    const uint32_t mask = c ? see[1] : see[0];
+    uint32_t pk[16];
 #pragma unroll
-  for (int c = 0; c < 64; c += 2) {
-    const float p0 = ex2f(x[c] + shift), p1 = ex2f(x[c + 1] + shift);
-    sum += p0 + p1;
-    const __half2 hh = __floats2half2_rn(p0, p1);
-    pk[c >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
+    for (int e = 0; e < 32; e += 2) {
+      const float p0 = ex2f(((mask >> e) & 1u ? x[e] * f : -INFINITY) + shift), p1 = ex2f(((mask >> (e + 1)) & 1u ? x[e + 1] * f : -INFINITY) + shift);
+      sum += p0 + p1;
+      const __half2 hh = __floats2half2_rn(p0, p1);
+      pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
+    }
+    tc::tmem_st16(tS + 16 * c, pk);
   }
-  tc::tmem_st32(tS, pk);
   tc::tmem_wait_st();
   out.l += sum;
   return out;
 }
 
-// eight codes -> eight values in the order 0 4 1 5 2 6 3 7: the nibble at the top of the mantissa is 16 + (code + 8), one fma takes 24
-// scales off.  24 * scale and the result have at most ten and eleven bits: exact for scales up to 2048 (24 * scale is an fp16 number).
-__device__ __forceinline__ uint4 values8(uint32_t w, __half2 s, __half2 s24) {
-  const uint32_t x0 = lop3_and_xor(w << 6, 0x03C003C0u, 0x4E004E00u), x1 = lop3_and_xor(w << 2, 0x03C003C0u, 0x4E004E00u);
-  const uint32_t x2 = lop3_and_xor(w >> 2, 0x03C003C0u, 0x4E004E00u), x3 = lop3_and_xor(w >> 6, 0x03C003C0u, 0x4E004E00u);
-  auto val = [&](uint32_t x) {
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&x), s, s24);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  };
-  return make_uint4(val(x0), val(x1), val(x2), val(x3));
+// Eight codes -> eight values in the order 0 4 1 5 2 6 3 7.  Nibbles in the low mantissa bits are 1024 + 8 + code, or 1024 + 16 (8 + code)
+// four bits up; the code is taken out exactly and its product with the scale is an fp16 number.
+struct Unpack { uint32_t lo, hi, lo8, hi8; };
+__device__ __forceinline__ uint4 values8(const Unpack& k, uint32_t w, __half2 s) {
+  const uint32_t w8 = w >> 8;
+  auto h2 = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
+  auto u32 = [](__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); };
+  const __half2 c1032 = h2(0xE408E408u), c16th = h2(0x2C002C00u), c72 = h2(0xD480D480u);       // -1032, 1 / 16, -72
+  return make_uint4(u32(__hmul2(__hadd2(h2(lop3_and_xor(w, k.lo, k.lo8)), c1032), s)),
+                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w, k.hi, k.hi8)), c16th, c72), s)),
+                    u32(__hmul2(__hadd2(h2(lop3_and_xor(w8, k.lo, k.lo8)), c1032), s)),
+                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w8, k.hi, k.hi8)), c16th, c72), s)));
 }
-// the same for any scale: the code by itself first
-__device__ __forceinline__ uint4 values8_any(uint32_t w, __half2 s) {
-  const uint32_t x0 = lop3_and_xor(w << 6, 0x03C003C0u, 0x4E004E00u), x1 = lop3_and_xor(w << 2, 0x03C003C0u, 0x4E004E00u);
-  const uint32_t x2 = lop3_and_xor(w >> 2, 0x03C003C0u, 0x4E004E00u), x3 = lop3_and_xor(w >> 6, 0x03C003C0u, 0x4E004E00u);
-  const __half2 c24 = __float2half2_rn(24.f);
-  auto val = [&](uint32_t x) {
-    const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&x), c24), s);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  };
-  return make_uint4(val(x0), val(x1), val(x2), val(x3));
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void halves_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the eight softmax warps
 
 template <bool kBf16>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -194,6 +212,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ long long s_part[kTileThreads + 1], s_warp[kTileThreads / 32];
+  __shared__ float2 s_state[2][128];             // (maximum, sum) of a half's rows, for the other
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (warp == kIssue) {
@@ -213,58 +232,64 @@ tile_kernel(const AttnParams p, int piece_rows) {
 
   // ---- where this block's part lies
   auto weight = [&](const Request& q) {
-    long long w = 0;
-    for (int qt = 0, n = query_tiles(p, q); qt < n; ++qt) w += key_tiles(p, q, qt) + kItemCost;
+    Item x;
+    x.q = q;
+    int w = 0;
+    for (x.qt = 0, x.n_qt = query_tiles(p, q); x.qt < x.n_qt; ++x.qt) { size_item(p, x); w += x.positions(); }
     return w;
   };
   const int per = (p.R + kTileThreads - 1) / kTileThreads;
   long long mine = 0;
-  for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += p.H_KV * weight(request_of(p, r));
+  for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += (long long)p.H_KV * weight(request_of(p, r));
   long long x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < kTileThreads / 32; ++w) { if (w < warp) before += s_warp[w]; total += s_warp[w]; }
+  long long sums = lane < kTileThreads / 32 ? s_warp[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, sums, o); if (lane >= o) sums += y; }
+  const long long total = __shfl_sync(0xffffffffu, sums, 31), before = warp ? __shfl_sync(0xffffffffu, sums, (warp + 31) & 31) : 0;
   s_part[tid + 1] = before + x;
   if (tid == 0) s_part[0] = 0;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const int blocks = (int)max(1ll, min((long long)gridDim.x, total / (kItemCost + 1))), block = blockIdx.x;
+  // block b's part: total / blocks positions, one more for the first total % blocks
+  const int blocks = (int)max(1ll, min((long long)gridDim.x, quotient(total, kItemCost + 2))), block = blockIdx.x;
+  const long long share = quotient(total, blocks);
+  const int more = (int)(total - share * blocks);
+  const long long b0 = share * block + min(block, more);
   const int64_t piece_floats = (int64_t)piece_rows * 130;
   TileMerge* todo = reinterpret_cast<TileMerge*>(p.ws + 2 * piece_floats * gridDim.x) + block;
-  const long long b0 = block < blocks ? total * block / blocks : 0, b1 = block < blocks ? total * (block + 1) / blocks : 0;
   if (tid == 0) todo->go = 0;
   Pieces pc;
-  pc.left = b1 - b0;
+  pc.left = block < blocks ? share + (block < more ? 1 : 0) : 0;
   if (pc.left > 0) {
     int lo = 0, hi = kTileThreads;
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= b0) lo = mid; else hi = mid; }
-    long long at = s_part[lo];
+    long long in = b0 - s_part[lo];
     Item it;
     it.r = lo * per;
-    long long w;
+    int w;
     for (;; ++it.r) {
       it.q = request_of(p, it.r);
       w = weight(it.q);
-      if (b0 < at + w * p.H_KV) break;
-      at += w * p.H_KV;
+      if (in < (long long)w * p.H_KV) break;
+      in -= (long long)w * p.H_KV;
     }
-    it.h = (int)((b0 - at) / w);
-    long long in = b0 - at - it.h * w;
+    it.h = (int)quotient(in, w);
+    in -= (long long)it.h * w;
     it.n_qt = query_tiles(p, it.q);
     for (it.qt = 0;; ++it.qt) {
-      it.tiles = key_tiles(p, it.q, it.qt);
-      if (in < it.tiles + kItemCost) break;
-      in -= it.tiles + kItemCost;
+      size_item(p, it);
+      if (in < it.positions()) break;
+      in -= it.positions();
     }
     it.u = (int)in;
     pc.it = it;
   }
-
   int* key_rows = reinterpret_cast<int*>(smem + TileSmem::Rows);           // [kAhead] keys of a tile that are there, the last ones missing
   uint8_t* bads = smem + TileSmem::Bad;                                    // [16] blocks of a tile whose page is not there
   if (warp == kFetch) {
@@ -309,60 +334,54 @@ tile_kernel(const AttnParams p, int piece_rows) {
     const uint64_t dQ = tc::smem_desc_k128(smem + TileSmem::Q + half * 32768, 0);
     const uint64_t dK = tc::smem_desc_k128(smem + TileSmem::K, 0), dV = tc::smem_desc_mn128(smem + TileSmem::V, 8192);
     const uint32_t tS = tmem + 128u * half, tO = tmem + 256u + 128u * half;
-    int ks = 0, vs = 0;
-    uint32_t kpar = 0, vpar = 0, tile = 0, q_par = 0;       // tile: of this half, over all pieces
+    uint32_t tile = 0, q_par = 0, ring = 0;      // tiles of this half and of the block so far
     bool ok = true;
-    auto k_step = [&]() { if (++ks == kStages) { ks = 0; kpar ^= 1u; } };
-    auto v_step = [&]() { if (++vs == kStages) { vs = 0; vpar ^= 1u; } };
     while (ok && pc.take(p)) {
-      const int n = pc.t1 - pc.t0, rows = pc.it.q.nq * p.G - pc.it.qt * kRows - 128 * half;
-      if (n > 0 && rows <= 0) {                  // the other half's tiles: handed back as they come
-        for (int t = 0; ok && t < n; ++t) {
-          ok = wait_warp(k_full + ks, kpar, abort_flag);
-          if (ok && tc::elect_one()) tc::mbar_arrive(k_empty + ks);
-          ok = ok && wait_warp(v_full + vs, vpar, abort_flag);
-          if (ok && tc::elect_one()) tc::mbar_arrive(v_empty + vs);
-          k_step(); v_step();
-        }
-      } else if (n > 0) {
+      const int n_all = pc.t1 - pc.t0, first = pc.split() ? half : 0, step = pc.split() ? 2 : 1, n = (n_all - first + step - 1) / step;
+      if (n > 0) {
         ok = wait_warp(q_full + half, q_par, abort_flag);
         q_par ^= 1u;
-        uint32_t tq = tile;
+        int tq = 0;
+        // a slot goes back when both halves have arrived; a half that has a tile to itself arrives twice
+        auto hand_back = [&](uint64_t* bar) { tc::mma_commit(bar); if (step == 2) tc::mma_commit(bar); };
         auto qk = [&]() {
-          ok = ok && wait_warp(k_full + ks, kpar, abort_flag);
+          const uint32_t at = ring + (uint32_t)(first + step * tq), ks = at % kStages, slot = (tile + (uint32_t)tq) & 1u;
+          ok = ok && wait_warp(k_full + ks, (at / kStages) & 1u, abort_flag);
           if (!ok) return;
           tc::fence_after_sync();
           if (tc::elect_one()) {
-            const uint32_t dS = tS + 64u * (tq & 1u);
+            const uint32_t dS = tS + 64u * slot;
             const uint64_t bK = dK + (uint64_t)(ks * 1024);
 #pragma unroll
             for (int k = 0; k < 8; ++k) tc::mma_bf16_ss(dS, dQ + (k >> 2) * 1024 + 2 * (k & 3), bK + (k >> 2) * 512 + 2 * (k & 3), idesc_qk, k > 0);
-            tc::mma_commit(k_empty + ks);
-            tc::mma_commit(s_full + 2 * half + (tq & 1u));
+            hand_back(k_empty + ks);
+            tc::mma_commit(s_full + 2 * half + slot);
           }
           __syncwarp();
           ++tq;
-          k_step();
         };
         qk();
         if (n > 1) qk();
-        for (int t = 0; ok && t < n; ++t, ++tile) {
-          ok = wait_warp(v_full + vs, vpar, abort_flag) && wait_warp(p_ready + 2 * half + (tile & 1u), (tile >> 1) & 1u, abort_flag);
+        for (int t = 0; ok && t < n; ++t) {
+          const uint32_t at = ring + (uint32_t)(first + step * t), vs = at % kStages, slot = (tile + (uint32_t)t) & 1u;
+          ok = wait_warp(v_full + vs, (at / kStages) & 1u, abort_flag) &&
+               wait_warp(p_ready + 2 * half + slot, ((tile + (uint32_t)t) >> 1) & 1u, abort_flag);
           if (!ok) break;
           tc::fence_after_sync();
           if (tc::elect_one()) {
-            const uint32_t aP = tS + 64u * (tile & 1u);
+            const uint32_t aP = tS + 64u * slot;
             const uint64_t bV = dV + (uint64_t)(vs * 1024);
 #pragma unroll
             for (int k = 0; k < 4; ++k) tc::mma_bf16_ts(tO, aP + 8 * k, bV + 128 * k, idesc_pv, (t > 0 || k > 0) ? 1u : 0u);
-            tc::mma_commit(v_empty + vs);
-            tc::mma_commit(pv_done + 2 * half + (tile & 1u));
+            hand_back(v_empty + vs);
+            tc::mma_commit(pv_done + 2 * half + slot);
           }
           __syncwarp();
-          v_step();
           if (t + 2 < n) qk();
         }
+        tile += (uint32_t)n;
       }
+      ring += (uint32_t)n_all;
       pc.done(p);
     }
     // nothing may still write tensor memory or arrive on a barrier when the block ends
@@ -374,109 +393,114 @@ tile_kernel(const AttnParams p, int piece_rows) {
     // Lane: row lane / 4 of a group of eight keys, channels 32 (lane % 4) ..  A warp reads 512 bytes in one piece; the lanes of the
     // upper channels take their words two apart, so that no two of eight lanes write to the same banks either.
     const int w = warp - 8, rowl = lane >> 2, quarter = lane & 3, turn = quarter & 2;
+    Unpack uk;                                   // kept in registers: as constants they are loaded again beside every use
+    asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(uk.lo));
+    asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(uk.hi));
+    asm volatile("mov.b32 %0, 0x64086408;" : "=r"(uk.lo8));
+    asm volatile("mov.b32 %0, 0x64806480;" : "=r"(uk.hi8));
     int n_all = 0;
     while (pc.take(p)) { n_all += pc.t1 - pc.t0; pc.done(p); }
     int ks = 0;
     uint32_t kpar = 1u;                          // empty barriers: the first round passes
     bool ok = true;
+    // K and V of a tile in turn.  The values are in registers before their place is free; a part's stores are made visible to the
+    // tensor core behind the arithmetic of the next part, when they are long done.
+    uint64_t* due = nullptr;
+    auto hand_over = [&]() {
+      if (due == nullptr) return;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(due);
+    };
 #pragma unroll 1
     for (int tile = 0; ok && tile < n_all; ++tile) {
       const int cs = tile % kAhead;
-      ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
-      if (!ok) break;
+      const uint32_t cpar = (uint32_t)(tile / kAhead) & 1u;
+      if (!__all_sync(0xffffffffu, mbar_test_wait(c_full + cs, cpar))) {      // nothing to do meanwhile
+        hand_over();
+        due = nullptr;
+        ok = wait_warp(c_full + cs, cpar, abort_flag);
+        if (!ok) break;
+      }
       const uint8_t* block = smem + TileSmem::Codes + cs * kCodeBytes + w * kBlockBytes;       // keys 16 w .. + 15
       const int info = key_rows[cs], rows = ((info >> (16 + w)) & 1) ? 0 : (info & 0xFFFF) - kTok * w;
       uint8_t* to = smem + TileSmem::K + ks * 16384 + (quarter >> 1) * 8192 + (kTok * w + rowl) * 128;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         uint4 val[2][4];
-        {
-          uint4 c[2];
-          float s[2];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {          // keys 16 w + 8 g .. + 7
-            c[g] = *reinterpret_cast<const uint4*>(block + kv * kVOff + g * 512 + lane * 16);
-            const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * g + rowl));
-            s[g] = 8 * g + rowl < rows ? __uint_as_float((uint32_t)sb << 16) : 0.f;        // keys that are not there: zeros, whatever lies here
-          }
-          const bool big = __any_sync(0xffffffffu, s[0] > 2048.f || s[1] > 2048.f);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const uint32_t cw[4] = {turn ? c[g].z : c[g].x, turn ? c[g].w : c[g].y, turn ? c[g].x : c[g].z, turn ? c[g].y : c[g].w};
-            const __half2 s2 = __float2half2_rn(s[g]), s24 = __float2half2_rn(-24.f * s[g]);
-            if (__builtin_expect(big, 0)) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) val[g][k] = values8_any(cw[k], s2);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) val[g][k] = values8(cw[k], s2, s24);
-            }
-          }
+        for (int g = 0; g < 2; ++g) {            // keys 16 w + 8 g .. + 7
+          const uint8_t* c = block + kv * kVOff + g * 512 + lane * 16;
+          const uint2 c0 = *reinterpret_cast<const uint2*>(c + 4 * turn), c1 = *reinterpret_cast<const uint2*>(c + 8 - 4 * turn);
+          const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * g + rowl));
+          // keys that are not there: zeros, whatever lies here
+          const __half2 s = __float2half2_rn(8 * g + rowl < rows ? __uint_as_float((uint32_t)sb << 16) : 0.f);
+          val[g][0] = values8(uk, c0.x, s); val[g][1] = values8(uk, c0.y, s);
+          val[g][2] = values8(uk, c1.x, s); val[g][3] = values8(uk, c1.y, s);
         }
-        // the values are in registers before their place is free: from then on it takes eight stores
+        hand_over();
         ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
+        due = nullptr;
         if (ok) {
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               *reinterpret_cast<uint4*>(to + kv * (TileSmem::V - TileSmem::K) + g * 1024 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (kv) tc::mbar_arrive(c_empty + cs);
-            tc::mbar_arrive((kv ? v_full : k_full) + ks);
-          }
+          due = (kv ? v_full : k_full) + ks;
         }
       }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(c_empty + cs);
       if (++ks == kStages) { ks = 0; kpar ^= 1u; }
     }
+    hand_over();
   } else {
     // ------------------------------------------------------------ softmax: a thread per row
     const int half = warp >> 2, wq = warp & 3, r = wq * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(wq * 32) << 16), tO = lane_base + 256u + 128u * half;
     uint8_t* sQ = smem + TileSmem::Q + half * 32768;
-    uint32_t tile = 0, all = 0;                  // tiles of this half; of the block
+    uint32_t tile = 0, all = 0;                  // tiles of this half and of the block so far
     bool ok = true;
     while (pc.take(p)) {
       const Request& q = pc.it.q;
-      const int n = pc.t1 - pc.t0, rows = min(128, q.nq * p.G - pc.it.qt * kRows - 128 * half);
-      const int row = pc.it.qt * kRows + 128 * half + r, i = row / p.G, gh = pc.it.h * p.G + row - i * p.G;
+      const bool split = pc.split();
+      const int row0 = pc.it.qt * kRows + (split ? 0 : 128 * half), rows = min(128, q.nq * p.G - row0);
+      const int n_all = pc.t1 - pc.t0, first = split ? half : 0, step = split ? 2 : 1, n = (n_all - first + step - 1) / step;
+      const int row = row0 + r, i = row / p.G;
       float m = -INFINITY, l = 0.f;
-      if (n > 0 && rows > 0 && ok) {
+      if (n > 0 && ok) {
         // queries: scaled by a power of two of the row so that fp16 holds them exactly, into the operand tile
-        float f;
-        {
-          const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st + (int64_t)gh * p.q_sh;
-          const bool live = r < rows;
-          auto value = [&](uint32_t u, int hi) {
-            if (kBf16) return __uint_as_float(hi ? u & 0xFFFF0000u : u << 16);
-            return __half2float(__ushort_as_half((unsigned short)(hi ? u >> 16 : u & 0xFFFFu)));
-          };
-          float top = 0.f;
-          uint4 raw[16];
+        uint8_t* mine = sQ + r * 128;
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + (r < rows ? i : 0)) * p.q_st +
+                               (int64_t)(pc.it.h * p.G + (r < rows ? row - i * p.G : 0)) * p.q_sh;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) raw[c] = live ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < 16; ++c) cp_async16(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4), from + 8 * c, r < rows);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        uint32_t top2 = 0u;                      // magnitudes of 16-bit numbers order like integers
+#pragma unroll 4
+        for (int c = 0; c < 16; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
+          top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, u.x & 0x7FFF7FFFu), u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+        }
+        auto value = [&](uint32_t u, int hi) {
+          if (kBf16) return __uint_as_float(hi ? u & 0xFFFF0000u : u << 16);
+          return __half2float(__ushort_as_half((unsigned short)(hi ? u >> 16 : u & 0xFFFFu)));
+        };
+        const float top = value(max(top2 & 0xFFFFu, top2 >> 16), 0);
+        const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 255 ? 0 : 140 - max(ex, 14);       // largest magnitude to [2^13, 2^14)
+        const float scale = __uint_as_float((uint32_t)(127 + up) << 23), f = p.sml * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll 2
+        for (int c = 0; c < 16; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
+          const uint32_t u[4] = {at->x, at->y, at->z, at->w};
+          uint32_t o[4];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(value(u[k], 0)), fabsf(value(u[k], 1))));
+          for (int k = 0; k < 4; ++k) {          // channels k and k + 4 of the eight
+            const __half2 hh = __floats2half2_rn(value(u[k >> 1], k & 1) * scale, value(u[2 + (k >> 1)], k & 1) * scale);
+            o[k] = *reinterpret_cast<const uint32_t*>(&hh);
           }
-          const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 255 ? 0 : 140 - max(ex, 14);       // largest magnitude to [2^13, 2^14)
-          const float scale = __uint_as_float((uint32_t)(127 + up) << 23);
-          f = p.sml * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {        // channels k and k + 4 of the eight
-              const __half2 hh = __floats2half2_rn(value(u[k >> 1], k & 1) * scale, value(u[2 + (k >> 1)], k & 1) * scale);
-              o[k] = *reinterpret_cast<const uint32_t*>(&hh);
-            }
-            *reinterpret_cast<uint4*>(sQ + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          }
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         tc::mbar_arrive(q_full + half);
@@ -490,8 +514,9 @@ tile_kernel(const AttnParams p, int piece_rows) {
           if (!ok) break;
           tc::fence_after_sync();
           const uint32_t tS = lane_base + 128u * half + 64u * slot;
-          const uint32_t bad = bads[(all + t) & 15u];
-          const int see = lim - (pc.t0 + t) * kKeys;
+          const int at = first + step * t;
+          const uint32_t bad = bads[(all + (uint32_t)at) & 15u];
+          const int see = lim - (pc.t0 + at) * kKeys;
           const bool masks = __any_sync(0xffffffffu, see < kKeys || bad != 0u);
           bool need = false;
           uint32_t pk[32];
@@ -531,25 +556,55 @@ tile_kernel(const AttnParams p, int piece_rows) {
           tc::mbar_arrive(p_ready + 2 * half + slot);
         }
         if (ok) ok = wait_warp(pv_done + 2 * half + ((tile - 1u) & 1u), ((tile - 1u) >> 1) & 1u, abort_flag);
-        tc::fence_after_sync();
       }
-      all += (uint32_t)n;
-      if (rows > 0) {
-        // O leaves through the rows' own part of the query tile, 32 columns at a time, so that a store writes whole sectors
+      all += (uint32_t)n_all;
+      if (!ok) { m = 0.f; l = __int_as_float(0x7FC00000); }            // gave up: the rows are NaN
+      // weights of this half's O and of the other's, where both have some
+      float wa = n > 0 && ok ? 1.f : 0.f, wb = 0.f;
+      const bool other = split && n_all > 1;     // (a half without tiles has no O)
+      if (split) {
+        s_state[half][r] = make_float2(m, l);
+        tc::fence_before_sync();
+        halves_meet();
+        const float2 o = s_state[half ^ 1][r];
+        const float M = fmaxf(m, o.x), ref = M == -INFINITY ? 0.f : M;
+        wa = ex2f(m - ref); wb = ex2f(o.x - ref);
+        l = l * wa + o.y * wb;
+        m = M;
+        if (l != l) { wa = l; wb = l; }
+      }
+      tc::fence_after_sync();
+      {
+        // O leaves through the rows' own part of the query tile, 32 columns at a time, so that a store writes whole sectors.  Halves
+        // that share their rows take two of the four parts each.
         const bool whole = !pc.began && pc.ends;
-        if (!ok) { m = 0.f; l = __int_as_float(0x7FC00000); }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l, fa = whole ? wa * inv : wa, fb = whole ? wb * inv : wb;
         float* piece = p.ws + (int64_t)(2 * block + (pc.began ? 0 : 1)) * piece_floats;
+        const int prow0 = row0 - pc.it.qt * kRows;
         uint8_t* stage = sQ + wq * 32 * 128;     // of the first half of the channels: 4 KB that only this warp touches
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
+        const uint32_t tOther = lane_base + 256u + 128u * (half ^ 1);
+#pragma unroll 1
+        for (int ch = split ? 2 * half : 0; ch < (split ? 2 * half + 2 : 4); ++ch) {
           float o[32];
-          if (n > 0 && ok) {
+          if (split ? (half == 0 || other) : n > 0) {
             tc::tmem_ld32(tO + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
             tc::tmem_wait_ld();
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (n_all == 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= fa;
+          if (split && n_all > (half == 0 ? 1 : 0)) {
+            float o2[32];
+            tc::tmem_ld32(tOther + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&o2[0]));
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(o2[e], fb, o[e]);
           }
           __syncwarp();
           // column 8 k + 2 j + b holds channel 8 k + 4 b + j
@@ -559,8 +614,6 @@ tile_kernel(const AttnParams p, int piece_rows) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) { v[j] = o[8 * k + 2 * j]; v[4 + j] = o[8 * k + 2 * j + 1]; }
             if (whole) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = ok ? v[j] * inv : __int_as_float(0x7FC00000);
               uint32_t u[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -575,37 +628,33 @@ tile_kernel(const AttnParams p, int piece_rows) {
           }
           __syncwarp();
           if (whole) {                           // four lanes a row, 64 bytes
-#pragma unroll
-            for (int x8 = 0; x8 < 4; ++x8) {
-              const int rr = 8 * x8 + (lane >> 2), part = lane & 3, orow = wq * 32 + rr;
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((part ^ (rr & 7)) << 4));
-              if (orow < rows) {
-                const int grow = pc.it.qt * kRows + 128 * half + orow, gi = grow / p.G;
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(q.q0 + gi) * p.o_st +
-                                          (int64_t)(pc.it.h * p.G + grow - gi * p.G) * p.o_sh + ch * 32 + part * 8) = v;
-              }
+#pragma unroll 1
+            for (int rr = lane >> 2; rr < 32 && wq * 32 + rr < rows; rr += 8) {
+              const int part = lane & 3, orow = row0 + wq * 32 + rr, gi = orow / p.G;
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(q.q0 + gi) * p.o_st +
+                                        (int64_t)(pc.it.h * p.G + orow - gi * p.G) * p.o_sh + ch * 32 + part * 8) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((part ^ (rr & 7)) << 4));
             }
           } else {                               // eight lanes a row, 128 bytes
-#pragma unroll
-            for (int x4 = 0; x4 < 8; ++x4) {
-              const int rr = 4 * x4 + (lane >> 3), part = lane & 7, orow = wq * 32 + rr;
-              const float4 v = *reinterpret_cast<const float4*>(stage + rr * 128 + ((part ^ (rr & 7)) << 4));
-              if (orow < rows) *reinterpret_cast<float4*>(piece + (int64_t)(128 * half + orow) * 128 + ch * 32 + part * 4) = v;
+#pragma unroll 2
+            for (int rr = lane >> 3; rr < 32 && wq * 32 + rr < rows; rr += 4) {
+              const int part = lane & 7;
+              *reinterpret_cast<float4*>(piece + (int64_t)(prow0 + wq * 32 + rr) * 128 + ch * 32 + part * 4) =
+                  *reinterpret_cast<const float4*>(stage + rr * 128 + ((part ^ (rr & 7)) << 4));
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
-        if (!whole && r < rows) {
-          piece[(int64_t)piece_rows * 128 + 128 * half + r] = m;
-          piece[(int64_t)piece_rows * 129 + 128 * half + r] = l;
+        if (!whole && r < rows && !(split && half)) {
+          piece[(int64_t)piece_rows * 128 + prow0 + r] = m;
+          piece[(int64_t)piece_rows * 129 + prow0 + r] = l;
         }
       }
+      if (split) { tc::fence_before_sync(); halves_meet(); }           // the other half has read this one's O and state
       if (pc.began && pc.ends && tid == 0) {
-        const long long start = b0 - pc.t0;      // the block's first piece: its query tile began t0 positions before
-        int first = (int)(start * blocks / total);
-        while (total * first / blocks > start) --first;
-        while (total * (first + 1) / blocks <= start) ++first;
-        *todo = TileMerge{q.q0, min(kRows, q.nq * p.G - pc.it.qt * kRows), pc.it.h, pc.it.qt, first, 1, {0, 0}};
+        const long long start = b0 - pc.it.u;    // where the query tile begins: the block of that position has its first piece
+        int first_block = (int)(start < (share + 1) * more ? quotient(start, (int)(share + 1)) : more + quotient(start - (share + 1) * more, (int)share));
+        *todo = TileMerge{q.q0, min(kRows, q.nq * p.G - pc.it.qt * kRows), pc.it.h, pc.it.qt, first_block, 1, {0, 0}};
       }
       pc.done(p);
     }
