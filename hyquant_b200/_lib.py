@@ -149,8 +149,8 @@ def _declare(lib):
     lib.hq_page_advance.argtypes = [vp, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.hq_paged_append.argtypes = [vp, vp, i32, i64, i64, i64, i64, i32, i32, vp, vp, i64, i32, vp]
     lib.hq_paged_read.argtypes = [vp, i64, i32, vp, i32, i32, i32, vp, vp, vp]
-    lib.hq_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionArgs), C.POINTER(i64)]
-    lib.hq_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs), vp]
+    lib.hq_paged_attention_workspace_bytes.argtypes = [vp, C.POINTER(i64)]       # PagedAttentionArgs by reference, or its bytes
+    lib.hq_paged_attention.argtypes = [vp, vp]
     lib.hq_tc_peak.argtypes = [i32, i32, vp, C.POINTER(C.c_int), vp]
     lib.hq_peer_exchange_bytes.argtypes = [i32, i32, C.POINTER(i64)]
     lib.hq_peer_slot.argtypes = [vp, i32, i32, C.c_uint32, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]

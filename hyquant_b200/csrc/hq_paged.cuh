@@ -27,7 +27,7 @@ struct AttnParams {
   int R, T, H_Q, H_KV, G, page_shift, max_pages, max_q_len;
   float sml;                                   // sm_scale * log2(e)
   int dtype;
-  int64_t num_pages;
+  int num_pages, page_bytes, blocks_mask;      // bytes of a page of one head; its blocks - 1
   const void* q; int64_t q_st, q_sh;
   const uint8_t* pages;
   const int* table; int64_t table_stride;
@@ -115,6 +115,81 @@ __device__ __forceinline__ Request request_of(const AttnParams& p, int r) {
   x.past = x.len - n;
   return x;
 }
+
+// a / b for a >= 0, b > 0: 64-bit division only where it is needed
+__device__ __forceinline__ long long quotient(long long a, int b) {
+  return (unsigned long long)a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
+// Even cuts of `total` positions over the blocks of a launch: block b has `share` of them from share * b + min(b, more) on, the first
+// `more` blocks one more.
+struct Cuts {
+  long long total, share;
+  int blocks, more;
+  __device__ __forceinline__ Cuts(long long t, int n) : total(t), blocks(n) { share = quotient(t, n); more = (int)(t - share * n); }
+  __device__ __forceinline__ long long begin(int b) const { return share * b + min(b, more); }
+  __device__ __forceinline__ int block_of(long long pos) const {
+    const long long cut = (share + 1) * more;
+    return (int)(pos < cut ? quotient(pos, (int)(share + 1)) : more + quotient(pos - cut, (int)share));
+  }
+};
+
+// The requests' weights in a row.  Up to 64 requests every warp adds them up by itself; more go through shared memory (s_part: threads + 1,
+// s_warp: a word per warp), a run of requests per thread.  All threads call the constructor, whole warps `seek`.
+template <int kThreads, class Weight>
+struct Prefix {
+  const AttnParams& p;
+  Weight weight;
+  long long total;
+  const long long* s_part;
+  long long w0, w1;                              // up to 64 requests: running sums at request `lane` and 32 + `lane`
+  int per;
+  __device__ __forceinline__ static long long scan(long long x) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    return x;
+  }
+  __device__ __forceinline__ Prefix(const AttnParams& pp, Weight w, long long* part, long long* s_warp) : p(pp), weight(w), s_part(part) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (p.R <= 64) {
+      w0 = lane < p.R ? weight(request_of(p, lane)) : 0;
+      w1 = 32 + lane < p.R ? weight(request_of(p, 32 + lane)) : 0;
+      w0 = scan(w0);
+      w1 = scan(w1) + __shfl_sync(0xffffffffu, w0, 31);
+      total = __shfl_sync(0xffffffffu, w1, 31);
+      return;
+    }
+    per = (p.R + kThreads - 1) / kThreads;
+    long long mine = 0;
+    for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += weight(request_of(p, r));
+    const long long x = scan(mine);
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    const long long sums = scan(lane < kThreads / 32 ? s_warp[lane] : 0), before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+    total = __shfl_sync(0xffffffffu, sums, 31);
+    part[tid + 1] = x + (warp ? before : 0);
+    if (tid == 0) part[0] = 0;
+    __syncthreads();
+  }
+  // the request that position pos < total lies in, and the position in it
+  __device__ __forceinline__ int seek(long long pos, long long& in) const {
+    if (p.R <= 64) {
+      const int a = __popc(__ballot_sync(0xffffffffu, w0 <= pos)), b = __popc(__ballot_sync(0xffffffffu, w1 <= pos)), r = a < 32 ? a : 32 + b;
+      const long long below = r == 0 ? 0 : r <= 32 ? __shfl_sync(0xffffffffu, w0, r - 1) : __shfl_sync(0xffffffffu, w1, r - 33);
+      in = pos - below;
+      return r;
+    }
+    int lo = 0, hi = kThreads;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= pos) lo = mid; else hi = mid; }
+    in = pos - s_part[lo];
+    for (int r = lo * per;; ++r) {
+      const long long w = weight(request_of(p, r));
+      if (in < w) return r;
+      in -= w;
+    }
+  }
+};
 
 // first byte of the sixteen-token block of `slot` (page * page_size + position in the page) of head `h`
 __device__ __forceinline__ int64_t block_offset(int64_t slot, int h, int H, int page_shift) {

@@ -39,7 +39,7 @@ static AttnParams params_of(const hq_paged_attention_args* a) {
   p.R = a->R; p.T = a->T; p.H_Q = a->H_Q; p.H_KV = a->H_KV; p.G = a->H_Q / a->H_KV;
   p.page_shift = shift_of(a->page_size); p.max_pages = a->max_pages; p.max_q_len = a->max_q_len;
   p.sml = a->sm_scale * 1.44269504f;
-  p.num_pages = a->num_pages;
+  p.num_pages = (int)a->num_pages; p.page_bytes = kBlockBytes << (p.page_shift - 4); p.blocks_mask = (1 << (p.page_shift - 4)) - 1;
   p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh; p.pages = (const uint8_t*)a->pages;
   p.table = a->page_table; p.table_stride = a->table_stride; p.kv_lens = a->kv_lens; p.cu_q = a->cu_q;
   p.ws = (float*)a->workspace;
@@ -67,8 +67,9 @@ extern "C" int hq_paged_attention(const hq_paged_attention_args* a, void* stream
   if (int rc = check(a)) return rc;
   if (a->R == 0 || a->T == 0) return HQ_OK;
   const AttnParams p = params_of(a);
-  HQ_REQUIRE(a->workspace && a->workspace_bytes >= workspace_of(p), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
-             (long long)a->workspace_bytes, (long long)workspace_of(p));
+  const int64_t need = workspace_of(p);
+  HQ_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
+             (long long)a->workspace_bytes, (long long)need);
   HQ_REQUIRE(aligned16(a->workspace), HQ_ERR_ALIGNMENT, "hq_paged_attention: the workspace must be 16-byte aligned");
   return few_rows(p) ? decode_launch(p, (cudaStream_t)stream) : tile_launch(p, (cudaStream_t)stream);
 }

@@ -25,6 +25,8 @@ namespace paged {
 constexpr int kUnit = 32, kUnitBytes = 2 * kBlockBytes, kSlots = 3;
 constexpr int kRowPad = 132;                    // floats of a row of a piece
 constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9): at most 2^10 when a reference is set, 2^15 before it moves
+constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
+constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ that lets it stay
 __host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 16 : 12; }
 __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
 
@@ -69,21 +71,19 @@ __device__ __forceinline__ float over_g(float v, bool max) {      // over the ei
 }
 __device__ __forceinline__ float bf16_bits(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 
-// A place in the row of runs.  pos = first + u; u == units is the closing unit.
-struct Walk {
-  int r, h, u, units;
-  Request q;
-};
+// A place in the row of runs; u == units is the closing unit.
+struct Walk { int r, h, u, units; };
 __device__ __forceinline__ int units_of(const Request& x) { return x.nq > 0 ? (x.len + kUnit - 1) / kUnit : -1; }     // -1: no run at all
-__device__ __forceinline__ void next_run(const AttnParams& p, Walk& w) {
+// true where the next run is another request's
+__device__ __forceinline__ bool next_run(const AttnParams& p, Walk& w) {
   w.u = 0;
-  if (++w.h < p.H_KV) return;
+  if (++w.h < p.H_KV) return false;
   w.h = 0;
   do {
-    if (++w.r >= p.R) return;
-    w.q = request_of(p, w.r);
-    w.units = units_of(w.q);
+    if (++w.r >= p.R) break;
+    w.units = units_of(request_of(p, w.r));
   } while (w.units < 0);
+  return true;
 }
 
 // Workspace: pieces of runs that begin before a warp's part and end in it; two pieces per block; what the merge kernel has to
@@ -92,11 +92,11 @@ struct Merge { int q0, nq, h, first, go, unused[3]; };
 template <int NT> __host__ __device__ inline int64_t ws_block_pieces(int blocks) { return (int64_t)blocks * warps_of(NT) * piece_floats(NT); }
 template <int NT> __host__ __device__ inline int64_t ws_merge(int blocks) { return ws_block_pieces<NT>(blocks) + (int64_t)blocks * 2 * piece_floats(NT); }
 
-__device__ __forceinline__ void store_row4(const AttnParams& p, int64_t at, float4 v, float l) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;                // a row that saw no key: 0
+template <bool kBf16>
+__device__ __forceinline__ void store_row4(const AttnParams& p, int64_t at, float4 v, float inv) {
   v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
   uint2 o;
-  if (p.dtype == HQ_BF16) {
+  if (kBf16) {
     __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
     o = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
   } else {
@@ -109,13 +109,21 @@ __device__ __forceinline__ int64_t out_row(const AttnParams& p, const Request& q
   return (int64_t)(q.q0 + n / p.G) * p.o_st + (int64_t)(h * p.G + n % p.G) * p.o_sh;
 }
 
+// a block has at least one position for every warp: fewer blocks take part in short calls
+__device__ __forceinline__ int blocks_of(long long total, int warps) { return (int)max(1ll, min((long long)gridDim.x, quotient(total, warps))); }
 template <int NT>
+__device__ __forceinline__ Merge* todo_of(const AttnParams& p) { return reinterpret_cast<Merge*>(p.ws + ws_merge<NT>(gridDim.x)) + blockIdx.x; }
+
+template <int NT, bool kBf16>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1)
-decode_kernel(const AttnParams p) {
+decode_kernel(const AttnParams p, bool whole) {
   constexpr int kWarps = warps_of(NT), kThreads = kWarps * 32;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_before;                                   // units of the block's first run that lie before it
   __shared__ uint64_t bars[kWarps * kSlots];
   __shared__ int s_live[kWarps * kSlots];                    // which of a unit's two blocks lie in the pool
+  __shared__ int2 s_page[kWarps][32];                        // pages of a unit's blocks, 32 units ahead
+  __shared__ long long s_cut[2];                             // where the block's part begins, all positions
   __shared__ long long s_part[kThreads + 1], s_warp[kWarps];
   __shared__ int s_seg[32], s_q0[32], s_nq[32];              // run (r * H_KV + h) of a warp's first and last piece, or -1; its request
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -124,202 +132,172 @@ decode_kernel(const AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- where this warp's part lies
-  const int per = (p.R + kThreads - 1) / kThreads;
-  long long mine = 0;
-  for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += (long long)p.H_KV * (units_of(request_of(p, r)) + 1);
-  long long x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < kWarps; ++w) { if (w < warp) before += s_warp[w]; total += s_warp[w]; }
-  s_part[tid + 1] = before + x;
-  if (tid == 0) s_part[0] = 0;
-  __syncthreads();
-  // a block has at least one unit for every warp: fewer blocks take part in short calls
-  const int blocks = (int)max(1ll, min((long long)gridDim.x, total / kWarps)), block = blockIdx.x;
-  Merge* todo = reinterpret_cast<Merge*>(p.ws + ws_merge<NT>(gridDim.x)) + block;
-  if (block >= blocks) { if (tid == 0) todo->go = 0; return; }
-  const long long b0 = total * block / blocks, b1 = total * (block + 1) / blocks;
-  const long long w0 = b0 + (b1 - b0) * warp / kWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kWarps;
-  int left = (int)(w1 - w0);
-  // the run at position w0
-  Walk c{0, 0, 0, -1, Request{0, 0, 0, 0}};
-  auto locate = [&](long long pos, Walk& w) {
-    int lo = 0, hi = kThreads;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= pos) lo = mid; else hi = mid; }
-    long long at = s_part[lo];
-    w.r = lo * per;
-    for (;; ++w.r) {
-      w.q = request_of(p, w.r);
-      w.units = units_of(w.q);
-      const long long n = (long long)p.H_KV * (w.units + 1);
-      if (pos < at + n) break;
-      at += n;
+  const int block = blockIdx.x;
+  Walk c{0, 0, 0, -1};
+  int left = 0;
+  auto weight = [&](const Request& q) { return (long long)p.H_KV * (units_of(q) + 1); };
+  if (whole) {                                               // one run a block
+    __syncthreads();
+    c.r = block / p.H_KV; c.h = block - c.r * p.H_KV;
+    c.units = units_of(request_of(p, c.r));
+    if (c.units < 0) return;
+    const int n = c.units + 1;
+    c.u = n * warp / kWarps;
+    left = n * (warp + 1) / kWarps - c.u;
+  } else {
+    const Prefix<kThreads, decltype(weight)> prefix(p, weight, s_part, s_warp);
+    if (p.R <= 64) __syncthreads();
+    const Cuts cuts(prefix.total, blocks_of(prefix.total, kWarps));
+    if (block >= cuts.blocks) { if (tid == 0) todo_of<NT>(p)->go = 0; return; }
+    const long long b0 = cuts.begin(block), n = cuts.begin(block + 1) - b0;
+    if (tid == 0) { s_cut[0] = b0; s_cut[1] = prefix.total; }
+    const long long first = (unsigned long long)n >> 26 ? n * warp / kWarps : (int)n * warp / kWarps;
+    const long long last = (unsigned long long)n >> 26 ? n * (warp + 1) / kWarps : (int)n * (warp + 1) / kWarps;
+    left = (int)(last - first);
+    if (left > 0) {
+      long long in;
+      c.r = prefix.seek(b0 + first, in);
+      c.units = units_of(request_of(p, c.r));
+      c.h = (int)quotient(in, c.units + 1);
+      c.u = (int)(in - (long long)c.h * (c.units + 1));
     }
-    const int in = (int)((pos - at) / (w.units + 1));
-    w.h = in;
-    w.u = (int)(pos - at - (long long)in * (w.units + 1));
-  };
-  if (left > 0) locate(w0, c);
+  }
   const int start_u = c.u;                                   // the part begins inside a run if start_u > 0
+
+  if (warp == 0 && lane == 0) s_before = start_u;
 
   // ---- the ring
   uint8_t* ring = smem + warp * (kSlots * kUnitBytes);
   uint64_t* bar = bars + warp * kSlots;
-  int* live = s_live + warp * kSlots;
-  const int num_pages = (int)p.num_pages, page_bytes = kBlockBytes << (p.page_shift - 4), blocks_mask = (1 << (p.page_shift - 4)) - 1;
+  int slot = 0, ahead = 0;                                   // the slot that is read next; units under way
+  uint32_t parity = 0;
   Walk f = c;                                                // the unit that is fetched next
-  int f_left = left, f_slot = 0;
-  int tab_r = -1, tab_u = 0, pg0 = -1, pg1 = -1;             // pages of 32 units of request tab_r, a unit per lane
-  auto fetch = [&]() {                                       // the next unit that is there; all lanes
-    while (f_left > 0 && f.u >= f.units) { --f_left; next_run(p, f); }
+  int f_left = left, tab_r = -1, tab_u = 0;                  // pages of the units tab_u .. + 31 of request tab_r are at hand
+  auto fetch = [&]() {                                       // asks for the next unit, if there is one; all lanes
+    while (f_left > 0 && f.u >= f.units) { if (--f_left > 0) next_run(p, f); }
     if (f_left <= 0) return;
     if (f.r != tab_r || f.u - tab_u >= 32 || f.u < tab_u) {
       tab_r = f.r; tab_u = f.u;
       const int64_t tok = ((int64_t)tab_u + lane) * kUnit;
       const int* row = p.table + (int64_t)f.r * p.table_stride;
-      pg0 = tok < f.q.len ? __ldg(row + (tok >> p.page_shift)) : -1;
-      pg1 = tok + kTok < f.q.len ? __ldg(row + ((tok + kTok) >> p.page_shift)) : -1;
+      const int len = request_of(p, f.r).len;
+      __syncwarp();
+      s_page[warp][lane] = make_int2(tok < len ? __ldg(row + (tok >> p.page_shift)) : -1, tok + kTok < len ? __ldg(row + ((tok + kTok) >> p.page_shift)) : -1);
+      __syncwarp();
     }
-    const int a = __shfl_sync(0xffffffffu, pg0, f.u - tab_u), b = __shfl_sync(0xffffffffu, pg1, f.u - tab_u);
     if (lane == 0) {
-      const bool la = (uint32_t)a < (uint32_t)num_pages, lb = (uint32_t)b < (uint32_t)num_pages;
-      live[f_slot] = (la ? 1 : 0) | (lb ? 2 : 0);
-      uint8_t* dst = ring + f_slot * kUnitBytes;
-      const uint8_t* src = p.pages + (int64_t)(a * p.H_KV + f.h) * page_bytes + ((f.u << 1) & blocks_mask) * kBlockBytes;
-      mbar_expect_tx(bar + f_slot, ((la ? 1 : 0) + (lb ? 1 : 0)) * kBlockBytes);
-      if (la && lb && p.page_shift > 4) bulk_g2s(dst, src, kUnitBytes, bar + f_slot);
+      const int at = slot + ahead >= kSlots ? slot + ahead - kSlots : slot + ahead;
+      const int2 pg = s_page[warp][f.u - tab_u];
+      const bool la = (uint32_t)pg.x < (uint32_t)p.num_pages, lb = (uint32_t)pg.y < (uint32_t)p.num_pages;
+      s_live[warp * kSlots + at] = (la ? 1 : 0) | (lb ? 2 : 0);
+      uint8_t* dst = ring + at * kUnitBytes;
+      const uint8_t* src = p.pages + (int64_t)(pg.x * p.H_KV + f.h) * p.page_bytes + ((f.u << 1) & p.blocks_mask) * kBlockBytes;
+      mbar_expect_tx(bar + at, ((la ? 1 : 0) + (lb ? 1 : 0)) * kBlockBytes);
+      if (la && lb && p.page_shift > 4) bulk_g2s(dst, src, kUnitBytes, bar + at);
       else {
-        if (la) bulk_g2s(dst, src, kBlockBytes, bar + f_slot);
-        if (lb) bulk_g2s(dst + kBlockBytes, p.page_shift > 4 ? src + kBlockBytes : p.pages + (int64_t)(b * p.H_KV + f.h) * page_bytes, kBlockBytes,
-                         bar + f_slot);
+        if (la) bulk_g2s(dst, src, kBlockBytes, bar + at);
+        if (lb) bulk_g2s(dst + kBlockBytes, p.page_shift > 4 ? src + kBlockBytes : p.pages + (int64_t)(pg.y * p.H_KV + f.h) * p.page_bytes, kBlockBytes,
+                         bar + at);
       }
     }
-    if (++f_slot == kSlots) f_slot = 0;
     ++f.u; --f_left;
   };
-#pragma unroll 1
-  for (int i = 0; i < kSlots; ++i) fetch();
 
   // ---- the state of the run in hand
   uint32_t qf[NT][16];                                       // query operand: word w, nibble k at 4 w + k
+  uint4 raw[NT][4];                                          // its row as it lies: channels 32 t4 .. + 31
   float2 fac[NT], start[NT];                                 // factor of a score, start of the accumulators: columns 2 t4, 2 t4 + 1
-  float2 m[NT], l[NT], shift[NT];                            // shift = kShift - m
-  float vback = 1.f;                                         // 2^-vexp
+  float2 l[NT], shift[NT];                                   // P = 2^(score + shift); kNone: no key so far
   const Masks km = masks();
   float O[NT][8][4], Ls[NT][4];
-  int vexp = 0;                                              // V scales are taken relative to 2^vexp
+  float vback = 1.f;                                         // V scales are taken times this power of two
   int lim0 = 0;                                              // keys that the run's first token sees
-  int lim[NT][2];
-  auto open = [&]() {
-    const int rows = c.q.nq * p.G;
+  auto ask_q = [&]() {
+    const Request q = request_of(p, c.r);
+    const int rows = q.nq * p.G;
+    lim0 = q.past + 1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int n = 8 * nt + g;
-      uint4 raw[4];
-      const bool there = n < rows;
-      const int64_t at = (int64_t)(c.q.q0 + n / p.G) * p.q_st + (int64_t)(c.h * p.G + n % p.G) * p.q_sh + 32 * t4;
+      const int n = 8 * nt + g, i = n / p.G;
+      const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st +
+                                                       (int64_t)(c.h * p.G + n - i * p.G) * p.q_sh + 32 * t4);
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        raw[w] = there ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at) + w) : make_uint4(0u, 0u, 0u, 0u);
-      float top = 0.f;
-      auto value = [&](int w, int i) {                       // channel 32 t4 + 8 w + i
-        const uint32_t u = i < 2 ? raw[w].x : i < 4 ? raw[w].y : i < 6 ? raw[w].z : raw[w].w;
-        if (p.dtype == HQ_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
-        return __half2float(__ushort_as_half((unsigned short)(i & 1 ? u >> 16 : u & 0xFFFFu)));
-      };
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(value(w, i)));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the largest magnitude to [2^13, 2^14): below it fp16 has 37 bits
-      const int ex = (int)(__float_as_uint(top) >> 23);      // 0: zero or below the normal numbers, 255: infinite
-      const int up = ex == 255 ? 0 : 140 - max(ex, 14);      // at most 2^126, a normal number
-      const float scale = __uint_as_float((uint32_t)(127 + up) << 23);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float s = k & 1 ? scale * 0.0625f : scale;
-          const __half2 hh = __floats2half2_rn(value(w, k) * s, value(w, k + 4) * s);
-          qf[nt][4 * w + k] = *reinterpret_cast<const uint32_t*>(&hh);
-          const float2 back = __half22float2(hh);
-          sum += (back.x + back.y) * (k & 1 ? 16.f : 1.f);
-        }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float back = p.sml * __uint_as_float((uint32_t)min(127 + 24 - up, 255) << 23);       // sml 2^24 / scale
-      const float first = -8.f * 0x1p-24f * sum;
-      fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
-      start[nt] = make_float2(__shfl_sync(0xffffffffu, first, 8 * t4), __shfl_sync(0xffffffffu, first, 8 * t4 + 4));
-      m[nt] = make_float2(-INFINITY, -INFINITY);
-      shift[nt] = make_float2(INFINITY, INFINITY);
-      l[nt] = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) lim[nt][j] = c.q.past + 1 + min((8 * nt + 2 * t4 + j) / p.G, c.q.nq - 1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Ls[nt][i] = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) O[nt][mt][i] = 0.f;
+      for (int w = 0; w < 4; ++w) raw[nt][w] = n < rows ? __ldg(at + w) : make_uint4(0u, 0u, 0u, 0u);
     }
-    lim0 = c.q.past + 1;
-    vexp = -1000;
-    vback = 1.f;
   };
-  // what the row is at the end: the 8 of the codes taken off, the powers of two put back
-  auto close = [&](auto&& row) {
-    const float back = vexp == -1000 ? 0.f : ldexpf(1.f, vexp);
+  auto open = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t top2 = 0u;                                    // magnitudes of 16-bit numbers order like integers
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint4 u = raw[nt][w];
+        top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, u.x & 0x7FFF7FFFu), u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+      }
+      top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+      top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+      auto value = [&](uint32_t u, int hi) {
+        if (kBf16) return __uint_as_float(hi ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half((unsigned short)(hi ? u >> 16 : u & 0xFFFFu)));
+      };
+      // the largest magnitude to [2^13, 2^14): below it fp16 has 37 bits
+      const int ex = (int)(__float_as_uint(value(max(top2 & 0xFFFFu, top2 >> 16), 0)) >> 23);      // 0: zero or below the normal numbers, 255: infinite
+      const int up = ex == 255 ? 0 : 140 - max(ex, 14);      // at most 2^126, a normal number
+      const float scale = __uint_as_float((uint32_t)(127 + up) << 23), scale16 = scale * 0.0625f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t u[4] = {raw[nt][w].x, raw[nt][w].y, raw[nt][w].z, raw[nt][w].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                        // channels k and k + 4 of the eight
+          const float2 x = fmul2(make_float2(value(u[k >> 1], k & 1), value(u[2 + (k >> 1)], k & 1)),
+                                 k & 1 ? make_float2(scale16, scale16) : make_float2(scale, scale));
+          const __half2 hh = __floats2half2_rn(x.x, x.y);
+          qf[nt][4 * w + k] = *reinterpret_cast<const uint32_t*>(&hh);
+        }
+      }
+      // what codes of zero give: the 8 that is in every nibble, to be taken off
+      float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 8; ++w) mma16816(zero, km.lo8, km.lo8, km.hi8, km.hi8, qf[nt][2 * w], qf[nt][2 * w + 1]);
+      start[nt] = make_float2(-zero[0], -zero[1]);
+      shift[nt] = make_float2(kShift - kFirst, kShift - kFirst);
+      const float back = p.sml * __uint_as_float((uint32_t)min(127 + 24 - up, 255) << 23);       // sml 2^24 / scale
+      fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
+    }
+  };
+  // The run's rows so far: the 8 of the codes taken off, the powers of two put back.  To the output (piece == nullptr) or as a piece.
+  auto finish = [&](float* piece) {
+    const Request q = request_of(p, c.r);
+    const int rows = q.nq * p.G;
+    const float back = 1.f / vback;                          // a power of two, exact
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float ls[2] = {over_g(l[nt].x, false), over_g(l[nt].y, false)};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float4 v[4];
-        const float eight = 8.f * Ls[nt][j];
+        const int n = 8 * nt + 2 * t4 + j;
+        const float f = piece ? back : ls[j] == 0.f ? 0.f : back / ls[j], eight = -8.f * Ls[nt][j] * f, f24 = f * 0x1p24f, f20 = f * 0x1p20f;
+        if (n < rows) {
+          const int64_t at = out_row(p, q, c.h, n) + 16 * g;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          v[q4].x = (O[nt][2 * q4][j] * 0x1p24f - eight) * back;
-          v[q4].y = (O[nt][2 * q4 + 1][j] * 0x1p20f - eight) * back;
-          v[q4].z = (O[nt][2 * q4][2 + j] * 0x1p24f - eight) * back;
-          v[q4].w = (O[nt][2 * q4 + 1][2 + j] * 0x1p20f - eight) * back;
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const float4 v = make_float4(fmaf(O[nt][2 * q4][j], f24, eight), fmaf(O[nt][2 * q4 + 1][j], f20, eight),
+                                         fmaf(O[nt][2 * q4][2 + j], f24, eight), fmaf(O[nt][2 * q4 + 1][2 + j], f20, eight));
+            if (piece) *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = v;
+            else store_row4<kBf16>(p, at + 4 * q4, v, 1.f);
+          }
+          if (piece && g == 0) { piece[8 * NT * kRowPad + n] = -(j ? shift[nt].y : shift[nt].x); piece[8 * NT * kRowPad + 8 * NT + n] = ls[j]; }
         }
-        row(8 * nt + 2 * t4 + j, v, j ? m[nt].y : m[nt].x, ls[j]);
       }
     }
   };
-  auto to_piece = [&](float* piece) {
-    close([&](int n, const float4 (&v)[4], float mm, float ll) {
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = v[q4];
-      if (g == 0) { piece[8 * NT * kRowPad + n] = mm; piece[8 * NT * kRowPad + 8 * NT + n] = ll; }
-    });
-  };
-  auto to_out = [&]() {
-    const int rows = c.q.nq * p.G;
-    close([&](int n, const float4 (&v)[4], float, float ll) {
-      if (n < rows) {
-        const int64_t at = out_row(p, c.q, c.h, n) + 16 * g;
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) store_row4(p, at + 4 * q4, v[q4], ll);
-      }
-    });
-  };
 
-  int slot = 0;
-  uint32_t parity = 0;
   const int tau = (g >> 1) + 4 * (g & 1);                    // token of score row g (and + 8): the four tokens of a V fragment's
                                                              // load are neighbours then, on both halves of the banks
-  auto unit = [&]() {
+  auto unit = [&](bool fresh) {                              // fresh: the run's first one here
     const bool ok = mbar_wait_bounded(bar + slot, parity);
     const uint8_t* u0 = ring + slot * kUnitBytes;
-    const int there = live[slot];
+    const int there = s_live[warp * kSlots + slot];
     float S[NT][2][4];
     float ks[2][2], vs[2][2];
 #pragma unroll
@@ -358,30 +336,35 @@ decode_kernel(const AttnParams p) {
         }
     const int tok0 = c.u * kUnit;
     if (__builtin_expect(tok0 + kUnit > lim0 || there != 3, 0)) {        // keys behind a row's last one, pages that are not there
+      const Request q = request_of(p, c.r);
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int tok = tok0 + 16 * cb + tau + 8 * i;
           const bool here = (there >> cb) & 1;
-          if (!here || tok >= c.q.len) vs[cb][i] = 0.f;                  // what lies there may be anything, NaN too
+          if (!here || tok >= q.len) vs[cb][i] = 0.f;                    // what lies there may be anything, NaN too
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              if (!here || tok >= lim[nt][j]) S[nt][cb][2 * i + j] = -INFINITY;
+              if (!here || tok >= lim0 + min((8 * nt + 2 * t4 + j) / p.G, q.nq - 1)) S[nt][cb][2 * i + j] = -INFINITY;
         }
     }
     // P against the references as they stand: a row's reference maximum, the power of two of the V scales.  Nothing is compared
-    // beforehand: a term that fp16 could not hold shows in the sum of the terms (so does a row's first unit, whose shift is infinite);
-    // only then the maxima are taken, the references move and the unit's P is formed again.
+    // beforehand: a term that fp16 could not hold shows in the sum of the terms.  Only then the maxima are taken, the references
+    // move and the unit's P is formed again.  A run's first unit is tried with a reference of 2^kFirst and scales as they are, which fits
+    // if every row's sum comes out large enough for fp16's lower end, too.
     uint32_t P[NT][2][2];
     float2 le[NT];
-    auto form = [&]() {
-      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int pass = 0;; ++pass) {
+      float most = 0.f;
+      bool fits = true;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         le[nt] = make_float2(0.f, 0.f);
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -395,36 +378,34 @@ decode_kernel(const AttnParams p) {
             const __half2 hh = __floats2half2_rn(pv.x, pv.y);
             P[nt][cb][i] = *reinterpret_cast<const uint32_t*>(&hh);
           }
+        most += sum.x + sum.y;
+        if (fresh && pass == 0) {
+          const int n = 8 * nt + 2 * t4, rows = request_of(p, c.r).nq * p.G;
+          const float x0 = over_g(sum.x, false), x1 = over_g(sum.y, false);
+          fits = fits && (x0 >= kLeast || n >= rows) && (x1 >= kLeast || n + 1 >= rows);
+        }
       }
-      return sum.x + sum.y;
-    };
-    const float sum = form();
-    if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 32768.f)), 0)) {
+      if (pass) break;
+      if (!__any_sync(0xffffffffu, !(most <= 32768.f) || !fits)) break;
       const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
-      const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 127;
-      const int nv = max(vexp, e);
-      const float vscale = vexp == -1000 ? 0.f : ldexpf(1.f, max(vexp - nv, -200));
-      vexp = nv;
-      vback = __uint_as_float((uint32_t)(127 - max(vexp, -126)) << 23);                 // 2^-vexp
+      // 2^-e for the largest scale's power of two e, kept in the range of normal numbers; smaller than before unless nothing was before
+      const int e = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23), 1), 253);
+      const float nb = __uint_as_float((uint32_t)(254 - e) << 23), vnew = fresh ? nb : fminf(vback, nb), vscale = fresh ? 0.f : vnew / vback;
+      vback = vnew;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float x0 = over_g(fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2])), true);
         const float x1 = over_g(fmaxf(fmaxf(S[nt][0][1], S[nt][0][3]), fmaxf(S[nt][1][1], S[nt][1][3])), true);
-        const float2 nm = make_float2(fmaxf(m[nt].x, x0), fmaxf(m[nt].y, x1));
-        const float2 al = make_float2(m[nt].x == -INFINITY ? 0.f : ex2f(m[nt].x - nm.x), m[nt].y == -INFINITY ? 0.f : ex2f(m[nt].y - nm.y));
-        m[nt] = nm;
+        // the reference rises to the maximum, or falls to it if there was none; P so far is of 2^(new - old)
+        const float2 old = fresh ? make_float2(kNone, kNone) : shift[nt];
+        const float2 ns = make_float2(fminf(old.x, kShift - x0), fminf(old.y, kShift - x1));
+        const float2 al = make_float2(old.x == kNone ? 0.f : ex2f(ns.x - old.x), old.y == kNone ? 0.f : ex2f(ns.y - old.y));
         l[nt] = fmul2(l[nt], al);
         const float2 av = make_float2(al.x * vscale, al.y * vscale);
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) { O[nt][mt][0] *= av.x; O[nt][mt][1] *= av.y; O[nt][mt][2] *= av.x; O[nt][mt][3] *= av.y; }
         Ls[nt][0] *= av.x; Ls[nt][1] *= av.y; Ls[nt][2] *= av.x; Ls[nt][3] *= av.y;
-        shift[nt] = make_float2(nm.x == -INFINITY ? 0.f : kShift - nm.x, nm.y == -INFINITY ? 0.f : kShift - nm.y);
-      }
-      form();
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {                      // a row without a key so far: its next unit comes here again
-        if (m[nt].x == -INFINITY) shift[nt].x = INFINITY;
-        if (m[nt].y == -INFINITY) shift[nt].y = INFINITY;
+        shift[nt] = ns;
       }
     }
 #pragma unroll
@@ -461,84 +442,93 @@ decode_kernel(const AttnParams p) {
     if (++slot == kSlots) { slot = 0; parity ^= 1u; }
   };
 
-  float* first_piece = p.ws + (int64_t)(block * kWarps + warp) * piece_floats(NT);
   if (tid < 32) s_seg[tid] = -1;
   __syncthreads();
-  auto mark = [&](int i) {
-    if (lane == 0) { s_seg[2 * warp + i] = c.r * p.H_KV + c.h; s_q0[2 * warp + i] = c.q.q0; s_nq[2 * warp + i] = c.q.nq; }
-  };
   bool inside = start_u > 0;                                 // the run in hand began before this part
-  if (left > 0) {
-    open();
+  if (left > 0) ask_q();
 #pragma unroll 1
-    while (true) {
-      if (c.u < c.units) {
-        unit();
-        fetch();
-        ++c.u; --left;
-      } else {                                               // the run ends here
-        if (inside) { to_piece(first_piece); mark(0); }
-        else to_out();
-        inside = false;
-        --left;
-        if (left > 0) { next_run(p, c); open(); }
-        else { c.u = -1; }
-      }
-      if (left == 0) break;
+  while (left > 0) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      shift[nt] = make_float2(kNone, kNone);
+      l[nt] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ls[nt][i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[nt][mt][i] = 0.f;
     }
-    if (c.u != -1) {                                         // and goes on in the next part: its piece into the ring, which is empty
-      to_piece(reinterpret_cast<float*>(ring));
-      mark(1);
+    vback = 1.f;
+    const int n = min(c.units - c.u, left);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+#pragma unroll 1
+      for (; ahead < kSlots; ++ahead) fetch();               // three at first, then the slot that has just been read
+      if (i == 0) open();
+      unit(i == 0);
+      --ahead;
+      ++c.u;
     }
+    left -= n;
+    const bool ends = left > 0;                              // else it goes on in the next part
+    float* mine = reinterpret_cast<float*>(ring);            // empty when it is the part's last
+    float* piece = !ends ? mine : !inside ? nullptr : whole ? mine : p.ws + (int64_t)(block * kWarps + warp) * piece_floats(NT);
+    finish(piece);
+    if (piece && lane == 0) {
+      const int at = 2 * warp + (ends ? 0 : 1);
+      const Request q = request_of(p, c.r);
+      s_seg[at] = c.r * p.H_KV + c.h; s_q0[at] = q.q0; s_nq[at] = q.nq;
+    }
+    if (ends && --left > 0) { inside = false; next_run(p, c); ask_q(); }
   }
-  if (tid == 0) todo->go = 0;
-  __syncthreads();
+  if (!whole && tid == 0) todo_of<NT>(p)->go = 0;
 
   // ---- runs that several warps share: pieces in order are the warps' first and last ones, a lane each; neighbours of the same
   // run are a group.  A warp takes a row of a group at a time.
+  __syncthreads();
   const int seg = s_seg[lane];
   const uint32_t valid = __ballot_sync(0xffffffffu, seg >= 0);
   if (valid == 0) return;
   const uint32_t below = valid & ((1u << lane) - 1u);
   const int prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : 0);
   const uint32_t heads = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0u || prev != seg));
-  const bool from_before = __shfl_sync(0xffffffffu, start_u, 0) > 0;      // of warp 0 only
-  __shared__ int s_before;
-  __shared__ long long s_start;
-  if (tid == 0) { s_before = from_before; s_start = b0 - start_u; }
-  __syncthreads();
+  const float* my_piece = (lane & 1) || whole ? reinterpret_cast<const float*>(smem + (lane >> 1) * (kSlots * kUnitBytes))
+                                              : p.ws + (int64_t)(block * kWarps + (lane >> 1)) * piece_floats(NT);
   int item = 0;
+#pragma unroll 1
   for (uint32_t rest = heads; rest; rest &= rest - 1) {
     const int head = __ffs(rest) - 1;
     const uint32_t later = rest & (rest - 1);
     const uint32_t group = valid & ~((1u << head) - 1u) & (later ? (later & (0u - later)) - 1u : 0xffffffffu);
-    const int id = s_seg[head], q0 = s_q0[head], nq = s_nq[head], rows = nq * p.G, r = id / p.H_KV, h = id - r * p.H_KV;
-    const bool began_before = head == __ffs(valid) - 1 && s_before, ends = ((31 - __clz(group)) & 1) == 0;
-    float* to = p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block + (began_before ? 0 : 1)) * piece_floats(NT);
-    if (began_before && ends && tid == 0) {
-      int first = (int)(s_start * blocks / total);
-      while (total * first / blocks > s_start) --first;
-      while (total * (first + 1) / blocks <= s_start) ++first;
-      *todo = Merge{q0, nq, h, first, 1, {0, 0, 0}};
-    }
+    const int id = s_seg[head], q0 = s_q0[head], nq = s_nq[head], rows = nq * p.G, h = id % p.H_KV;
+    const bool began_before = !whole && head == __ffs(valid) - 1 && s_before > 0, ends = ((31 - __clz(group)) & 1) == 0;
+    if (began_before && ends && tid == 0) *todo_of<NT>(p) = Merge{q0, nq, h, Cuts(s_cut[1], blocks_of(s_cut[1], kWarps)).block_of(s_cut[0] - s_before), 1, {0, 0, 0}};
+#pragma unroll 1
     for (int n = 0; n < rows; ++n, ++item) {
       if (item % kWarps != warp) continue;
-      auto piece = [&](int i) -> const float* {
-        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes)) : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
-      };
-      float M = -INFINITY, L = 0.f;
+      const bool in = (group >> lane) & 1u;
+      const float mi = in ? my_piece[8 * NT * kRowPad + n] : -INFINITY;
+      float M = mi;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float w = ex2f(mi - (M == -INFINITY ? 0.f : M));
+      float L = in ? w * my_piece[8 * NT * kRowPad + 8 * NT + n] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t x = group; x; x &= x - 1) M = fmaxf(M, piece(__ffs(x) - 1)[8 * NT * kRowPad + n]);
-      const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll 1
       for (uint32_t x = group; x; x &= x - 1) {
-        const float* from = piece(__ffs(x) - 1);
-        const float w = ex2f(from[8 * NT * kRowPad + n] - ref);
+        const int i = __ffs(x) - 1;
+        const float* from = (i & 1) || whole ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes))
+                                             : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
         const float4 v = *reinterpret_cast<const float4*>(from + n * kRowPad + 4 * lane);
-        L += w * from[8 * NT * kRowPad + 8 * NT + n];
-        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        acc.x += wi * v.x; acc.y += wi * v.y; acc.z += wi * v.z; acc.w += wi * v.w;
       }
-      if (!began_before && ends) store_row4(p, out_row(p, Request{q0, nq, 0, 0}, h, n) + 4 * lane, acc, L);
+      if (!began_before && ends) store_row4<kBf16>(p, out_row(p, Request{q0, nq, 0, 0}, h, n) + 4 * lane, acc, L == 0.f ? 0.f : 1.f / L);
       else {
+        float* to = p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block + (began_before ? 0 : 1)) * piece_floats(NT);
         *reinterpret_cast<float4*>(to + n * kRowPad + 4 * lane) = acc;
         if (lane == 0) { to[8 * NT * kRowPad + n] = M; to[8 * NT * kRowPad + 8 * NT + n] = L; }
       }
@@ -585,24 +575,35 @@ merge_kernel(const AttnParams p, int grid) {
     L += w * s_l[i];
     acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
   }
-  store_row4(p, out_row(p, Request{todo.q0, todo.nq, 0, 0}, todo.h, n) + 4 * lane, acc, L);
+  const int64_t at = out_row(p, Request{todo.q0, todo.nq, 0, 0}, todo.h, n) + 4 * lane;
+  const float inv = L == 0.f ? 0.f : 1.f / L;                // a row that saw no key: 0
+  if (p.dtype == HQ_BF16) store_row4<true>(p, at, acc, inv);
+  else store_row4<false>(p, at, acc, inv);
 }
 
 static int tiles_of(const AttnParams& p) { return p.max_q_len * p.G <= 8 ? 1 : 2; }
 
-int64_t decode_workspace(const AttnParams& p) {
-  const int grid = sm_count();
-  return tiles_of(p) == 1 ? ws_merge<1>(grid) * 4 + grid * (int64_t)sizeof(Merge) : ws_merge<2>(grid) * 4 + grid * (int64_t)sizeof(Merge);
+// Short tables and no more runs than SMs: a block per run, nothing to merge across blocks, one launch and no workspace.  Longer
+// ones gain more from every SM's share of the bandwidth: KEEP
+static bool block_per_run(const AttnParams& p) {
+  return ((int64_t)p.max_pages << p.page_shift) <= 1024 && (int64_t)p.R * p.H_KV <= sm_count();
 }
 
-template <int NT>
+int64_t decode_workspace(const AttnParams& p) {
+  if (block_per_run(p)) return 0;
+  const int grid = sm_count();
+  return (tiles_of(p) == 1 ? ws_merge<1>(grid) : ws_merge<2>(grid)) * 4 + grid * (int64_t)sizeof(Merge);
+}
+
+template <int NT, bool kBf16>
 static int launch(const AttnParams& p, cudaStream_t st) {
-  const int grid = sm_count(), smem = warps_of(NT) * kSlots * kUnitBytes;
+  const bool whole = block_per_run(p);
+  const int grid = whole ? p.R * p.H_KV : sm_count(), smem = warps_of(NT) * kSlots * kUnitBytes;
   static thread_local int attr_dev = -1;
   int dev = 0;
   HQ_CUDA(cudaGetDevice(&dev));
   if (attr_dev != dev) {
-    HQ_CUDA(cudaFuncSetAttribute(decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    HQ_CUDA(cudaFuncSetAttribute(decode_kernel<NT, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_dev = dev;
   }
   cudaLaunchAttribute after{};
@@ -611,13 +612,17 @@ static int launch(const AttnParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid); cfg.blockDim = dim3(warps_of(NT) * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cfg.attrs = &after; cfg.numAttrs = 1;
-  HQ_CUDA(cudaLaunchKernelEx(&cfg, decode_kernel<NT>, p));
+  HQ_CUDA(cudaLaunchKernelEx(&cfg, decode_kernel<NT, kBf16>, p, whole));
+  if (whole) return HQ_OK;
   cfg.gridDim = dim3(grid, p.max_q_len * p.G); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 0;
   HQ_CUDA(cudaLaunchKernelEx(&cfg, merge_kernel<NT>, p, grid));
   return HQ_OK;
 }
 
-int decode_launch(const AttnParams& p, cudaStream_t st) { return tiles_of(p) == 1 ? launch<1>(p, st) : launch<2>(p, st); }
+int decode_launch(const AttnParams& p, cudaStream_t st) {
+  if (tiles_of(p) == 1) return p.dtype == HQ_BF16 ? launch<1, true>(p, st) : launch<1, false>(p, st);
+  return p.dtype == HQ_BF16 ? launch<2, true>(p, st) : launch<2, false>(p, st);
+}
 
 }  // namespace paged
 }  // namespace hq

@@ -96,9 +96,6 @@ struct Pieces {
   }
   __device__ __forceinline__ bool split() const { return it.cost == 1; }      // every other key tile to each half
 };
-// a / b for a >= 0, b > 0: 64-bit division only where it is needed
-__device__ __forceinline__ long long quotient(long long a, int b) { return (unsigned long long)a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b); }
-
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, tc::mbar_wait_abortable(bar, parity, abort_flag, 0, kTPolls));
@@ -236,49 +233,27 @@ tile_kernel(const AttnParams p, int piece_rows) {
     x.q = q;
     int w = 0;
     for (x.qt = 0, x.n_qt = query_tiles(p, q); x.qt < x.n_qt; ++x.qt) { size_item(p, x); w += x.positions(); }
-    return w;
+    return (long long)w * p.H_KV;
   };
-  const int per = (p.R + kTileThreads - 1) / kTileThreads;
-  long long mine = 0;
-  for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += (long long)p.H_KV * weight(request_of(p, r));
-  long long x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  long long sums = lane < kTileThreads / 32 ? s_warp[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, sums, o); if (lane >= o) sums += y; }
-  const long long total = __shfl_sync(0xffffffffu, sums, 31), before = warp ? __shfl_sync(0xffffffffu, sums, (warp + 31) & 31) : 0;
-  s_part[tid + 1] = before + x;
-  if (tid == 0) s_part[0] = 0;
+  const Prefix<kTileThreads, decltype(weight)> prefix(p, weight, s_part, s_warp);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  // block b's part: total / blocks positions, one more for the first total % blocks
-  const int blocks = (int)max(1ll, min((long long)gridDim.x, quotient(total, kItemCost + 2))), block = blockIdx.x;
-  const long long share = quotient(total, blocks);
-  const int more = (int)(total - share * blocks);
-  const long long b0 = share * block + min(block, more);
+  const Cuts cuts(prefix.total, (int)max(1ll, min((long long)gridDim.x, quotient(prefix.total, kItemCost + 2))));
+  const int block = blockIdx.x;
+  const long long b0 = cuts.begin(block);
   const int64_t piece_floats = (int64_t)piece_rows * 130;
   TileMerge* todo = reinterpret_cast<TileMerge*>(p.ws + 2 * piece_floats * gridDim.x) + block;
   if (tid == 0) todo->go = 0;
   Pieces pc;
-  pc.left = block < blocks ? share + (block < more ? 1 : 0) : 0;
+  pc.left = block < cuts.blocks ? cuts.begin(block + 1) - b0 : 0;
   if (pc.left > 0) {
-    int lo = 0, hi = kTileThreads;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= b0) lo = mid; else hi = mid; }
-    long long in = b0 - s_part[lo];
     Item it;
-    it.r = lo * per;
-    int w;
-    for (;; ++it.r) {
-      it.q = request_of(p, it.r);
-      w = weight(it.q);
-      if (in < (long long)w * p.H_KV) break;
-      in -= (long long)w * p.H_KV;
-    }
+    long long in;
+    it.r = prefix.seek(b0, in);
+    it.q = request_of(p, it.r);
+    const int w = (int)quotient(weight(it.q), p.H_KV);
     it.h = (int)quotient(in, w);
     in -= (long long)it.h * w;
     it.n_qt = query_tiles(p, it.q);
@@ -294,7 +269,6 @@ tile_kernel(const AttnParams p, int piece_rows) {
   uint8_t* bads = smem + TileSmem::Bad;                                    // [16] blocks of a tile whose page is not there
   if (warp == kFetch) {
     // ------------------------------------------------------------ codes
-    const int num_pages = (int)p.num_pages, page_bytes = kBlockBytes << (p.page_shift - 4), blocks_mask = (1 << (p.page_shift - 4)) - 1;
     int tab_r = -1, tab_t = 0, pg = -1;          // pages of eight tiles of request tab_r: lane 4 i + b, block b of tile tab_t + i
     int stage = 0;
     uint32_t par = 1u, tile = 0;                 // empty barriers: the first round passes
@@ -308,7 +282,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
           pg = tok < pc.it.q.len ? __ldg(p.table + (int64_t)tab_r * p.table_stride + (tok >> p.page_shift)) : -1;
         }
         const int page = __shfl_sync(0xffffffffu, pg, 4 * (t - tab_t) + (lane & 3)), tok = t * kKeys + kTok * (lane & 3);
-        const bool in = tok < pc.it.q.len && lane < 4, there = in && (uint32_t)page < (uint32_t)num_pages;
+        const bool in = tok < pc.it.q.len && lane < 4, there = in && (uint32_t)page < (uint32_t)p.num_pages;
         const uint32_t have = __ballot_sync(0xffffffffu, there), gone = __ballot_sync(0xffffffffu, in && !there);
         ok = wait_warp(c_empty + stage, par, abort_flag);
         if (!ok) break;
@@ -320,7 +294,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
         __syncwarp();
         if (there)
           bulk_g2s(smem + TileSmem::Codes + stage * kCodeBytes + lane * kBlockBytes,
-                   p.pages + (int64_t)(page * p.H_KV + pc.it.h) * page_bytes + ((tok >> 4) & blocks_mask) * kBlockBytes, kBlockBytes, c_full + stage);
+                   p.pages + (int64_t)(page * p.H_KV + pc.it.h) * p.page_bytes + ((tok >> 4) & p.blocks_mask) * kBlockBytes, kBlockBytes, c_full + stage);
         if (++stage == kAhead) { stage = 0; par ^= 1u; }
       }
       pc.done(p);
@@ -653,8 +627,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
       if (split) { tc::fence_before_sync(); halves_meet(); }           // the other half has read this one's O and state
       if (pc.began && pc.ends && tid == 0) {
         const long long start = b0 - pc.it.u;    // where the query tile begins: the block of that position has its first piece
-        int first_block = (int)(start < (share + 1) * more ? quotient(start, (int)(share + 1)) : more + quotient(start - (share + 1) * more, (int)share));
-        *todo = TileMerge{q.q0, min(kRows, q.nq * p.G - pc.it.qt * kRows), pc.it.h, pc.it.qt, first_block, 1, {0, 0}};
+        *todo = TileMerge{q.q0, min(kRows, q.nq * p.G - pc.it.qt * kRows), pc.it.h, pc.it.qt, cuts.block_of(start), 1, {0, 0}};
       }
       pc.done(p);
     }

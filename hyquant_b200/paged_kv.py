@@ -17,6 +17,7 @@ can be captured in a CUDA graph.  :class:`PagedKVCache` keeps the state of a who
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -63,9 +64,10 @@ def paged_pages(num_pages: int, num_kv_heads: int, page_size: int = 64, device="
 
 def _pool(pages: torch.Tensor) -> Tuple[int, int, int]:
     """(num_pages, H_KV, page_size) of a pool."""
-    _lib.require_cuda(pages, "pages")
+    if not pages.is_cuda:
+        _lib.require_cuda(pages, "pages")
     shape = pages.shape
-    if pages.dtype != torch.uint8 or len(shape) != 4 or shape[3] != BLOCK_BYTES or not pages.is_contiguous():
+    if pages.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != BLOCK_BYTES or not pages.is_contiguous():
         raise HyQuantError(f"pages must be contiguous uint8 [num_pages, H_KV, page_size // {BLOCK}, {BLOCK_BYTES}]")
     page_size = shape[2] * BLOCK
     if page_size not in PAGE_SIZES:
@@ -73,21 +75,22 @@ def _pool(pages: torch.Tensor) -> Tuple[int, int, int]:
     return shape[0], shape[1], page_size
 
 
-def _vector(t: torch.Tensor, n: Optional[int], dtype, device, name: str) -> int:
-    """Address of a contiguous one-dimensional tensor."""
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != device or not t.is_contiguous():
-        raise HyQuantError(f"{name} must be contiguous {dtype} [{'n' if n is None else n}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _vector(t: torch.Tensor, n: int, dtype, device, name: str) -> int:
+    """Address of a contiguous one-dimensional tensor of n entries (-1: any number)."""
+    if t.dtype is dtype and t.device == device and t.dim() == 1 and (n < 0 or t.numel() == n) and t.is_contiguous():
+        return t.data_ptr()
+    raise HyQuantError(f"{name} must be contiguous {dtype} [{'n' if n < 0 else n}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _table(page_table: torch.Tensor, R: int, device) -> Tuple[int, int, int]:
     """(address, row stride, columns) of a block table."""
-    if page_table.dtype != _I32 or page_table.dim() != 2 or page_table.shape[0] != R or page_table.device != device:
+    if page_table.dtype is not _I32 or page_table.device != device or page_table.dim() != 2 or page_table.size(0) != R:
         raise HyQuantError(f"page_table must be int32 [{R}, max_pages] on {device}")
-    cols = page_table.shape[1]
-    if cols > 1 and page_table.stride(1) != 1:
+    cols = page_table.size(1)
+    stride, one = page_table.stride()
+    if cols > 1 and one != 1:
         raise HyQuantError("page_table rows must be contiguous")
-    return page_table.data_ptr(), page_table.stride(0) if R > 1 else max(cols, 1), cols
+    return page_table.data_ptr(), stride if R > 1 else max(cols, 1), cols
 
 
 def page_advance(kv_lens: torch.Tensor, held: torch.Tensor, add: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
@@ -104,28 +107,33 @@ def page_advance(kv_lens: torch.Tensor, held: torch.Tensor, add: torch.Tensor, p
 
     A step that cannot be done changes nothing and sets ``status``; its ``cu_q`` is 0 throughout and its slots -1, so that appending
     and attention do nothing with it."""
-    _lib.require_cuda(kv_lens, "kv_lens")
-    dev, R = kv_lens.device, kv_lens.shape[0]
+    if not kv_lens.is_cuda:
+        _lib.require_cuda(kv_lens, "kv_lens")
+    if kv_lens.dim() != 1:
+        raise HyQuantError("kv_lens must be int32 [R]")
+    dev, R = kv_lens.device, kv_lens.numel()
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
     if max_tokens < 0:
         raise ValueError(f"max_tokens must be >= 0, got {max_tokens}")
     lens_p, held_p, add_p = _vector(kv_lens, R, _I32, dev, "kv_lens"), _vector(held, R, _I32, dev, "held"), _vector(add, R, _I32, dev, "add")
     keep_p = None if keep is None else _vector(keep, R, _I32, dev, "keep")
-    free_p, count_p = _vector(free_pages, None, _I32, dev, "free_pages"), _vector(free_count, 1, _I32, dev, "free_count")
+    free_p, count_p = _vector(free_pages, -1, _I32, dev, "free_pages"), _vector(free_count, 1, _I32, dev, "free_count")
     table_p, stride, cols = _table(page_table, R, dev)
-    # one allocation: cu_q, positions, status, and the new state unless it goes over the old
-    ints = torch.empty(R + 2 + max_tokens + (0 if in_place else 2 * R + 1), dtype=_I32, device=dev)
     slots = torch.empty(max_tokens, dtype=_I64, device=dev)
-    cu_q, positions, status, rest = ints.split_with_sizes((R + 1, max_tokens, 1, ints.shape[0] - R - 2 - max_tokens))
     if in_place:
-        lens2, held2, count2 = kv_lens, held, free_count
+        ints = torch.empty(R + 2 + max_tokens, dtype=_I32, device=dev)
+        cu_q, positions, status = ints.split_with_sizes((R + 1, max_tokens, 1))
+        lens2, held2, count2, lens2_p, held2_p, count2_p = kv_lens, held, free_count, lens_p, held_p, count_p
+        base = ints.data_ptr()
     else:
-        lens2, held2, count2 = rest.split_with_sizes((R, R, 1))
-    base = ints.data_ptr()
-    rc = _call(_lib.lib().hq_page_advance, dev, lens_p, held_p, add_p, keep_p, R, table_p, stride, cols, free_p, free_pages.shape[0], count_p,
-               page_size, max_tokens, lens2.data_ptr(), held2.data_ptr(), count2.data_ptr(), base, slots.data_ptr(), base + 4 * (R + 1),
-               base + 4 * (R + 1 + max_tokens))
+        ints = torch.empty(3 * R + 3 + max_tokens, dtype=_I32, device=dev)
+        cu_q, positions, status, lens2, held2, count2 = ints.split_with_sizes((R + 1, max_tokens, 1, R, R, 1))
+        base = ints.data_ptr()
+        lens2_p = base + 4 * (R + 2 + max_tokens)
+        held2_p, count2_p = lens2_p + 4 * R, lens2_p + 8 * R
+    rc = _call(_lib.lib().hq_page_advance, dev, lens_p, held_p, add_p, keep_p, R, table_p, stride, cols, free_p, free_pages.numel(), count_p,
+               page_size, max_tokens, lens2_p, held2_p, count2_p, base, slots.data_ptr(), base + 4 * (R + 1), base + 4 * (R + 1 + max_tokens))
     if rc != 0:
         _lib.check(rc, "hq_page_advance")
     return PageStep(lens2, held2, count2, cu_q, slots, positions, status)
@@ -135,33 +143,39 @@ def paged_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: t
     """Quantise rows ``k``, ``v`` [T, H_KV, 128] (bf16, fp16 or fp32, views are fine) into their slots of ``pages``.  Slots that are -1
     or outside the pool are skipped; the others of one call are distinct."""
     num_pages, H, page_size = _pool(pages)
-    T, dev = slots.shape[0], pages.device
-    if k.shape != (T, H, 128) or v.shape != (T, H, 128) or k.dtype != v.dtype or k.device != dev or v.device != dev:
+    T, dev = slots.numel(), pages.device
+    if k.shape != (T, H, 128) or v.shape != k.shape or k.dtype is not v.dtype or k.device != dev or v.device != dev:
         raise HyQuantError(f"k and v must be [{T}, {H}, 128] of one dtype on {dev}, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     code = _lib.dtype_code(k.dtype)
     slots_p = _vector(slots, T, _I64, dev, "slots")
-    k, v = _rows(k), _rows(v)
-    rc = _call(_lib.lib().hq_paged_append, dev, k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), T, H,
-               slots_p, pages.data_ptr(), num_pages, page_size)
+    k, k_p, k_st, k_sh = _rows(k)
+    v, v_p, v_st, v_sh = _rows(v)
+    rc = _call(_lib.lib().hq_paged_append, dev, k_p, v_p, code, k_st, k_sh, v_st, v_sh, T, H, slots_p, pages.data_ptr(), num_pages, page_size)
     if rc != 0:
         _lib.check(rc, "hq_paged_append")
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x with rows of 128 that the kernels read in 16-byte pieces; a copy if it has none."""
+def _rows(x: torch.Tensor):
+    """(x, address, strides) with rows of 128 that the kernels read in 16-byte pieces; of a copy if x has none."""
     st, sh, sd = x.stride()
-    return x if sd == 1 and not (st | sh) & 7 and not x.data_ptr() & 15 else x.contiguous()
+    address = x.data_ptr()
+    if sd == 1 and not (st | sh) & 7 and not address & 15:
+        return x, address, st, sh
+    x = x.contiguous()
+    return x, x.data_ptr(), x.stride(0), x.stride(1)
 
 
 def paged_read(pages: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cache's values of ``slots`` as rows (k, v) [T, H_KV, 128] (fp16 and fp32 hold them exactly); zeros for slots outside the pool."""
     num_pages, H, page_size = _pool(pages)
     code = _lib.dtype_code(dtype)
-    T, dev = slots.shape[0], pages.device
+    T, dev = slots.numel(), pages.device
     slots_p = _vector(slots, T, _I64, dev, "slots")
-    k = torch.empty(T, H, 128, dtype=dtype, device=dev)
-    v = torch.empty(T, H, 128, dtype=dtype, device=dev)
-    rc = _call(_lib.lib().hq_paged_read, dev, pages.data_ptr(), num_pages, page_size, slots_p, T, H, code, k.data_ptr(), v.data_ptr())
+    rows = torch.empty((2, T, H, 128), dtype=dtype, device=dev)
+    k, v = rows.unbind(0)
+    k_p = rows.data_ptr()
+    rc = _call(_lib.lib().hq_paged_read, dev, pages.data_ptr(), num_pages, page_size, slots_p, T, H, code, k_p,
+               k_p + T * H * 128 * rows.element_size())
     if rc != 0:
         _lib.check(rc, "hq_paged_read")
     return k, v
@@ -177,44 +191,67 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
     ``max_q_len`` is the most tokens of a request (tokens beyond it are not computed).  ``sm_scale`` is 128 ** -0.5 by default.
     Rows of ``out`` behind the last token stay as they are (without ``out`` they are not initialised)."""
     num_pages, H, page_size = _pool(pages)
-    dev = pages.device
-    if q.dim() != 3 or q.shape[2] != 128 or q.device != dev:
-        raise HyQuantError(f"q must be [T, H_Q, 128] on {dev}, got {tuple(q.shape)} on {q.device}")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise HyQuantError(f"q must be bf16 or fp16, got {q.dtype}")
-    T, H_Q, _ = q.shape
-    if kv_lens.dim() != 1:
-        raise HyQuantError("kv_lens must be int32 [R]")
-    R = kv_lens.shape[0]
+    dev, dtype, shape = pages.device, q.dtype, q.shape
+    if len(shape) != 3 or shape[2] != 128 or q.device != dev:
+        raise HyQuantError(f"q must be [T, H_Q, 128] on {dev}, got {tuple(shape)} on {q.device}")
+    if dtype is torch.bfloat16:
+        code = _lib.HQ_BF16
+    elif dtype is torch.float16:
+        code = _lib.HQ_F16
+    else:
+        raise HyQuantError(f"q must be bf16 or fp16, got {dtype}")
+    T, H_Q, _ = shape
+    R = kv_lens.numel()
     lens_p = _vector(kv_lens, R, _I32, dev, "kv_lens")
     table_p, stride, cols = _table(page_table, R, dev)
     if cu_q is None:
         if T != R or max_q_len != 1:
             raise HyQuantError(f"without cu_q every request has one token: q has {T} rows, kv_lens {R}, max_q_len {max_q_len}")
-        cu_p = None
+        cu_p = 0
     else:
         cu_p = _vector(cu_q, R + 1, _I32, dev, "cu_q")
         if max_q_len < 1:
             raise ValueError(f"max_q_len must be >= 1, got {max_q_len}")
-    q = _rows(q)
+    q, q_p, q_st, q_sh = _rows(q)
     if out is None:
-        out = torch.empty(T, H_Q, 128, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-        raise HyQuantError(f"out must be {tuple(q.shape)} {q.dtype} on {dev} with contiguous rows")
-    a = PagedAttentionArgs(C.sizeof(PagedAttentionArgs), R, T, H_Q, H, 128, page_size, cols, max_q_len, _lib.dtype_code(q.dtype),
-                           128 ** -0.5 if sm_scale is None else sm_scale, 0, num_pages, q.data_ptr(), q.stride(0), q.stride(1),
-                           pages.data_ptr(), table_p, stride, lens_p, cu_p, out.data_ptr(), out.stride(0), out.stride(1), None, 0)
-    lib, n = _lib.lib(), C.c_int64()
-    ref = C.byref(a)
-    rc = lib.hq_paged_attention_workspace_bytes(ref, C.byref(n))
-    if rc == 0:
-        if n.value:
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-        rc = _call(lib.hq_paged_attention, dev, ref)
+        out = torch.empty(shape, dtype=dtype, device=dev)
+        o_st, o_sh = H_Q * 128, 128
+    else:
+        if out.shape != shape or out.dtype is not dtype or out.device != dev or out.stride(2) != 1:
+            raise HyQuantError(f"out must be {tuple(shape)} {dtype} on {dev} with contiguous rows")
+        o_st, o_sh, _ = out.stride()
+    a = [_ARGS_BYTES, R, T, H_Q, H, 128, page_size, cols, max_q_len, code, 128 ** -0.5 if sm_scale is None else sm_scale, 0, num_pages,
+         q_p, q_st, q_sh, pages.data_ptr(), table_p, stride, lens_p, cu_p, out.data_ptr(), o_st, o_sh, 0, 0]
+    need = _workspace_bytes(a, dev)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        a[24], a[25] = ws.data_ptr(), need
+    rc = _call(_lib.lib().hq_paged_attention, dev, _pack_args(*a))
     if rc != 0:
         _lib.check(rc, "hq_paged_attention")
     return out
+
+
+# hq_paged_attention_args as bytes: a block is read during the call and not kept, and packing one costs a fifth of filling a
+# ctypes structure.  The fields are those of PagedAttentionArgs.
+_ARGS_BYTES = C.sizeof(PagedAttentionArgs)
+_pack_args = struct.Struct("@10ifi14q").pack
+_workspace: dict = {}
+
+
+def _workspace_bytes(a, dev) -> int:
+    """Scratch of a call.  It depends on the heads, the longest request and, for short tables, the number of requests, so that the
+    answers for a device are few."""
+    key = dev.index, a[3], a[4], a[8], a[1] if a[1] == 0 or a[6] * a[7] <= 1024 else -1, a[2] > 0
+    need = _workspace.get(key)
+    if need is None:
+        n = C.c_int64()
+        _lib.check(_call(lambda block, out, stream: _lib.lib().hq_paged_attention_workspace_bytes(block, out), dev, _pack_args(*a), C.byref(n)),
+                   "hq_paged_attention_workspace_bytes")
+        if len(_workspace) > 4096:
+            _workspace.clear()
+        need = _workspace[key] = n.value
+    return need
 
 
 class PagedKVCache:

@@ -100,10 +100,11 @@ def attention(q, pages, table, lens, cu, sm_scale=None):
 
     The tolerance is what 16-bit operands and 32-bit sums may be off by: P~ rounded to fp16 (2^-11 of every term), scores summed
     over 128 products in 32 bits (128 * 2^-23 of the sum of magnitudes, on both sides of the quotient), 2^-16 for exponentials,
-    row sums and the quotient, and half a step of the output's type.  Terms that vanish: P~ is held as the fp16 number nearest to
-    2^9 p v_scale / (a power of two that is less than four times the largest v_scale), p = 1 at the reference or above it at the
-    maximum, so that a term is off by half of fp16's smallest step, 2^-25, at most: 2^-34 of 4 v_scale, or 2^-32 max|v| with
-    codes up to 7, against a row sum of at least 1; exponentials below the normal 32-bit numbers (2^-126) are far less.  Products of V:
+    row sums and the quotient, and half a step of the output's type.  Terms that vanish: P~ is held as
+    the fp16 number nearest to 2^e p v_scale for an e that makes the largest term of a row at least 8 (2^9 times a scale relative to
+    the largest one where references are taken, 256 over 32 terms where a first guess stays), so that a term is off by half of fp16's
+    smallest step, 2^-25, at most: 2^-28 of the largest p v_scale, 2^-25 max|v| with codes up to 7, against a row sum of at least 1;
+    exponentials below the normal 32-bit numbers (2^-126) are far less.  Products of V:
     the short form adds p (code + 8) v_scale and takes 8 p v_scale off again; its codes are fp16 numbers below the normal ones,
     (code + 8) 2^-24, whose exponent field is that of 2^-14.  The tensor core lines products up by these fields and keeps 24
     bits: the last one is 2^-37, or 2^-13 of a code, so that a product is off by 2^-13 p v_scale at most."""
@@ -142,5 +143,5 @@ def attention(q, pages, table, lens, cu, sm_scale=None):
             out[t0:t0 + n, h * G:h * G + G] = o
             tol[t0:t0 + n, h * G:h * G + G] = torch.finfo(q.dtype).eps / 2 * o.abs() * 1.01 + \
                 (2.0 ** -11 + 2 * delta + 2.0 ** -16) * (p @ vv.abs()) + \
-                2.0 ** -13 * (p @ vs[:, h]) + 2.0 ** -32 * L * vv.abs().max() / l.clamp(min=1.0) + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+                2.0 ** -13 * (p @ vs[:, h]) + 2.0 ** -25 * L * vv.abs().max() / l.clamp(min=1.0) + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
     return out, tol
