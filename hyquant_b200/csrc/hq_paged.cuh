@@ -25,6 +25,7 @@ static_assert(kVsOff + 2 * kTok == kBlockBytes && kBlockBytes % 16 == 0, "block 
 
 struct AttnParams {
   int R, T, H_Q, H_KV, G, page_shift, max_pages, max_q_len;
+  uint32_t g_inv;                              // row / G == __umulhi(row, g_inv) for rows below 2^27 (G > 1)
   float sml;                                   // sm_scale * log2(e)
   int dtype;
   int num_pages, page_bytes, blocks_mask;      // bytes of a page of one head; its blocks - 1
@@ -116,75 +117,77 @@ __device__ __forceinline__ Request request_of(const AttnParams& p, int r) {
   return x;
 }
 
-// a / b for a >= 0, b > 0: 64-bit division only where it is needed
-__device__ __forceinline__ long long quotient(long long a, int b) {
-  return (unsigned long long)a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
+// token of a row (token, head of the group)
+__device__ __forceinline__ int token_of(const AttnParams& p, int row) { return p.G == 1 ? row : (int)__umulhi((uint32_t)row, p.g_inv); }
 
-// Even cuts of `total` positions over the blocks of a launch: block b has `share` of them from share * b + min(b, more) on, the first
-// `more` blocks one more.
+// Even cuts of `total` positions (below 2^31) over the blocks of a launch: block b has `share` of them from share * b + min(b, more)
+// on, the first `more` blocks one more.
 struct Cuts {
-  long long total, share;
-  int blocks, more;
-  __device__ __forceinline__ Cuts(long long t, int n) : total(t), blocks(n) { share = quotient(t, n); more = (int)(t - share * n); }
-  __device__ __forceinline__ long long begin(int b) const { return share * b + min(b, more); }
-  __device__ __forceinline__ int block_of(long long pos) const {
-    const long long cut = (share + 1) * more;
-    return (int)(pos < cut ? quotient(pos, (int)(share + 1)) : more + quotient(pos - cut, (int)share));
+  int total, blocks, share, more;
+  __device__ __forceinline__ Cuts(int t, int n) : total(t), blocks(n) { share = (int)((uint32_t)t / (uint32_t)n); more = t - share * n; }
+  __device__ __forceinline__ int begin(int b) const { return share * b + min(b, more); }
+  __device__ __forceinline__ int block_of(int pos) const {
+    const int cut = (share + 1) * more;
+    return pos < cut ? (int)((uint32_t)pos / (uint32_t)(share + 1)) : more + (int)((uint32_t)(pos - cut) / (uint32_t)share);
   }
 };
 
-// The requests' weights in a row.  Up to 64 requests every warp adds them up by itself; more go through shared memory (s_part: threads + 1,
-// s_warp: a word per warp), a run of requests per thread.  All threads call the constructor, whole warps `seek`.
+// The requests' weights in a row.  Up to 64 requests every warp adds them up by itself; more go through shared memory (part: threads + 1
+// words, s_warp: a word per warp), a run of requests per thread.  All threads call the constructor, whole warps `seek`.
 template <int kThreads, class Weight>
 struct Prefix {
   const AttnParams& p;
   Weight weight;
-  long long total;
-  const long long* s_part;
-  long long w0, w1;                              // up to 64 requests: running sums at request `lane` and 32 + `lane`
+  int total, w0, w1;                             // up to 64 requests: running sums at request `lane` and 32 + `lane`
+  const int* s_part;
   int per;
-  __device__ __forceinline__ static long long scan(long long x) {
+  __device__ __forceinline__ static int scan(int x) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
     return x;
   }
-  __device__ __forceinline__ Prefix(const AttnParams& pp, Weight w, long long* part, long long* s_warp) : p(pp), weight(w), s_part(part) {
+  __device__ __forceinline__ Prefix(const AttnParams& pp, Weight w, int* part, int* s_warp) : p(pp), weight(w), s_part(part) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (p.R <= 64) {
-      w0 = lane < p.R ? weight(request_of(p, lane)) : 0;
-      w1 = 32 + lane < p.R ? weight(request_of(p, 32 + lane)) : 0;
-      w0 = scan(w0);
-      w1 = scan(w1) + __shfl_sync(0xffffffffu, w0, 31);
-      total = __shfl_sync(0xffffffffu, w1, 31);
+      w0 = scan(lane < p.R ? weight(request_of(p, lane)) : 0);
+      total = __shfl_sync(0xffffffffu, w0, 31);
+      if (p.R > 32) {
+        w1 = scan(32 + lane < p.R ? weight(request_of(p, 32 + lane)) : 0) + total;
+        total = __shfl_sync(0xffffffffu, w1, 31);
+      }
       return;
     }
     per = (p.R + kThreads - 1) / kThreads;
-    long long mine = 0;
+    int mine = 0;
     for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += weight(request_of(p, r));
-    const long long x = scan(mine);
+    const int x = scan(mine);
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    const long long sums = scan(lane < kThreads / 32 ? s_warp[lane] : 0), before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+    const int sums = scan(lane < kThreads / 32 ? s_warp[lane] : 0), before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
     total = __shfl_sync(0xffffffffu, sums, 31);
     part[tid + 1] = x + (warp ? before : 0);
     if (tid == 0) part[0] = 0;
     __syncthreads();
   }
   // the request that position pos < total lies in, and the position in it
-  __device__ __forceinline__ int seek(long long pos, long long& in) const {
+  __device__ __forceinline__ int seek(int pos, int& in) const {
     if (p.R <= 64) {
-      const int a = __popc(__ballot_sync(0xffffffffu, w0 <= pos)), b = __popc(__ballot_sync(0xffffffffu, w1 <= pos)), r = a < 32 ? a : 32 + b;
-      const long long below = r == 0 ? 0 : r <= 32 ? __shfl_sync(0xffffffffu, w0, r - 1) : __shfl_sync(0xffffffffu, w1, r - 33);
-      in = pos - below;
+      int r = __popc(__ballot_sync(0xffffffffu, w0 <= pos));
+      int below = __shfl_sync(0xffffffffu, w0, max(r - 1, 0));
+      if (r == 32) {
+        const int b = __popc(__ballot_sync(0xffffffffu, w1 <= pos)), y = __shfl_sync(0xffffffffu, w1, max(b - 1, 0));
+        if (b) below = y;
+        r += b;
+      }
+      in = r ? pos - below : pos;
       return r;
     }
     int lo = 0, hi = kThreads;
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (s_part[mid] <= pos) lo = mid; else hi = mid; }
     in = pos - s_part[lo];
     for (int r = lo * per;; ++r) {
-      const long long w = weight(request_of(p, r));
+      const int w = weight(request_of(p, r));
       if (in < w) return r;
       in -= w;
     }

@@ -24,6 +24,13 @@ static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a->cu_q || (a->R == a->T && a->max_q_len == 1), HQ_ERR_INVALID, "hq_paged_attention: without cu_q every request has one token");
   HQ_REQUIRE((int64_t)a->R * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %d requests of %d kv heads", a->R, a->H_KV);
   HQ_REQUIRE(a->num_pages * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %lld pages of %d kv heads", (long long)a->num_pages, a->H_KV);
+  HQ_REQUIRE((int64_t)a->T * (a->H_Q / a->H_KV) < (1 << 27), HQ_ERR_UNSUPPORTED, "hq_paged_attention: %d tokens of %d query heads a kv head", a->T,
+             a->H_Q / a->H_KV);
+  // places in the row of all requests' keys are 32-bit numbers: a key tile of 64 costs two, or one for each of 32 keys, and every query
+  // tile of 256 rows has its own
+  const double tiles = (double)a->R + (double)a->T * (a->H_Q / a->H_KV) / 256, keys = (double)a->max_pages * a->page_size;
+  HQ_REQUIRE(tiles * a->H_KV * (keys / 32 + 8) < 2147483647.0, HQ_ERR_UNSUPPORTED,
+             "hq_paged_attention: %d requests, %d tokens and tables of %d pages of %d tokens are too much for one call", a->R, a->T, a->max_pages, a->page_size);
   if (a->R == 0 || a->T == 0) return HQ_OK;
   HQ_REQUIRE(a->q && a->out && a->kv_lens && (a->page_table || a->max_pages == 0) && (a->pages || a->num_pages == 0), HQ_ERR_INVALID,
              "hq_paged_attention: null pointer");
@@ -37,6 +44,7 @@ static int check(const hq_paged_attention_args* a) {
 static AttnParams params_of(const hq_paged_attention_args* a) {
   AttnParams p{};
   p.R = a->R; p.T = a->T; p.H_Q = a->H_Q; p.H_KV = a->H_KV; p.G = a->H_Q / a->H_KV;
+  p.g_inv = (uint32_t)(0x100000000ull / (uint64_t)p.G) + 1u;      // G == 1 is not looked up
   p.page_shift = shift_of(a->page_size); p.max_pages = a->max_pages; p.max_q_len = a->max_q_len;
   p.sml = a->sm_scale * 1.44269504f;
   p.num_pages = (int)a->num_pages; p.page_bytes = kBlockBytes << (p.page_shift - 4); p.blocks_mask = (1 << (p.page_shift - 4)) - 1;

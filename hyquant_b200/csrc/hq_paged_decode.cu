@@ -106,11 +106,12 @@ __device__ __forceinline__ void store_row4(const AttnParams& p, int64_t at, floa
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = o;
 }
 __device__ __forceinline__ int64_t out_row(const AttnParams& p, const Request& q, int h, int n) {
-  return (int64_t)(q.q0 + n / p.G) * p.o_st + (int64_t)(h * p.G + n % p.G) * p.o_sh;
+  const int i = token_of(p, n);
+  return (int64_t)(q.q0 + i) * p.o_st + (int64_t)(h * p.G + n - i * p.G) * p.o_sh;
 }
 
 // a block has at least one position for every warp: fewer blocks take part in short calls
-__device__ __forceinline__ int blocks_of(long long total, int warps) { return (int)max(1ll, min((long long)gridDim.x, quotient(total, warps))); }
+__device__ __forceinline__ int blocks_of(int total, int warps) { return max(1, min((int)gridDim.x, total / warps)); }
 template <int NT>
 __device__ __forceinline__ Merge* todo_of(const AttnParams& p) { return reinterpret_cast<Merge*>(p.ws + ws_merge<NT>(gridDim.x)) + blockIdx.x; }
 
@@ -123,9 +124,10 @@ decode_kernel(const AttnParams p, bool whole) {
   __shared__ uint64_t bars[kWarps * kSlots];
   __shared__ int s_live[kWarps * kSlots];                    // which of a unit's two blocks lie in the pool
   __shared__ int2 s_page[kWarps][32];                        // pages of a unit's blocks, 32 units ahead
-  __shared__ long long s_cut[2];                             // where the block's part begins, all positions
-  __shared__ long long s_part[kThreads + 1], s_warp[kWarps];
-  __shared__ int s_seg[32], s_q0[32], s_nq[32];              // run (r * H_KV + h) of a warp's first and last piece, or -1; its request
+  __shared__ int s_cut[2];                             // where the block's part begins, all positions
+  __shared__ int s_part[kThreads + 1], s_warp[kWarps];
+  __shared__ int s_seg[32];                                  // run (r * H_KV + h) of a warp's first and last piece, or -1
+  __shared__ int4 s_run[32];                                 // its first row of q, rows, head
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   if (tid < kWarps * kSlots) { mbar_init(bars + tid, 1); fence_mbar_init(); }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -135,7 +137,7 @@ decode_kernel(const AttnParams p, bool whole) {
   const int block = blockIdx.x;
   Walk c{0, 0, 0, -1};
   int left = 0;
-  auto weight = [&](const Request& q) { return (long long)p.H_KV * (units_of(q) + 1); };
+  auto weight = [&](const Request& q) { return p.H_KV * (units_of(q) + 1); };
   if (whole) {                                               // one run a block
     __syncthreads();
     c.r = block / p.H_KV; c.h = block - c.r * p.H_KV;
@@ -149,17 +151,15 @@ decode_kernel(const AttnParams p, bool whole) {
     if (p.R <= 64) __syncthreads();
     const Cuts cuts(prefix.total, blocks_of(prefix.total, kWarps));
     if (block >= cuts.blocks) { if (tid == 0) todo_of<NT>(p)->go = 0; return; }
-    const long long b0 = cuts.begin(block), n = cuts.begin(block + 1) - b0;
+    const int b0 = cuts.begin(block), n = cuts.begin(block + 1) - b0, each = n / kWarps, rest = n - each * kWarps;
     if (tid == 0) { s_cut[0] = b0; s_cut[1] = prefix.total; }
-    const long long first = (unsigned long long)n >> 26 ? n * warp / kWarps : (int)n * warp / kWarps;
-    const long long last = (unsigned long long)n >> 26 ? n * (warp + 1) / kWarps : (int)n * (warp + 1) / kWarps;
-    left = (int)(last - first);
+    left = each + (warp < rest ? 1 : 0);
     if (left > 0) {
-      long long in;
-      c.r = prefix.seek(b0 + first, in);
+      int in;
+      c.r = prefix.seek(b0 + each * warp + min(warp, rest), in);
       c.units = units_of(request_of(p, c.r));
-      c.h = (int)quotient(in, c.units + 1);
-      c.u = (int)(in - (long long)c.h * (c.units + 1));
+      c.h = (int)((uint32_t)in / (uint32_t)(c.units + 1));
+      c.u = in - c.h * (c.units + 1);
     }
   }
   const int start_u = c.u;                                   // the part begins inside a run if start_u > 0
@@ -218,7 +218,7 @@ decode_kernel(const AttnParams p, bool whole) {
     lim0 = q.past + 1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int n = 8 * nt + g, i = n / p.G;
+      const int n = 8 * nt + g, i = token_of(p, n);
       const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st +
                                                        (int64_t)(c.h * p.G + n - i * p.G) * p.q_sh + 32 * t4);
 #pragma unroll
@@ -266,8 +266,7 @@ decode_kernel(const AttnParams p, bool whole) {
     }
   };
   // The run's rows so far: the 8 of the codes taken off, the powers of two put back.  To the output (piece == nullptr) or as a piece.
-  auto finish = [&](float* piece) {
-    const Request q = request_of(p, c.r);
+  auto finish = [&](float* piece, const Request& q) {
     const int rows = q.nq * p.G;
     const float back = 1.f / vback;                          // a power of two, exact
 #pragma unroll
@@ -277,16 +276,28 @@ decode_kernel(const AttnParams p, bool whole) {
       for (int j = 0; j < 2; ++j) {
         const int n = 8 * nt + 2 * t4 + j;
         const float f = piece ? back : ls[j] == 0.f ? 0.f : back / ls[j], eight = -8.f * Ls[nt][j] * f, f24 = f * 0x1p24f, f20 = f * 0x1p20f;
-        if (n < rows) {
-          const int64_t at = out_row(p, q, c.h, n) + 16 * g;
+        float v[16];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const float4 v = make_float4(fmaf(O[nt][2 * q4][j], f24, eight), fmaf(O[nt][2 * q4 + 1][j], f20, eight),
-                                         fmaf(O[nt][2 * q4][2 + j], f24, eight), fmaf(O[nt][2 * q4 + 1][2 + j], f20, eight));
-            if (piece) *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = v;
-            else store_row4<kBf16>(p, at + 4 * q4, v, 1.f);
+        for (int q4 = 0; q4 < 4; ++q4) {
+          v[4 * q4] = fmaf(O[nt][2 * q4][j], f24, eight); v[4 * q4 + 1] = fmaf(O[nt][2 * q4 + 1][j], f20, eight);
+          v[4 * q4 + 2] = fmaf(O[nt][2 * q4][2 + j], f24, eight); v[4 * q4 + 3] = fmaf(O[nt][2 * q4 + 1][2 + j], f20, eight);
+        }
+        if (n >= rows) continue;
+        if (piece) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = make_float4(v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]);
+          if (g == 0) { piece[8 * NT * kRowPad + n] = -(j ? shift[nt].y : shift[nt].x); piece[8 * NT * kRowPad + 8 * NT + n] = ls[j]; }
+        } else {
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (kBf16) { const __nv_bfloat162 hh = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]); w[k] = *reinterpret_cast<const uint32_t*>(&hh); }
+            else { const __half2 hh = __floats2half2_rn(v[2 * k], v[2 * k + 1]); w[k] = *reinterpret_cast<const uint32_t*>(&hh); }
           }
-          if (piece && g == 0) { piece[8 * NT * kRowPad + n] = -(j ? shift[nt].y : shift[nt].x); piece[8 * NT * kRowPad + 8 * NT + n] = ls[j]; }
+          uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + out_row(p, q, c.h, n) + 16 * g);
+          to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          to[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
     }
@@ -348,7 +359,7 @@ decode_kernel(const AttnParams p, bool whole) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              if (!here || tok >= lim0 + min((8 * nt + 2 * t4 + j) / p.G, q.nq - 1)) S[nt][cb][2 * i + j] = -INFINITY;
+              if (!here || tok >= lim0 + min(token_of(p, 8 * nt + 2 * t4 + j), q.nq - 1)) S[nt][cb][2 * i + j] = -INFINITY;
         }
     }
     // P against the references as they stand: a row's reference maximum, the power of two of the V scales.  Nothing is compared
@@ -445,7 +456,9 @@ decode_kernel(const AttnParams p, bool whole) {
   if (tid < 32) s_seg[tid] = -1;
   __syncthreads();
   bool inside = start_u > 0;                                 // the run in hand began before this part
-  if (left > 0) ask_q();
+  // the first unit is asked for before anything else, the others of the ring behind the queries: a copy takes the SM's copy engine some
+  // 25 ns, 16 warps' rings 1.2 us
+  if (left > 0) { ask_q(); fetch(); ++ahead; }
 #pragma unroll 1
   while (left > 0) {
 #pragma unroll
@@ -463,9 +476,9 @@ decode_kernel(const AttnParams p, bool whole) {
     const int n = min(c.units - c.u, left);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-#pragma unroll 1
-      for (; ahead < kSlots; ++ahead) fetch();               // three at first, then the slot that has just been read
       if (i == 0) open();
+#pragma unroll 1
+      for (; ahead < kSlots; ++ahead) fetch();               // the slot that has just been read
       unit(i == 0);
       --ahead;
       ++c.u;
@@ -474,18 +487,19 @@ decode_kernel(const AttnParams p, bool whole) {
     const bool ends = left > 0;                              // else it goes on in the next part
     float* mine = reinterpret_cast<float*>(ring);            // empty when it is the part's last
     float* piece = !ends ? mine : !inside ? nullptr : whole ? mine : p.ws + (int64_t)(block * kWarps + warp) * piece_floats(NT);
-    finish(piece);
+    const Request q = request_of(p, c.r);
+    finish(piece, q);
     if (piece && lane == 0) {
       const int at = 2 * warp + (ends ? 0 : 1);
-      const Request q = request_of(p, c.r);
-      s_seg[at] = c.r * p.H_KV + c.h; s_q0[at] = q.q0; s_nq[at] = q.nq;
+      s_seg[at] = c.r * p.H_KV + c.h;
+      s_run[at] = make_int4(q.q0, q.nq, c.h, 0);
     }
     if (ends && --left > 0) { inside = false; next_run(p, c); ask_q(); }
   }
-  if (!whole && tid == 0) todo_of<NT>(p)->go = 0;
+  if (!whole && tid == kThreads - 1) todo_of<NT>(p)->go = 0;
 
   // ---- runs that several warps share: pieces in order are the warps' first and last ones, a lane each; neighbours of the same
-  // run are a group.  A warp takes a row of a group at a time.
+  // run are a group.  A warp takes half a row of a group at a time.
   __syncthreads();
   const int seg = s_seg[lane];
   const uint32_t valid = __ballot_sync(0xffffffffu, seg >= 0);
@@ -493,46 +507,64 @@ decode_kernel(const AttnParams p, bool whole) {
   const uint32_t below = valid & ((1u << lane) - 1u);
   const int prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : 0);
   const uint32_t heads = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0u || prev != seg));
-  const float* my_piece = (lane & 1) || whole ? reinterpret_cast<const float*>(smem + (lane >> 1) * (kSlots * kUnitBytes))
-                                              : p.ws + (int64_t)(block * kWarps + (lane >> 1)) * piece_floats(NT);
+  auto piece_of = [&](int i) {
+    return (i & 1) || whole ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes)) : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
+  };
+  const float* my_piece = piece_of(lane);
+  const bool first_before = !whole && s_before > 0;          // the first group's run began in another block
   int item = 0;
 #pragma unroll 1
   for (uint32_t rest = heads; rest; rest &= rest - 1) {
     const int head = __ffs(rest) - 1;
     const uint32_t later = rest & (rest - 1);
     const uint32_t group = valid & ~((1u << head) - 1u) & (later ? (later & (0u - later)) - 1u : 0xffffffffu);
-    const int id = s_seg[head], q0 = s_q0[head], nq = s_nq[head], rows = nq * p.G, h = id % p.H_KV;
-    const bool began_before = !whole && head == __ffs(valid) - 1 && s_before > 0, ends = ((31 - __clz(group)) & 1) == 0;
-    if (began_before && ends && tid == 0) *todo_of<NT>(p) = Merge{q0, nq, h, Cuts(s_cut[1], blocks_of(s_cut[1], kWarps)).block_of(s_cut[0] - s_before), 1, {0, 0, 0}};
+    const int4 run = s_run[head];
+    const int rows = run.y * p.G;
+    const bool began_before = first_before && rest == heads, ends = ((31 - __clz(group)) & 1) == 0;
+    const bool in = (group >> lane) & 1u;
 #pragma unroll 1
-    for (int n = 0; n < rows; ++n, ++item) {
-      if (item % kWarps != warp) continue;
-      const bool in = (group >> lane) & 1u;
-      const float mi = in ? my_piece[8 * NT * kRowPad + n] : -INFINITY;
+    for (int n2 = (warp + kWarps - item % kWarps) % kWarps; n2 < 2 * rows; n2 += kWarps) {
+      const int n = n2 >> 1, ch = 64 * (n2 & 1) + 2 * lane;
+      const float mi = in ? my_piece[8 * NT * kRowPad + n] : -INFINITY, li = in ? my_piece[8 * NT * kRowPad + 8 * NT + n] : 0.f;
       float M = mi;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       const float w = ex2f(mi - (M == -INFINITY ? 0.f : M));
-      float L = in ? w * my_piece[8 * NT * kRowPad + 8 * NT + n] : 0.f;
+      float L = w * li;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float2 acc = make_float2(0.f, 0.f);
+      uint32_t x = group;
 #pragma unroll 1
-      for (uint32_t x = group; x; x &= x - 1) {
-        const int i = __ffs(x) - 1;
-        const float* from = (i & 1) || whole ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes))
-                                             : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
-        const float4 v = *reinterpret_cast<const float4*>(from + n * kRowPad + 4 * lane);
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        acc.x += wi * v.x; acc.y += wi * v.y; acc.z += wi * v.z; acc.w += wi * v.w;
+      while (x) {                                            // four pieces' loads at a time
+        float2 v[4];
+        float wi[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = x ? __ffs(x) - 1 : head;
+          wi[k] = __shfl_sync(0xffffffffu, w, i);
+          if (!x) wi[k] = 0.f;
+          v[k] = *reinterpret_cast<const float2*>(piece_of(i) + n * kRowPad + ch);
+          x &= x - 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { acc.x = fmaf(wi[k], v[k].x, acc.x); acc.y = fmaf(wi[k], v[k].y, acc.y); }
       }
-      if (!began_before && ends) store_row4<kBf16>(p, out_row(p, Request{q0, nq, 0, 0}, h, n) + 4 * lane, acc, L == 0.f ? 0.f : 1.f / L);
-      else {
+      if (!began_before && ends) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;          // a row that saw no key: 0
+        uint32_t o;
+        if (kBf16) { const __nv_bfloat162 hh = __floats2bfloat162_rn(acc.x * inv, acc.y * inv); o = *reinterpret_cast<const uint32_t*>(&hh); }
+        else { const __half2 hh = __floats2half2_rn(acc.x * inv, acc.y * inv); o = *reinterpret_cast<const uint32_t*>(&hh); }
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + out_row(p, Request{run.x, run.y, 0, 0}, run.z, n) + ch) = o;
+      } else {
         float* to = p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block + (began_before ? 0 : 1)) * piece_floats(NT);
-        *reinterpret_cast<float4*>(to + n * kRowPad + 4 * lane) = acc;
-        if (lane == 0) { to[8 * NT * kRowPad + n] = M; to[8 * NT * kRowPad + 8 * NT + n] = L; }
+        *reinterpret_cast<float2*>(to + n * kRowPad + ch) = acc;
+        if (lane == 0) { to[8 * NT * kRowPad + n] = M; to[8 * NT * kRowPad + 8 * NT + n] = L; }      // (both halves write the same)
       }
     }
+    item += 2 * rows;
+    if (began_before && ends && tid == kThreads - 1)
+      *todo_of<NT>(p) = Merge{run.x, run.y, run.z, Cuts(s_cut[1], blocks_of(s_cut[1], kWarps)).block_of(s_cut[0] - s_before), 1, {0, 0, 0}};
   }
 }
 

@@ -53,7 +53,7 @@ struct Item {
 __device__ __forceinline__ int query_tiles(const AttnParams& p, const Request& q) { return (q.nq * p.G + kRows - 1) / kRows; }
 __device__ __forceinline__ void size_item(const AttnParams& p, Item& x) {
   const int rows = x.q.nq * p.G, last = min(rows, (x.qt + 1) * kRows) - 1;
-  const int keys = min(x.q.len, x.q.past + 1 + last / p.G);
+  const int keys = min(x.q.len, x.q.past + 1 + token_of(p, last));
   x.tiles = keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
   x.cost = rows - x.qt * kRows > 128 ? 2 : 1;
 }
@@ -75,12 +75,11 @@ __device__ __forceinline__ void next_item(const AttnParams& p, Item& x) {
 // A block's part as pieces of query tiles: key tiles [t0, t1) of `it`
 struct Pieces {
   Item it;
-  long long left;
-  int t0, t1;
+  int left, t0, t1;
   bool began, ends;                              // earlier, in another block; here
   __device__ __forceinline__ bool take(const AttnParams& p) {
     while (left > 0) {
-      const int to = (int)min((long long)it.tiles * it.cost, it.u + left);
+      const int to = min(it.tiles * it.cost, it.u + left);
       t0 = (it.u + it.cost - 1) / it.cost;
       t1 = (to + it.cost - 1) / it.cost;
       began = it.u > 0;
@@ -208,7 +207,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
   uint64_t* drained = pv_done + 4;               // [half]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ long long s_part[kTileThreads + 1], s_warp[kTileThreads / 32];
+  __shared__ int s_part[kTileThreads + 1], s_warp[kTileThreads / 32];
   __shared__ float2 s_state[2][128];             // (maximum, sum) of a half's rows, for the other
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
@@ -233,16 +232,16 @@ tile_kernel(const AttnParams p, int piece_rows) {
     x.q = q;
     int w = 0;
     for (x.qt = 0, x.n_qt = query_tiles(p, q); x.qt < x.n_qt; ++x.qt) { size_item(p, x); w += x.positions(); }
-    return (long long)w * p.H_KV;
+    return w * p.H_KV;
   };
   const Prefix<kTileThreads, decltype(weight)> prefix(p, weight, s_part, s_warp);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const Cuts cuts(prefix.total, (int)max(1ll, min((long long)gridDim.x, quotient(prefix.total, kItemCost + 2))));
+  const Cuts cuts(prefix.total, max(1, min((int)gridDim.x, prefix.total / (kItemCost + 2))));
   const int block = blockIdx.x;
-  const long long b0 = cuts.begin(block);
+  const int b0 = cuts.begin(block);
   const int64_t piece_floats = (int64_t)piece_rows * 130;
   TileMerge* todo = reinterpret_cast<TileMerge*>(p.ws + 2 * piece_floats * gridDim.x) + block;
   if (tid == 0) todo->go = 0;
@@ -250,19 +249,19 @@ tile_kernel(const AttnParams p, int piece_rows) {
   pc.left = block < cuts.blocks ? cuts.begin(block + 1) - b0 : 0;
   if (pc.left > 0) {
     Item it;
-    long long in;
+    int in;
     it.r = prefix.seek(b0, in);
     it.q = request_of(p, it.r);
-    const int w = (int)quotient(weight(it.q), p.H_KV);
-    it.h = (int)quotient(in, w);
-    in -= (long long)it.h * w;
+    const int w = weight(it.q) / p.H_KV;
+    it.h = in / w;
+    in -= it.h * w;
     it.n_qt = query_tiles(p, it.q);
     for (it.qt = 0;; ++it.qt) {
       size_item(p, it);
       if (in < it.positions()) break;
       in -= it.positions();
     }
-    it.u = (int)in;
+    it.u = in;
     pc.it = it;
   }
   int* key_rows = reinterpret_cast<int*>(smem + TileSmem::Rows);           // [kAhead] keys of a tile that are there, the last ones missing
@@ -441,7 +440,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
       const bool split = pc.split();
       const int row0 = pc.it.qt * kRows + (split ? 0 : 128 * half), rows = min(128, q.nq * p.G - row0);
       const int n_all = pc.t1 - pc.t0, first = split ? half : 0, step = split ? 2 : 1, n = (n_all - first + step - 1) / step;
-      const int row = row0 + r, i = row / p.G;
+      const int row = row0 + r, i = token_of(p, row);
       float m = -INFINITY, l = 0.f;
       if (n > 0 && ok) {
         // queries: scaled by a power of two of the row so that fp16 holds them exactly, into the operand tile
@@ -602,9 +601,10 @@ tile_kernel(const AttnParams p, int piece_rows) {
           }
           __syncwarp();
           if (whole) {                           // four lanes a row, 64 bytes
-#pragma unroll 1
-            for (int rr = lane >> 2; rr < 32 && wq * 32 + rr < rows; rr += 8) {
-              const int part = lane & 3, orow = row0 + wq * 32 + rr, gi = orow / p.G;
+#pragma unroll 4
+            for (int rr = lane >> 2; rr < 32; rr += 8) {
+              if (wq * 32 + rr >= rows) break;
+              const int part = lane & 3, orow = row0 + wq * 32 + rr, gi = token_of(p, orow);
               *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + (int64_t)(q.q0 + gi) * p.o_st +
                                         (int64_t)(pc.it.h * p.G + orow - gi * p.G) * p.o_sh + ch * 32 + part * 8) =
                   *reinterpret_cast<const uint4*>(stage + rr * 128 + ((part ^ (rr & 7)) << 4));
@@ -626,7 +626,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
       }
       if (split) { tc::fence_before_sync(); halves_meet(); }           // the other half has read this one's O and state
       if (pc.began && pc.ends && tid == 0) {
-        const long long start = b0 - pc.it.u;    // where the query tile begins: the block of that position has its first piece
+        const int start = b0 - pc.it.u;    // where the query tile begins: the block of that position has its first piece
         *todo = TileMerge{q.q0, min(kRows, q.nq * p.G - pc.it.qt * kRows), pc.it.h, pc.it.qt, cuts.block_of(start), 1, {0, 0}};
       }
       pc.done(p);
@@ -658,7 +658,7 @@ tile_merge_kernel(const AttnParams p, int piece_rows, int grid) {
     M = nm;
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int grow = todo.qt * kRows + row, gi = grow / p.G;
+  const int grow = todo.qt * kRows + row, gi = token_of(p, grow);
   const int64_t at = (int64_t)(todo.q0 + gi) * p.o_st + (int64_t)(todo.h * p.G + grow - gi * p.G) * p.o_sh + 4 * lane;
   uint2 o;
   if (p.dtype == HQ_BF16) {
