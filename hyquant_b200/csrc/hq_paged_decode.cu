@@ -205,33 +205,29 @@ decode_kernel(const AttnParams p, bool whole) {
 
   // ---- the state of the run in hand
   uint32_t qf[NT][16];                                       // query operand: word w, nibble k at 4 w + k
-  uint4 raw[NT][4];                                          // its row as it lies: channels 32 t4 .. + 31
+  uint4 raw[4];                                              // a tile's rows as they lie: channels 32 t4 .. + 31
   float2 fac[NT], start[NT];                                 // factor of a score, start of the accumulators: columns 2 t4, 2 t4 + 1
   float2 l[NT], shift[NT];                                   // P = 2^(score + shift); kNone: no key so far
   const Masks km = masks();
   float O[NT][8][4], Ls[NT][4];
   float vback = 1.f;                                         // V scales are taken times this power of two
   int lim0 = 0;                                              // keys that the run's first token sees
-  auto ask_q = [&]() {
-    const Request q = request_of(p, c.r);
-    const int rows = q.nq * p.G;
+  auto ask_q = [&](const Request& q, int nt) {
+    const int n = 8 * nt + g, i = token_of(p, n);
+    const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st +
+                                                     (int64_t)(c.h * p.G + n - i * p.G) * p.q_sh + 32 * t4);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) raw[w] = n < q.nq * p.G ? __ldg(at + w) : make_uint4(0u, 0u, 0u, 0u);
     lim0 = q.past + 1;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int n = 8 * nt + g, i = token_of(p, n);
-      const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st +
-                                                       (int64_t)(c.h * p.G + n - i * p.G) * p.q_sh + 32 * t4);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) raw[nt][w] = n < rows ? __ldg(at + w) : make_uint4(0u, 0u, 0u, 0u);
-    }
   };
   auto open = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      if (nt > 0) ask_q(request_of(p, c.r), nt);
       uint32_t top2 = 0u;                                    // magnitudes of 16-bit numbers order like integers
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint4 u = raw[nt][w];
+        const uint4 u = raw[w];
         top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, u.x & 0x7FFF7FFFu), u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
       }
       top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
@@ -246,7 +242,7 @@ decode_kernel(const AttnParams p, bool whole) {
       const float scale = __uint_as_float((uint32_t)(127 + up) << 23), scale16 = scale * 0.0625f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint32_t u[4] = {raw[nt][w].x, raw[nt][w].y, raw[nt][w].z, raw[nt][w].w};
+        const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {                        // channels k and k + 4 of the eight
           const float2 x = fmul2(make_float2(value(u[k >> 1], k & 1), value(u[2 + (k >> 1)], k & 1)),
@@ -368,8 +364,7 @@ decode_kernel(const AttnParams p, bool whole) {
     // if every row's sum comes out large enough for fp16's lower end, too.
     uint32_t P[NT][2][2];
     float2 le[NT];
-#pragma unroll 1
-    for (int pass = 0;; ++pass) {
+    auto form = [&](bool first) {                            // true where the references do not fit
       float most = 0.f;
       bool fits = true;
 #pragma unroll
@@ -390,14 +385,15 @@ decode_kernel(const AttnParams p, bool whole) {
             P[nt][cb][i] = *reinterpret_cast<const uint32_t*>(&hh);
           }
         most += sum.x + sum.y;
-        if (fresh && pass == 0) {
+        if (first) {
           const int n = 8 * nt + 2 * t4, rows = request_of(p, c.r).nq * p.G;
           const float x0 = over_g(sum.x, false), x1 = over_g(sum.y, false);
           fits = fits && (x0 >= kLeast || n >= rows) && (x1 >= kLeast || n + 1 >= rows);
         }
       }
-      if (pass) break;
-      if (!__any_sync(0xffffffffu, !(most <= 32768.f) || !fits)) break;
+      return !(most <= 32768.f) || !fits;
+    };
+    if (__builtin_expect(__any_sync(0xffffffffu, form(fresh)), 0)) {
       const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
       // 2^-e for the largest scale's power of two e, kept in the range of normal numbers; smaller than before unless nothing was before
       const int e = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23), 1), 253);
@@ -418,6 +414,7 @@ decode_kernel(const AttnParams p, bool whole) {
         Ls[nt][0] *= av.x; Ls[nt][1] *= av.y; Ls[nt][2] *= av.x; Ls[nt][3] *= av.y;
         shift[nt] = ns;
       }
+      form(false);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -458,7 +455,7 @@ decode_kernel(const AttnParams p, bool whole) {
   bool inside = start_u > 0;                                 // the run in hand began before this part
   // the first unit is asked for before anything else, the others of the ring behind the queries: a copy takes the SM's copy engine some
   // 25 ns, 16 warps' rings 1.2 us
-  if (left > 0) { ask_q(); fetch(); ++ahead; }
+  if (left > 0) { ask_q(request_of(p, c.r), 0); fetch(); ++ahead; }
 #pragma unroll 1
   while (left > 0) {
 #pragma unroll
@@ -494,7 +491,7 @@ decode_kernel(const AttnParams p, bool whole) {
       s_seg[at] = c.r * p.H_KV + c.h;
       s_run[at] = make_int4(q.q0, q.nq, c.h, 0);
     }
-    if (ends && --left > 0) { inside = false; next_run(p, c); ask_q(); }
+    if (ends && --left > 0) { inside = false; next_run(p, c); ask_q(request_of(p, c.r), 0); }
   }
   if (!whole && tid == kThreads - 1) todo_of<NT>(p)->go = 0;
 
