@@ -128,6 +128,7 @@ decode_kernel(const AttnParams p, bool whole) {
   __shared__ int s_part[kThreads + 1], s_warp[kWarps];
   __shared__ int s_seg[32];                                  // run (r * H_KV + h) of a warp's first and last piece, or -1
   __shared__ int4 s_run[32];                                 // its first row of q, rows, head
+  __shared__ float s_max[8 * NT][32], s_sum[8 * NT][32];     // (log2) maximum and sum of a piece's rows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   if (tid < kWarps * kSlots) { mbar_init(bars + tid, 1); fence_mbar_init(); }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -262,7 +263,7 @@ decode_kernel(const AttnParams p, bool whole) {
     }
   };
   // The run's rows so far: the 8 of the codes taken off, the powers of two put back.  To the output (piece == nullptr) or as a piece.
-  auto finish = [&](float* piece, const Request& q) {
+  auto finish = [&](float* piece, int at_piece, const Request& q) {
     const int rows = q.nq * p.G;
     const float back = 1.f / vback;                          // a power of two, exact
 #pragma unroll
@@ -283,7 +284,7 @@ decode_kernel(const AttnParams p, bool whole) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
             *reinterpret_cast<float4*>(piece + n * kRowPad + 16 * g + 4 * q4) = make_float4(v[4 * q4], v[4 * q4 + 1], v[4 * q4 + 2], v[4 * q4 + 3]);
-          if (g == 0) { piece[8 * NT * kRowPad + n] = -(j ? shift[nt].y : shift[nt].x); piece[8 * NT * kRowPad + 8 * NT + n] = ls[j]; }
+          if (g == 0) { s_max[n][at_piece] = -(j ? shift[nt].y : shift[nt].x); s_sum[n][at_piece] = ls[j]; }
         } else {
           uint32_t w[8];
 #pragma unroll
@@ -485,49 +486,42 @@ decode_kernel(const AttnParams p, bool whole) {
     float* mine = reinterpret_cast<float*>(ring);            // empty when it is the part's last
     float* piece = !ends ? mine : !inside ? nullptr : whole ? mine : p.ws + (int64_t)(block * kWarps + warp) * piece_floats(NT);
     const Request q = request_of(p, c.r);
-    finish(piece, q);
+    const int at = 2 * warp + (ends ? 0 : 1);
+    finish(piece, at, q);
     if (piece && lane == 0) {
-      const int at = 2 * warp + (ends ? 0 : 1);
       s_seg[at] = c.r * p.H_KV + c.h;
       s_run[at] = make_int4(q.q0, q.nq, c.h, 0);
     }
     if (ends && --left > 0) { inside = false; next_run(p, c); ask_q(request_of(p, c.r), 0); }
   }
-  if (!whole && tid == kThreads - 1) todo_of<NT>(p)->go = 0;
 
   // ---- runs that several warps share: pieces in order are the warps' first and last ones, a lane each; neighbours of the same
   // run are a group.  A warp takes half a row of a group at a time.
   __syncthreads();
   const int seg = s_seg[lane];
-  const uint32_t valid = __ballot_sync(0xffffffffu, seg >= 0);
-  if (valid == 0) return;
-  const uint32_t below = valid & ((1u << lane) - 1u);
+  const uint32_t valid = __ballot_sync(0xffffffffu, seg >= 0), below = valid & ((1u << lane) - 1u);
   const int prev = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : 0);
   const uint32_t heads = __ballot_sync(0xffffffffu, seg >= 0 && (below == 0u || prev != seg));
-  auto piece_of = [&](int i) {
-    return (i & 1) || whole ? reinterpret_cast<const float*>(smem + (i >> 1) * (kSlots * kUnitBytes)) : p.ws + (int64_t)(block * kWarps + (i >> 1)) * piece_floats(NT);
-  };
-  const float* my_piece = piece_of(lane);
   const bool first_before = !whole && s_before > 0;          // the first group's run began in another block
-  int item = 0;
+  float* to = whole ? nullptr : p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block) * piece_floats(NT);
+  Merge todo{0, 0, 0, 0, 0, {0, 0, 0}};
+  int turn = warp;                                           // items are dealt out over all groups
 #pragma unroll 1
   for (uint32_t rest = heads; rest; rest &= rest - 1) {
     const int head = __ffs(rest) - 1;
     const uint32_t later = rest & (rest - 1);
     const uint32_t group = valid & ~((1u << head) - 1u) & (later ? (later & (0u - later)) - 1u : 0xffffffffu);
     const int4 run = s_run[head];
-    const int rows = run.y * p.G;
-    const bool began_before = first_before && rest == heads, ends = ((31 - __clz(group)) & 1) == 0;
-    const bool in = (group >> lane) & 1u;
+    const int items = 2 * run.y * p.G;
+    const bool began_before = first_before && rest == heads, ends = ((31 - __clz(group)) & 1) == 0, in = (group >> lane) & 1u;
+    if (began_before && ends) todo = Merge{run.x, run.y, run.z, 0, 1, {0, 0, 0}};
 #pragma unroll 1
-    for (int n2 = (warp + kWarps - item % kWarps) % kWarps; n2 < 2 * rows; n2 += kWarps) {
-      const int n = n2 >> 1, ch = 64 * (n2 & 1) + 2 * lane;
-      const float mi = in ? my_piece[8 * NT * kRowPad + n] : -INFINITY, li = in ? my_piece[8 * NT * kRowPad + 8 * NT + n] : 0.f;
-      float M = mi;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      const float w = ex2f(mi - (M == -INFINITY ? 0.f : M));
-      float L = w * li;
+    for (; turn < items; turn += kWarps) {
+      const int n = turn >> 1, ch = 64 * (turn & 1) + 2 * lane;
+      const float mi = in ? s_max[n][lane] : -INFINITY;
+      const int mb = __float_as_int(mi), top = __reduce_max_sync(0xffffffffu, mb >= 0 ? mb : mb ^ 0x7FFFFFFF);
+      const float M = __int_as_float(top >= 0 ? top : top ^ 0x7FFFFFFF), w = ex2f(mi - M);
+      float L = in ? w * s_sum[n][lane] : 0.f;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       float2 acc = make_float2(0.f, 0.f);
@@ -538,10 +532,12 @@ decode_kernel(const AttnParams p, bool whole) {
         float wi[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int i = x ? __ffs(x) - 1 : head;
-          wi[k] = __shfl_sync(0xffffffffu, w, i);
+          const int j = x ? __ffs(x) - 1 : head;
+          const float* piece = (j & 1) || whole ? reinterpret_cast<const float*>(smem + (j >> 1) * (kSlots * kUnitBytes))
+                                                : p.ws + (int64_t)(block * kWarps + (j >> 1)) * piece_floats(NT);
+          wi[k] = __shfl_sync(0xffffffffu, w, j);
           if (!x) wi[k] = 0.f;
-          v[k] = *reinterpret_cast<const float2*>(piece_of(i) + n * kRowPad + ch);
+          v[k] = *reinterpret_cast<const float2*>(piece + n * kRowPad + ch);
           x &= x - 1;
         }
 #pragma unroll
@@ -554,14 +550,16 @@ decode_kernel(const AttnParams p, bool whole) {
         else { const __half2 hh = __floats2half2_rn(acc.x * inv, acc.y * inv); o = *reinterpret_cast<const uint32_t*>(&hh); }
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + out_row(p, Request{run.x, run.y, 0, 0}, run.z, n) + ch) = o;
       } else {
-        float* to = p.ws + ws_block_pieces<NT>(gridDim.x) + (int64_t)(2 * block + (began_before ? 0 : 1)) * piece_floats(NT);
-        *reinterpret_cast<float2*>(to + n * kRowPad + ch) = acc;
-        if (lane == 0) { to[8 * NT * kRowPad + n] = M; to[8 * NT * kRowPad + 8 * NT + n] = L; }      // (both halves write the same)
+        float* mine = to + (began_before ? 0 : piece_floats(NT));
+        *reinterpret_cast<float2*>(mine + n * kRowPad + ch) = acc;
+        if (lane == 0) { mine[8 * NT * kRowPad + n] = M; mine[8 * NT * kRowPad + 8 * NT + n] = L; }      // (both halves write the same)
       }
     }
-    item += 2 * rows;
-    if (began_before && ends && tid == kThreads - 1)
-      *todo_of<NT>(p) = Merge{run.x, run.y, run.z, Cuts(s_cut[1], blocks_of(s_cut[1], kWarps)).block_of(s_cut[0] - s_before), 1, {0, 0, 0}};
+    turn -= items;
+  }
+  if (!whole && tid == kThreads - 1) {
+    if (todo.go) todo.first = Cuts(s_cut[1], blocks_of(s_cut[1], kWarps)).block_of(s_cut[0] - s_before);
+    *todo_of<NT>(p) = todo;
   }
 }
 
