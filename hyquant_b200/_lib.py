@@ -94,6 +94,17 @@ class PeerExchangeArgs(C.Structure):
     ]
 
 
+class PageAdvanceArgs(C.Structure):
+    """Mirror of ``hq_page_advance_args``."""
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("R", C.c_int32), ("T", C.c_int32), ("page_size", C.c_int32), ("max_pages", C.c_int32),
+        ("free_cap", C.c_int32), ("kv_lens", C.c_void_p), ("held", C.c_void_p), ("add", C.c_void_p), ("keep", C.c_void_p),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("free_pages", C.c_void_p), ("free_count", C.c_void_p),
+        ("kv_lens_out", C.c_void_p), ("held_out", C.c_void_p), ("free_count_out", C.c_void_p),
+        ("cu_q", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
 class PagedAttentionArgs(C.Structure):
     """Mirror of ``hq_paged_attention_args``."""
     _fields_ = [
@@ -146,10 +157,10 @@ def _declare(lib):
     lib.hq_prefill_quant_v_fp8.argtypes = [vp, i64, i64, i64, i32, i32, i32, vp, vp, vp, vp]
     lib.hq_prefill_vertical_gather_v_fp8.argtypes = [vp, i32, i32, i32, i32, i32, vp, i64, i64, i64, vp, vp, vp]
     lib.hq_prefill_hybrid.argtypes = [C.POINTER(PrefillArgs), vp]
-    lib.hq_page_advance.argtypes = [vp, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.hq_page_advance.argtypes = [vp, vp]           # PageAdvanceArgs, and below PagedAttentionArgs: by reference, or as bytes
     lib.hq_paged_append.argtypes = [vp, vp, i32, i64, i64, i64, i64, i32, i32, vp, vp, i64, i32, vp]
     lib.hq_paged_read.argtypes = [vp, i64, i32, vp, i32, i32, i32, vp, vp, vp]
-    lib.hq_paged_attention_workspace_bytes.argtypes = [vp, C.POINTER(i64)]       # PagedAttentionArgs by reference, or its bytes
+    lib.hq_paged_attention_workspace_bytes.argtypes = [vp, C.POINTER(i64)]
     lib.hq_paged_attention.argtypes = [vp, vp]
     lib.hq_tc_peak.argtypes = [i32, i32, vp, C.POINTER(C.c_int), vp]
     lib.hq_peer_exchange_bytes.argtypes = [i32, i32, C.POINTER(i64)]

@@ -283,23 +283,26 @@ static unsigned row_grid(int64_t rows) {
 }  // namespace paged
 }  // namespace hq
 
-extern "C" int hq_page_advance(const int32_t* kv_lens, const int32_t* held, const int32_t* add, const int32_t* keep, int R,
-                               int32_t* page_table, int64_t table_stride, int max_pages, int32_t* free_pages, int free_cap,
-                               const int32_t* free_count, int page_size, int T, int32_t* kv_lens_out, int32_t* held_out,
-                               int32_t* free_count_out, int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* status, void* stream) {
+extern "C" int hq_page_advance(const hq_page_advance_args* a, void* stream) {
   using namespace hq;
   using namespace hq::paged;
-  HQ_REQUIRE(R >= 0 && T >= 0 && max_pages >= 0 && free_cap >= 0, HQ_ERR_INVALID, "hq_page_advance: negative size");
-  HQ_REQUIRE(R <= kAdvMostR, HQ_ERR_UNSUPPORTED, "hq_page_advance: %d requests, at most %d", R, kAdvMostR);
-  HQ_REQUIRE(page_size_ok(page_size), HQ_ERR_UNSUPPORTED, "hq_page_advance: page_size must be 16, 32, 64 or 128, got %d", page_size);
-  HQ_REQUIRE(free_count && free_count_out && cu_q && status && (T == 0 || (slots && positions)), HQ_ERR_INVALID, "hq_page_advance: null pointer");
-  HQ_REQUIRE(R == 0 || (kv_lens && held && add && kv_lens_out && held_out), HQ_ERR_INVALID, "hq_page_advance: null pointer");
-  HQ_REQUIRE((R == 0 || max_pages == 0 || page_table) && (free_cap == 0 || free_pages), HQ_ERR_INVALID, "hq_page_advance: null pointer");
-  HQ_REQUIRE((int64_t)R * max_pages <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_page_advance: %d requests of %d pages", R, max_pages);
-  HQ_REQUIRE(table_stride >= max_pages, HQ_ERR_INVALID, "hq_page_advance: table rows of %d pages overlap at stride %lld", max_pages, (long long)table_stride);
-  AdvanceParams p{kv_lens, held, add, keep, R, page_table, table_stride, max_pages, free_pages, free_cap, free_count, shift_of(page_size), T,
-                  kv_lens_out, held_out, free_count_out, cu_q, slots, positions, status};
-  const int smem = (5 * R + 3) * (int)sizeof(int);
+  HQ_REQUIRE(a != nullptr, HQ_ERR_INVALID, "hq_page_advance: null argument block");
+  HQ_REQUIRE(a->struct_bytes == (int)sizeof(hq_page_advance_args), HQ_ERR_INVALID, "hq_page_advance: struct_bytes %d, expected %d", a->struct_bytes,
+             (int)sizeof(hq_page_advance_args));
+  HQ_REQUIRE(a->R >= 0 && a->T >= 0 && a->max_pages >= 0 && a->free_cap >= 0, HQ_ERR_INVALID, "hq_page_advance: negative size");
+  HQ_REQUIRE(a->R <= kAdvMostR, HQ_ERR_UNSUPPORTED, "hq_page_advance: %d requests, at most %d", a->R, kAdvMostR);
+  HQ_REQUIRE(page_size_ok(a->page_size), HQ_ERR_UNSUPPORTED, "hq_page_advance: page_size must be 16, 32, 64 or 128, got %d", a->page_size);
+  HQ_REQUIRE(a->free_count && a->free_count_out && a->cu_q && a->status && (a->T == 0 || (a->slots && a->positions)), HQ_ERR_INVALID,
+             "hq_page_advance: null pointer");
+  HQ_REQUIRE(a->R == 0 || (a->kv_lens && a->held && a->add && a->kv_lens_out && a->held_out), HQ_ERR_INVALID, "hq_page_advance: null pointer");
+  HQ_REQUIRE((a->R == 0 || a->max_pages == 0 || a->page_table) && (a->free_cap == 0 || a->free_pages), HQ_ERR_INVALID, "hq_page_advance: null pointer");
+  HQ_REQUIRE((int64_t)a->R * a->max_pages <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_page_advance: %d requests of %d pages", a->R, a->max_pages);
+  HQ_REQUIRE(a->table_stride >= a->max_pages, HQ_ERR_INVALID, "hq_page_advance: table rows of %d pages overlap at stride %lld", a->max_pages,
+             (long long)a->table_stride);
+  const AdvanceParams p{a->kv_lens, a->held, a->add, a->keep, a->R, a->page_table, a->table_stride, a->max_pages, a->free_pages, a->free_cap,
+                        a->free_count, shift_of(a->page_size), a->T, a->kv_lens_out, a->held_out, a->free_count_out, a->cu_q, a->slots,
+                        a->positions, a->status};
+  const int smem = (5 * a->R + 3) * (int)sizeof(int);
   static thread_local int attr_dev = -1;
   int dev = 0;
   HQ_CUDA(cudaGetDevice(&dev));

@@ -23,7 +23,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import HyQuantError, PagedAttentionArgs
+from ._lib import HyQuantError, PageAdvanceArgs, PagedAttentionArgs
 
 BLOCK = 16                  # tokens of a block
 BLOCK_BYTES = 2112
@@ -32,6 +32,12 @@ STATUS = {1: "too few free pages", 2: "a request longer than its table row", 4: 
           8: "arguments that do not fit the state"}
 
 _I32, _I64 = torch.int32, torch.int64
+
+
+# Argument blocks as bytes: a block is read during the call and not kept, and packing one costs a fifth of filling a ctypes
+# structure.  The fields are those of PageAdvanceArgs and PagedAttentionArgs.
+_ADVANCE_BYTES, _ARGS_BYTES = C.sizeof(PageAdvanceArgs), C.sizeof(PagedAttentionArgs)
+_pack_advance, _pack_args = struct.Struct("@6i15q").pack, struct.Struct("@10ifi14q").pack
 
 
 class PageStep(NamedTuple):
@@ -47,9 +53,12 @@ class PageStep(NamedTuple):
     status: torch.Tensor
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)       # without the check for a first use
+
+
 def _call(fn, dev, *args) -> int:
     """One library call on the current stream of ``dev``, which need not be the current device."""
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _current_device():
         with torch.cuda.device(dev):
             return fn(*args, _lib.stream_ptr(dev))
     return fn(*args, _lib.stream_ptr(dev))
@@ -117,23 +126,24 @@ def page_advance(kv_lens: torch.Tensor, held: torch.Tensor, add: torch.Tensor, p
     if max_tokens < 0:
         raise ValueError(f"max_tokens must be >= 0, got {max_tokens}")
     lens_p, held_p, add_p = _vector(kv_lens, R, _I32, dev, "kv_lens"), _vector(held, R, _I32, dev, "held"), _vector(add, R, _I32, dev, "add")
-    keep_p = None if keep is None else _vector(keep, R, _I32, dev, "keep")
+    keep_p = 0 if keep is None else _vector(keep, R, _I32, dev, "keep")
     free_p, count_p = _vector(free_pages, -1, _I32, dev, "free_pages"), _vector(free_count, 1, _I32, dev, "free_count")
     table_p, stride, cols = _table(page_table, R, dev)
-    slots = torch.empty(max_tokens, dtype=_I64, device=dev)
+    slots = kv_lens.new_empty(max_tokens, dtype=_I64)
     if in_place:
-        ints = torch.empty(R + 2 + max_tokens, dtype=_I32, device=dev)
-        cu_q, positions, status = ints.split_with_sizes((R + 1, max_tokens, 1))
+        ints = kv_lens.new_empty(R + 2 + max_tokens)
+        cu_q, positions, status = ints.unsafe_split_with_sizes((R + 1, max_tokens, 1))
         lens2, held2, count2, lens2_p, held2_p, count2_p = kv_lens, held, free_count, lens_p, held_p, count_p
         base = ints.data_ptr()
     else:
-        ints = torch.empty(3 * R + 3 + max_tokens, dtype=_I32, device=dev)
-        cu_q, positions, status, lens2, held2, count2 = ints.split_with_sizes((R + 1, max_tokens, 1, R, R, 1))
+        ints = kv_lens.new_empty(3 * R + 3 + max_tokens)
+        cu_q, positions, status, lens2, held2, count2 = ints.unsafe_split_with_sizes((R + 1, max_tokens, 1, R, R, 1))
         base = ints.data_ptr()
         lens2_p = base + 4 * (R + 2 + max_tokens)
         held2_p, count2_p = lens2_p + 4 * R, lens2_p + 8 * R
-    rc = _call(_lib.lib().hq_page_advance, dev, lens_p, held_p, add_p, keep_p, R, table_p, stride, cols, free_p, free_pages.numel(), count_p,
-               page_size, max_tokens, lens2_p, held2_p, count2_p, base, slots.data_ptr(), base + 4 * (R + 1), base + 4 * (R + 1 + max_tokens))
+    rc = _call(_lib.lib().hq_page_advance, dev, _pack_advance(
+        _ADVANCE_BYTES, R, max_tokens, page_size, cols, free_pages.numel(), lens_p, held_p, add_p, keep_p, table_p, stride, free_p, count_p,
+        lens2_p, held2_p, count2_p, base, slots.data_ptr(), base + 4 * (R + 1), base + 4 * (R + 1 + max_tokens)))
     if rc != 0:
         _lib.check(rc, "hq_page_advance")
     return PageStep(lens2, held2, count2, cu_q, slots, positions, status)
@@ -171,11 +181,8 @@ def paged_read(pages: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = to
     code = _lib.dtype_code(dtype)
     T, dev = slots.numel(), pages.device
     slots_p = _vector(slots, T, _I64, dev, "slots")
-    rows = torch.empty((2, T, H, 128), dtype=dtype, device=dev)
-    k, v = rows.unbind(0)
-    k_p = rows.data_ptr()
-    rc = _call(_lib.lib().hq_paged_read, dev, pages.data_ptr(), num_pages, page_size, slots_p, T, H, code, k_p,
-               k_p + T * H * 128 * rows.element_size())
+    k, v = pages.new_empty(T, H, 128, dtype=dtype), pages.new_empty(T, H, 128, dtype=dtype)
+    rc = _call(_lib.lib().hq_paged_read, dev, pages.data_ptr(), num_pages, page_size, slots_p, T, H, code, k.data_ptr(), v.data_ptr())
     if rc != 0:
         _lib.check(rc, "hq_paged_read")
     return k, v
@@ -214,7 +221,7 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
             raise ValueError(f"max_q_len must be >= 1, got {max_q_len}")
     q, q_p, q_st, q_sh = _rows(q)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = q.new_empty(T, H_Q, 128)
         o_st, o_sh = H_Q * 128, 128
     else:
         if out.shape != shape or out.dtype is not dtype or out.device != dev or out.stride(2) != 1:
@@ -224,7 +231,7 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
          q_p, q_st, q_sh, pages.data_ptr(), table_p, stride, lens_p, cu_p, out.data_ptr(), o_st, o_sh, 0, 0]
     need = _workspace_bytes(a, dev)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = pages.new_empty(need)
         a[24], a[25] = ws.data_ptr(), need
     rc = _call(_lib.lib().hq_paged_attention, dev, _pack_args(*a))
     if rc != 0:
@@ -232,10 +239,6 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
     return out
 
 
-# hq_paged_attention_args as bytes: a block is read during the call and not kept, and packing one costs a fifth of filling a
-# ctypes structure.  The fields are those of PagedAttentionArgs.
-_ARGS_BYTES = C.sizeof(PagedAttentionArgs)
-_pack_args = struct.Struct("@10ifi14q").pack
 _workspace: dict = {}
 
 

@@ -468,10 +468,16 @@ int hq_prefill_vertical_gather_v_fp8(const int32_t* vidx_asc, int B, int H_Q, in
  *   status int32 [1]: 0, or why nothing was changed (cu_q is then 0 throughout, slots -1): bit 0 too few free pages, bit 1 a
  *   request longer than max_pages, bit 2 more than T new tokens, bit 3 arguments that do not fit (keep > kv_lens, a negative
  *   number, held outside [ceil(kv_lens / page_size), max_pages], a full stack).  The word is written by every call. */
-int hq_page_advance(const int32_t* kv_lens, const int32_t* held, const int32_t* add, const int32_t* keep, int R,
-                    int32_t* page_table, int64_t table_stride, int max_pages, int32_t* free_pages, int free_cap,
-                    const int32_t* free_count, int page_size, int T, int32_t* kv_lens_out, int32_t* held_out,
-                    int32_t* free_count_out, int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* status, void* stream);
+typedef struct hq_page_advance_args {
+  int32_t struct_bytes;
+  int32_t R, T, page_size, max_pages, free_cap;
+  const int32_t* kv_lens; const int32_t* held; const int32_t* add; const int32_t* keep;
+  int32_t* page_table; int64_t table_stride;
+  int32_t* free_pages; const int32_t* free_count;
+  int32_t* kv_lens_out; int32_t* held_out; int32_t* free_count_out;
+  int32_t* cu_q; int64_t* slots; int32_t* positions; int32_t* status;
+} hq_page_advance_args;
+int hq_page_advance(const hq_page_advance_args* args, void* stream);
 
 /* T rows of K and V, [T, H_KV, 128] in dtype (bf16, fp16, fp32; rows 16-byte aligned, strides in elements, multiples of 8),
  * quantised into their slots.  A slot outside [0, num_pages * page_size) is skipped (padding is -1); the slots of a call are

@@ -57,16 +57,21 @@ def test_attention_null_block_and_nothing_to_do():
 
 
 def advance(**fields):
-    a = dict(kv_lens=FAKE, held=FAKE, add=FAKE, keep=None, R=3, table=FAKE, stride=10, max_pages=10, free=FAKE, cap=9, count=FAKE, page=16, T=4,
-             lens2=FAKE, held2=FAKE, count2=FAKE, cu=FAKE, slots=FAKE, pos=FAKE, status=FAKE)
-    a.update(fields)
-    return _lib.lib().hq_page_advance(*a.values(), None)
+    a = _lib.PageAdvanceArgs()
+    a.struct_bytes, a.R, a.T, a.page_size, a.max_pages, a.free_cap, a.table_stride = C.sizeof(a), 3, 4, 16, 10, 9, 10
+    for name, kind in a._fields_:
+        if kind is C.c_void_p and name != "keep":
+            setattr(a, name, FAKE)
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return _lib.lib().hq_page_advance(C.byref(a), None)
 
 
 @pytest.mark.parametrize("fields,code", [
-    (dict(R=-1), -1), (dict(T=-1), -1), (dict(cap=-1), -1), (dict(max_pages=-1), -1), (dict(R=8193), -2), (dict(page=8), -2), (dict(page=0), -2),
-    (dict(kv_lens=None), -1), (dict(add=None), -1), (dict(slots=None), -1), (dict(cu=None), -1), (dict(status=None), -1), (dict(table=None), -1),
-    (dict(free=None), -1), (dict(stride=9), -1), (dict(R=8192, max_pages=1 << 20, stride=1 << 20), -2)])
+    (dict(struct_bytes=100), -1), (dict(R=-1), -1), (dict(T=-1), -1), (dict(free_cap=-1), -1), (dict(max_pages=-1), -1), (dict(R=8193), -2),
+    (dict(page_size=8), -2), (dict(page_size=0), -2), (dict(kv_lens=None), -1), (dict(add=None), -1), (dict(slots=None), -1), (dict(cu_q=None), -1),
+    (dict(status=None), -1), (dict(page_table=None), -1), (dict(free_pages=None), -1), (dict(free_count_out=None), -1), (dict(table_stride=9), -1),
+    (dict(R=8192, max_pages=1 << 20, table_stride=1 << 20), -2)])
 def test_advance_refusals(fields, code):
     assert advance(**fields) == code
 
@@ -120,6 +125,15 @@ def test_python_refusals():
     cache.check()                                                           # no step yet: nothing to report
     with pytest.raises(hq.HyQuantError):
         cache.append(0, x, x)
+
+
+def test_argument_blocks_as_bytes():
+    assert _lib.lib().hq_page_advance(None, None) == -1
+    for struct_, pack, ints in ((_lib.PageAdvanceArgs, paged_kv._pack_advance, 21), (_lib.PagedAttentionArgs, paged_kv._pack_args, 26)):
+        values = [0.5 if kind is C.c_float else i + 1 for i, (_, kind) in enumerate(struct_._fields_)]
+        assert len(values) == ints
+        a = struct_.from_buffer_copy(pack(*values))
+        assert [getattr(a, name) for name, _ in struct_._fields_] == values
 
 
 def test_format_constants():
