@@ -183,9 +183,6 @@ __device__ __forceinline__ uint4 values8(const Unpack& k, uint32_t w, __half2 s)
                     u32(__hmul2(__hfma2(h2(lop3_and_xor(w8, k.hi, k.hi8)), c16th, c72), s)));
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void halves_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the eight softmax warps
 
 template <bool kBf16>
@@ -376,53 +373,66 @@ tile_kernel(const AttnParams p, int piece_rows) {
     int ks = 0;
     uint32_t kpar = 1u;                          // empty barriers: the first round passes
     bool ok = true;
-    // K and V of a tile in turn.  The values are in registers before their place is free; a part's stores are made visible to the
-    // tensor core behind the arithmetic of the next part, when they are long done.
+    // K and V of a tile in turn.  A part's codes are read while the part before is worked on, its values are in registers before their
+    // place is free, and its stores are made visible to the tensor core behind the arithmetic of the next part, when they are long
+    // done.
+    struct Codes { uint2 c[2][2]; __half2 s[2]; };
+    auto read = [&](int stage, int kv) {
+      const uint8_t* block = smem + TileSmem::Codes + stage * kCodeBytes + w * kBlockBytes;      // keys 16 w .. + 15
+      const int info = key_rows[stage], rows = ((info >> (16 + w)) & 1) ? 0 : (info & 0xFFFF) - kTok * w;
+      Codes x;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {              // keys 16 w + 8 g .. + 7
+        const uint8_t* c = block + kv * kVOff + g * 512 + lane * 16;
+        x.c[g][0] = *reinterpret_cast<const uint2*>(c + 4 * turn);
+        x.c[g][1] = *reinterpret_cast<const uint2*>(c + 8 - 4 * turn);
+        const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * g + rowl));
+        // keys that are not there: zeros, whatever lies here
+        x.s[g] = __float2half2_rn(8 * g + rowl < rows ? __uint_as_float((uint32_t)sb << 16) : 0.f);
+      }
+      return x;
+    };
     uint64_t* due = nullptr;
     auto hand_over = [&]() {
       if (due == nullptr) return;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(due);
+      due = nullptr;
     };
+    auto part = [&](const Codes& x, int kv) {
+      uint4 val[2][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        val[g][0] = values8(uk, x.c[g][0].x, x.s[g]); val[g][1] = values8(uk, x.c[g][0].y, x.s[g]);
+        val[g][2] = values8(uk, x.c[g][1].x, x.s[g]); val[g][3] = values8(uk, x.c[g][1].y, x.s[g]);
+      }
+      hand_over();
+      ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
+      if (!ok) return;
+      uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384 + (quarter >> 1) * 8192 + (kTok * w + rowl) * 128;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + g * 1024 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
+      due = (kv ? v_full : k_full) + ks;
+    };
+    Codes kc;
+    bool have = false;                           // kc holds the next tile's K
 #pragma unroll 1
     for (int tile = 0; ok && tile < n_all; ++tile) {
-      const int cs = tile % kAhead;
-      const uint32_t cpar = (uint32_t)(tile / kAhead) & 1u;
-      if (!__all_sync(0xffffffffu, mbar_test_wait(c_full + cs, cpar))) {      // nothing to do meanwhile
+      const int cs = tile % kAhead, next = (tile + 1) % kAhead;
+      if (!have) {                               // nothing to do meanwhile
         hand_over();
-        due = nullptr;
-        ok = wait_warp(c_full + cs, cpar, abort_flag);
+        ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
         if (!ok) break;
+        kc = read(cs, 0);
       }
-      const uint8_t* block = smem + TileSmem::Codes + cs * kCodeBytes + w * kBlockBytes;       // keys 16 w .. + 15
-      const int info = key_rows[cs], rows = ((info >> (16 + w)) & 1) ? 0 : (info & 0xFFFF) - kTok * w;
-      uint8_t* to = smem + TileSmem::K + ks * 16384 + (quarter >> 1) * 8192 + (kTok * w + rowl) * 128;
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        uint4 val[2][4];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {            // keys 16 w + 8 g .. + 7
-          const uint8_t* c = block + kv * kVOff + g * 512 + lane * 16;
-          const uint2 c0 = *reinterpret_cast<const uint2*>(c + 4 * turn), c1 = *reinterpret_cast<const uint2*>(c + 8 - 4 * turn);
-          const uint16_t sb = *reinterpret_cast<const uint16_t*>(block + (kv ? kVsOff : kKsOff) + 2 * (8 * g + rowl));
-          // keys that are not there: zeros, whatever lies here
-          const __half2 s = __float2half2_rn(8 * g + rowl < rows ? __uint_as_float((uint32_t)sb << 16) : 0.f);
-          val[g][0] = values8(uk, c0.x, s); val[g][1] = values8(uk, c0.y, s);
-          val[g][2] = values8(uk, c1.x, s); val[g][3] = values8(uk, c1.y, s);
-        }
-        hand_over();
-        ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
-        due = nullptr;
-        if (ok) {
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(to + kv * (TileSmem::V - TileSmem::K) + g * 1024 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
-          due = (kv ? v_full : k_full) + ks;
-        }
-      }
+      const Codes vc = read(cs, 1);
+      part(kc, 0);
+      have = tile + 1 < n_all && __all_sync(0xffffffffu, mbar_test_wait(c_full + next, (uint32_t)((tile + 1) / kAhead) & 1u));
+      if (have) kc = read(next, 0);
+      part(vc, 1);
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(c_empty + cs);
       if (++ks == kStages) { ks = 0; kpar ^= 1u; }
@@ -441,21 +451,27 @@ tile_kernel(const AttnParams p, int piece_rows) {
       const int row0 = pc.it.qt * kRows + (split ? 0 : 128 * half), rows = min(128, q.nq * p.G - row0);
       const int n_all = pc.t1 - pc.t0, first = split ? half : 0, step = split ? 2 : 1, n = (n_all - first + step - 1) / step;
       const int row = row0 + r, i = token_of(p, row);
+      const bool live = wq * 32 < rows;          // of the warp: one without rows only keeps the others' count
       float m = -INFINITY, l = 0.f;
-      if (n > 0 && ok) {
+      if (n > 0 && ok && !live) {
+        tc::mbar_arrive(q_full + half);
+#pragma unroll 1
+        for (int t = 0; t < n && ok; ++t, ++tile) {
+          ok = wait_warp(s_full + 2 * half + (tile & 1u), (tile >> 1) & 1u, abort_flag);
+          tc::mbar_arrive(p_ready + 2 * half + (tile & 1u));
+        }
+      } else if (n > 0 && ok) {
         // queries: scaled by a power of two of the row so that fp16 holds them exactly, into the operand tile
         uint8_t* mine = sQ + r * 128;
         const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + (r < rows ? i : 0)) * p.q_st +
                                (int64_t)(pc.it.h * p.G + (r < rows ? row - i * p.G : 0)) * p.q_sh;
+        uint4 raw[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) cp_async16(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4), from + 8 * c, r < rows);
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        for (int c = 0; c < 16; ++c) raw[c] = r < rows ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0u, 0u, 0u, 0u);
         uint32_t top2 = 0u;                      // magnitudes of 16-bit numbers order like integers
-#pragma unroll 4
-        for (int c = 0; c < 16; ++c) {
-          const uint4 u = *reinterpret_cast<const uint4*>(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
-          top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, u.x & 0x7FFF7FFFu), u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
-        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          top2 = __vmaxu2(__vmaxu2(__vmaxu2(top2, raw[c].x & 0x7FFF7FFFu), raw[c].y & 0x7FFF7FFFu), __vmaxu2(raw[c].z & 0x7FFF7FFFu, raw[c].w & 0x7FFF7FFFu));
         auto value = [&](uint32_t u, int hi) {
           if (kBf16) return __uint_as_float(hi ? u & 0xFFFF0000u : u << 16);
           return __half2float(__ushort_as_half((unsigned short)(hi ? u >> 16 : u & 0xFFFFu)));
@@ -463,17 +479,18 @@ tile_kernel(const AttnParams p, int piece_rows) {
         const float top = value(max(top2 & 0xFFFFu, top2 >> 16), 0);
         const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 255 ? 0 : 140 - max(ex, 14);       // largest magnitude to [2^13, 2^14)
         const float scale = __uint_as_float((uint32_t)(127 + up) << 23), f = p.sml * __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll 2
+        const float2 scale2 = make_float2(scale, scale);
+#pragma unroll
         for (int c = 0; c < 16; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
-          const uint32_t u[4] = {at->x, at->y, at->z, at->w};
+          const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
           uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {          // channels k and k + 4 of the eight
-            const __half2 hh = __floats2half2_rn(value(u[k >> 1], k & 1) * scale, value(u[2 + (k >> 1)], k & 1) * scale);
+            const float2 x = fmul2(make_float2(value(u[k >> 1], k & 1), value(u[2 + (k >> 1)], k & 1)), scale2);
+            const __half2 hh = __floats2half2_rn(x.x, x.y);
             o[k] = *reinterpret_cast<const uint32_t*>(&hh);
           }
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(mine + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         tc::mbar_arrive(q_full + half);
@@ -547,7 +564,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
         if (l != l) { wa = l; wb = l; }
       }
       tc::fence_after_sync();
-      {
+      if (live) {
         // O leaves through the rows' own part of the query tile, 32 columns at a time, so that a store writes whole sectors.  Halves
         // that share their rows take two of the four parts each.
         const bool whole = !pc.began && pc.ends;
