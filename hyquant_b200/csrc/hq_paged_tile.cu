@@ -32,7 +32,9 @@ constexpr int kIssue = 12, kFetch = 14;          // first issuing warp; the fetc
 constexpr int kStages = 3;                       // K tiles, and V tiles, in shared memory
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
-constexpr int kItemCost = 4;                     // positions that a query tile costs beside its key tiles
+// positions, of about 200 clocks each: a key tile that both halves work on, one that a half has to itself (KEEP clocks against 1950), and
+// what a query tile costs beside them (queries 3500, first reference and masks 2600 each, results 5000)
+constexpr int kFullCost = 10, kSplitCost = 8, kItemCost = 60;
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
 constexpr uint32_t kTPolls = 400000u;
 
@@ -44,18 +46,22 @@ static_assert(TileSmem::Bar % 16 == 0 && TileSmem::Total + 1024 <= 227 * 1024, "
 
 struct TileMerge { int q0, rows, h, qt, first, go, unused[2]; };
 
-// A query tile and where in it a block's part begins.  A key tile costs one position, or two where both halves work on it.
+// A query tile and where in it a block's part begins
 struct Item {
-  int r, h, qt, n_qt, u, tiles, cost;
+  int r, h, qt, n_qt, u, tiles;
+  bool split;                                    // every other key tile to each half
   Request q;
-  __device__ __forceinline__ int positions() const { return tiles * cost + kItemCost; }
+  __device__ __forceinline__ int positions() const { return tiles * (split ? kSplitCost : kFullCost) + kItemCost; }
+  __device__ __forceinline__ int tiles_to(int u) const {       // key tiles that begin before position u
+    return min(tiles, split ? (u + kSplitCost - 1) / kSplitCost : (u + kFullCost - 1) / kFullCost);
+  }
 };
 __device__ __forceinline__ int query_tiles(const AttnParams& p, const Request& q) { return (q.nq * p.G + kRows - 1) / kRows; }
 __device__ __forceinline__ void size_item(const AttnParams& p, Item& x) {
   const int rows = x.q.nq * p.G, last = min(rows, (x.qt + 1) * kRows) - 1;
   const int keys = min(x.q.len, x.q.past + 1 + token_of(p, last));
   x.tiles = keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
-  x.cost = rows - x.qt * kRows > 128 ? 2 : 1;
+  x.split = rows - x.qt * kRows <= 128;
 }
 __device__ __forceinline__ void next_item(const AttnParams& p, Item& x) {
   x.u = 0;
@@ -79,9 +85,8 @@ struct Pieces {
   bool began, ends;                              // earlier, in another block; here
   __device__ __forceinline__ bool take(const AttnParams& p) {
     while (left > 0) {
-      const int to = min(it.tiles * it.cost, it.u + left);
-      t0 = (it.u + it.cost - 1) / it.cost;
-      t1 = (to + it.cost - 1) / it.cost;
+      t0 = it.tiles_to(it.u);
+      t1 = it.tiles_to(it.u + left);
       began = it.u > 0;
       ends = t1 == it.tiles;
       if (t1 > t0 || (it.tiles == 0 && it.u == 0)) return true;
@@ -93,7 +98,7 @@ struct Pieces {
     left -= it.positions() - it.u;
     if (left > 0) next_item(p, it);
   }
-  __device__ __forceinline__ bool split() const { return it.cost == 1; }      // every other key tile to each half
+  __device__ __forceinline__ bool split() const { return it.split; }
 };
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
@@ -236,7 +241,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const Cuts cuts(prefix.total, max(1, min((int)gridDim.x, prefix.total / (kItemCost + 2))));
+  const Cuts cuts(prefix.total, max(1, min((int)gridDim.x, prefix.total / (kItemCost + kFullCost))));
   const int block = blockIdx.x;
   const int b0 = cuts.begin(block);
   const int64_t piece_floats = (int64_t)piece_rows * 130;
@@ -376,6 +381,9 @@ tile_kernel(const AttnParams p, int piece_rows) {
     // K and V of a tile in turn.  A part's codes are read while the part before is worked on, its values are in registers before their
     // place is free, and its stores are made visible to the tensor core behind the arithmetic of the next part, when they are long
     // done.
+    uint32_t place[4];                           // of a row's four chunks under the 128-byte swizzle
+#pragma unroll
+    for (int k = 0; k < 4; ++k) place[k] = (quarter >> 1) * 8192 + (kTok * w + rowl) * 128 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4);
     struct Codes { uint2 c[2][2]; __half2 s[2]; };
     auto read = [&](int stage, int kv) {
       const uint8_t* block = smem + TileSmem::Codes + stage * kCodeBytes + w * kBlockBytes;      // keys 16 w .. + 15
@@ -410,11 +418,11 @@ tile_kernel(const AttnParams p, int piece_rows) {
       hand_over();
       ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
       if (!ok) return;
-      uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384 + (quarter >> 1) * 8192 + (kTok * w + rowl) * 128;
+      uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384;
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + g * 1024 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4)) = val[g][k];
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + place[k] + g * 1024) = val[g][k];
       due = (kv ? v_full : k_full) + ks;
     };
     Codes kc;
