@@ -29,7 +29,7 @@ namespace paged {
 
 constexpr int kTileThreads = 480, kRows = 256, kKeys = 64;
 constexpr int kIssue = 12, kFetch = 14;          // first issuing warp; the fetching one
-constexpr int kStages = 3;                       // K tiles, and V tiles, in shared memory
+constexpr int kKStages = 3, kVStages = 4;        // K tiles and V tiles in shared memory
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
 // positions, of about 200 clocks each: a key tile that both halves work on, one that a half has to itself (KEEP clocks against 1950), and
@@ -39,7 +39,7 @@ constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9);
 constexpr uint32_t kTPolls = 400000u;
 
 struct TileSmem {
-  static constexpr int Q = 0, K = 65536, V = K + kStages * 16384, Codes = V + kStages * 16384, Bar = Codes + kAhead * kCodeBytes,
+  static constexpr int Q = 0, K = 65536, V = K + kKStages * 16384, Codes = V + kVStages * 16384, Bar = Codes + kAhead * kCodeBytes,
                        Rows = Bar + 320, Bad = Rows + 4 * kAhead, Total = Bad + 16;
 };
 static_assert(TileSmem::Bar % 16 == 0 && TileSmem::Total + 1024 <= 227 * 1024, "shared memory");
@@ -198,10 +198,10 @@ tile_kernel(const AttnParams p, int piece_rows) {
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + TileSmem::Bar);
   uint64_t* q_full = bars;                       // [half]
   uint64_t* k_full = bars + 2;                   // [stage]
-  uint64_t* k_empty = k_full + kStages;
-  uint64_t* v_full = k_empty + kStages;
-  uint64_t* v_empty = v_full + kStages;
-  uint64_t* c_full = v_empty + kStages;          // [kAhead]
+  uint64_t* k_empty = k_full + kKStages;
+  uint64_t* v_full = k_empty + kKStages;
+  uint64_t* v_empty = v_full + kVStages;
+  uint64_t* c_full = v_empty + kVStages;          // [kAhead]
   uint64_t* c_empty = c_full + kAhead;
   uint64_t* s_full = c_empty + kAhead;           // [half][2]
   uint64_t* p_ready = s_full + 4;
@@ -216,7 +216,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
   if (warp == kIssue) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 128); mbar_init(drained + i, 1); }
-      for (int i = 0; i < kStages; ++i) { mbar_init(k_full + i, 4); mbar_init(k_empty + i, 2); mbar_init(v_full + i, 4); mbar_init(v_empty + i, 2); }
+      for (int i = 0; i < kKStages; ++i) { mbar_init(k_full + i, 4); mbar_init(k_empty + i, 2); }
+      for (int i = 0; i < kVStages; ++i) { mbar_init(v_full + i, 4); mbar_init(v_empty + i, 2); }
       for (int i = 0; i < kAhead; ++i) { mbar_init(c_full + i, 1); mbar_init(c_empty + i, 4); }
       for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_ready + i, 128); mbar_init(pv_done + i, 1); }
       *abort_flag = 0;
@@ -320,8 +321,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
         // a slot goes back when both halves have arrived; a half that has a tile to itself arrives twice
         auto hand_back = [&](uint64_t* bar) { tc::mma_commit(bar); if (step == 2) tc::mma_commit(bar); };
         auto qk = [&]() {
-          const uint32_t at = ring + (uint32_t)(first + step * tq), ks = at % kStages, slot = (tile + (uint32_t)tq) & 1u;
-          ok = ok && wait_warp(k_full + ks, (at / kStages) & 1u, abort_flag);
+          const uint32_t at = ring + (uint32_t)(first + step * tq), ks = at % kKStages, slot = (tile + (uint32_t)tq) & 1u;
+          ok = ok && wait_warp(k_full + ks, (at / kKStages) & 1u, abort_flag);
           if (!ok) return;
           tc::fence_after_sync();
           if (tc::elect_one()) {
@@ -338,8 +339,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
         qk();
         if (n > 1) qk();
         for (int t = 0; ok && t < n; ++t) {
-          const uint32_t at = ring + (uint32_t)(first + step * t), vs = at % kStages, slot = (tile + (uint32_t)t) & 1u;
-          ok = wait_warp(v_full + vs, (at / kStages) & 1u, abort_flag) &&
+          const uint32_t at = ring + (uint32_t)(first + step * t), vs = at % kVStages, slot = (tile + (uint32_t)t) & 1u;
+          ok = wait_warp(v_full + vs, (at / kVStages) & 1u, abort_flag) &&
                wait_warp(p_ready + 2 * half + slot, ((tile + (uint32_t)t) >> 1) & 1u, abort_flag);
           if (!ok) break;
           tc::fence_after_sync();
@@ -375,12 +376,9 @@ tile_kernel(const AttnParams p, int piece_rows) {
     asm volatile("mov.b32 %0, 0x64806480;" : "=r"(uk.hi8));
     int n_all = 0;
     while (pc.take(p)) { n_all += pc.t1 - pc.t0; pc.done(p); }
-    int ks = 0;
-    uint32_t kpar = 1u;                          // empty barriers: the first round passes
+    int ks = 0, vs = 0;
+    uint32_t kpar = 1u, vpar = 1u;               // empty barriers: the first round passes
     bool ok = true;
-    // K and V of a tile in turn.  A part's codes are read while the part before is worked on, its values are in registers before their
-    // place is free, and its stores are made visible to the tensor core behind the arithmetic of the next part, when they are long
-    // done.
     uint32_t place[4];                           // of a row's four chunks under the 128-byte swizzle
 #pragma unroll
     for (int k = 0; k < 4; ++k) place[k] = (quarter >> 1) * 8192 + (kTok * w + rowl) * 128 + (((((quarter & 1) << 2) + (k ^ turn)) ^ rowl) << 4);
@@ -400,52 +398,46 @@ tile_kernel(const AttnParams p, int piece_rows) {
       }
       return x;
     };
-    uint64_t* due = nullptr;
-    auto hand_over = [&]() {
-      if (due == nullptr) return;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(due);
-      due = nullptr;
-    };
-    auto part = [&](const Codes& x, int kv) {
-      uint4 val[2][4];
+    auto values = [&](const Codes& x, uint4 (&val)[2][4]) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         val[g][0] = values8(uk, x.c[g][0].x, x.s[g]); val[g][1] = values8(uk, x.c[g][0].y, x.s[g]);
         val[g][2] = values8(uk, x.c[g][1].x, x.s[g]); val[g][3] = values8(uk, x.c[g][1].y, x.s[g]);
       }
-      hand_over();
-      ok = ok && wait_warp((kv ? v_empty : k_empty) + ks, kpar, abort_flag);
-      if (!ok) return;
-      uint8_t* to = smem + (kv ? TileSmem::V : TileSmem::K) + ks * 16384;
+    };
+    // K and V of a tile together: a question to a barrier costs some 100 clocks, a fence as much, and with K and V one after the other
+    // they were 600 of a tile's 1500.  V has a slot more than K, so that K does not wait for a P V that is still to come.  The
+    // values are in registers before their places are free.
+#pragma unroll 1
+    for (int tile = 0; tile < n_all; ++tile) {
+      const int cs = tile % kAhead;
+      ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
+      if (!ok) break;
+      uint4 kval[2][4], vval[2][4];
+      {
+        const Codes kc = read(cs, 0), vc = read(cs, 1);
+        values(kc, kval);
+        values(vc, vval);
+      }
+      if (!__all_sync(0xffffffffu, mbar_test_wait(k_empty + ks, kpar) & mbar_test_wait(v_empty + vs, vpar))) {
+        ok = wait_warp(k_empty + ks, kpar, abort_flag) && wait_warp(v_empty + vs, vpar, abort_flag);
+        if (!ok) break;
+      }
+      uint8_t* k_to = smem + TileSmem::K + ks * 16384;
+      uint8_t* v_to = smem + TileSmem::V + vs * 16384;
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + place[k] + g * 1024) = val[g][k];
-      due = (kv ? v_full : k_full) + ks;
-    };
-    Codes kc;
-    bool have = false;                           // kc holds the next tile's K
-#pragma unroll 1
-    for (int tile = 0; ok && tile < n_all; ++tile) {
-      const int cs = tile % kAhead, next = (tile + 1) % kAhead;
-      if (!have) {                               // nothing to do meanwhile
-        hand_over();
-        ok = wait_warp(c_full + cs, (uint32_t)(tile / kAhead) & 1u, abort_flag);
-        if (!ok) break;
-        kc = read(cs, 0);
-      }
-      const Codes vc = read(cs, 1);
-      part(kc, 0);
-      have = tile + 1 < n_all && __all_sync(0xffffffffu, mbar_test_wait(c_full + next, (uint32_t)((tile + 1) / kAhead) & 1u));
-      if (have) kc = read(next, 0);
-      part(vc, 1);
+        for (int k = 0; k < 4; ++k) {
+          *reinterpret_cast<uint4*>(k_to + place[k] + g * 1024) = kval[g][k];
+          *reinterpret_cast<uint4*>(v_to + place[k] + g * 1024) = vval[g][k];
+        }
+      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(c_empty + cs);
-      if (++ks == kStages) { ks = 0; kpar ^= 1u; }
+      if (lane == 0) { tc::mbar_arrive(k_full + ks); tc::mbar_arrive(v_full + vs); tc::mbar_arrive(c_empty + cs); }
+      if (++ks == kKStages) { ks = 0; kpar ^= 1u; }
+      if (++vs == kVStages) { vs = 0; vpar ^= 1u; }
     }
-    hand_over();
   } else {
     // ------------------------------------------------------------ softmax: a thread per row
     const int half = warp >> 2, wq = warp & 3, r = wq * 32 + lane;
