@@ -100,6 +100,29 @@ __device__ __forceinline__ float quant_row(const float (&v)[16], uint32_t (&code
   return s;
 }
 
+// Eight codes -> eight values in the order 0 4 1 5 2 6 3 7.  Nibbles in the low mantissa bits are 1024 + 8 + code, or 1024 + 16 (8 + code)
+// four bits up; the code is taken out exactly and its product with the scale is an fp16 number.
+struct Unpack { uint32_t lo, hi, lo8, hi8; };
+__device__ __forceinline__ uint4 values8(const Unpack& k, uint32_t w, __half2 s) {
+  const uint32_t w8 = w >> 8;
+  auto h2 = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
+  auto u32 = [](__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); };
+  const __half2 c1032 = h2(0xE408E408u), c16th = h2(0x2C002C00u), c72 = h2(0xD480D480u);       // -1032, 1 / 16, -72
+  return make_uint4(u32(__hmul2(__hadd2(h2(lop3_and_xor(w, k.lo, k.lo8)), c1032), s)),
+                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w, k.hi, k.hi8)), c16th, c72), s)),
+                    u32(__hmul2(__hadd2(h2(lop3_and_xor(w8, k.lo, k.lo8)), c1032), s)),
+                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w8, k.hi, k.hi8)), c16th, c72), s)));
+}
+// the masks, kept in registers: as constants they are loaded again beside every use
+__device__ __forceinline__ Unpack unpack_masks() {
+  Unpack k;
+  asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(k.lo));
+  asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(k.hi));
+  asm volatile("mov.b32 %0, 0x64086408;" : "=r"(k.lo8));
+  asm volatile("mov.b32 %0, 0x64806480;" : "=r"(k.hi8));
+  return k;
+}
+
 // Request r of a call: its first row of q, its rows, its cached tokens, and those before its first new one.  Starts outside q and
 // lengths past the table are cut, so that no address is formed from them.
 struct Request { int q0, nq, len, past; };

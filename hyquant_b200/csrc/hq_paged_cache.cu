@@ -19,9 +19,12 @@ struct AdvanceParams {
 };
 constexpr int kAdvThreads = 1024;
 constexpr int kAdvMostR = 8192;
+// From 12288 rows of slots on, eight blocks: 8192 rows took 6.2 us with one and 6.7 with eight, 16384 8.9 and 7.5, 65536 21.0 and
+// 8.7 (500 requests; four blocks 10.5).  Below, the cluster's launch and its barriers cost more than they save: 512 rows 4.2 and 5.7.
+constexpr int kAdvBlocks = 8, kAdvMany = 12288;
 
 __device__ __forceinline__ void adv_sync(bool cluster) {
-  if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (cluster) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
   else __syncthreads();
 }
 // the largest r in [0, R) with a[r] <= x, for a[0] = 0 and x >= 0
@@ -57,7 +60,7 @@ advance_kernel(const AdvanceParams p, int blocks) {
     const int kv = p.kv_lens[r], held = p.held[r], add = p.add[r], keep = p.keep ? p.keep[r] : kv;
     const long long target = (long long)keep + add;
     if (kv < 0 || add < 0 || keep < 0 || keep > kv || held < 0 || held > p.max_pages || (((long long)kv + page - 1) >> p.page_shift) > held) bad |= 8;
-    if (((target + page - 1) >> p.page_shift) > p.max_pages) bad |= 2;
+    if (((target + page - 1) >> p.page_shift) > p.max_pages || target > 0x7FFFFFFF) bad |= 2;
     int more = 0, back = 0;
     if (!bad) {
       const int need = (int)((target + page - 1) >> p.page_shift);
@@ -169,26 +172,28 @@ advance_kernel(const AdvanceParams p, int blocks) {
 }
 
 // ---------------------------------------------------------------------------------------------- rows in, rows out
-// HBM-bound: 256 bytes a 16-bit row read, 66 written.  Eight lanes take the K row and the V row of one token and head, so that two
-// rows' loads are in flight per lane; a row is one 256-byte line in and one 64-byte line out.
-__device__ __forceinline__ void load_row16(const __nv_bfloat16* p, float (&v)[16]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// HBM-bound: 256 bytes a 16-bit row read, 66 written, or the other way round.  Eight lanes take the K row and the V row of one token
+// and head, so that two rows' loads are in flight per lane; a lane has channels 8 sub .. + 7 and 64 + 8 sub .. + 7, so that an
+// instruction moves whole lines (thirty-two bytes a lane in one piece: every line took two instructions, 17.1 and 19.9 us below).
+// 12289 tokens of eight heads in fp16, rows in and out: 25.4 us for the two, where their 127 MB at a copy's rate take 19.4.
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
 }
-__device__ __forceinline__ void load_row16(const __half* p, float (&v)[16]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+__device__ __forceinline__ void load8(const __half* p, float* v) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     v[2 * i] = f.x; v[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void load_row16(const float* p, float (&v)[16]) {
+__device__ __forceinline__ void load8(const float* p, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
     v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
   }
@@ -205,45 +210,47 @@ append_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t k_st, in
     const int t = (int)((uint32_t)r / (uint32_t)H), h = (int)(r - (int64_t)t * H);
     const int64_t slot = __ldg(slots + t);
     float x[16], y[16];
-    load_row16(k + t * k_st + h * k_sh + sub * 16, x);
-    load_row16(v + t * v_st + h * v_sh + sub * 16, y);
+    const T* kr = k + t * k_st + h * k_sh + 8 * sub;
+    const T* vr = v + t * v_st + h * v_sh + 8 * sub;
+    load8(kr, x); load8(kr + 64, x + 8);
+    load8(vr, y); load8(vr + 64, y + 8);
     uint32_t ck[2], cv[2];
     const float ks = quant_row(x, ck), vs = quant_row(y, cv);
     if (mine < rows && slot >= 0 && slot < num_slots) {
       uint8_t* block = pages + block_offset(slot, h, H, page_shift);
       const int row = (int)(slot & (kTok - 1));
-      *reinterpret_cast<uint2*>(block + row * 64 + sub * 8) = make_uint2(ck[0], ck[1]);
-      *reinterpret_cast<uint2*>(block + kVOff + row * 64 + sub * 8) = make_uint2(cv[0], cv[1]);
+      uint32_t* to = reinterpret_cast<uint32_t*>(block + row * 64) + sub;
+      to[0] = ck[0]; to[8] = ck[1];
+      to += kVOff / 4;
+      to[0] = cv[0]; to[8] = cv[1];
       if (sub < 2)
         *reinterpret_cast<uint16_t*>(block + (sub ? kVsOff : kKsOff) + 2 * row) = (uint16_t)(__float_as_uint(sub ? vs : ks) >> 16);
     }
   }
 }
 
-__device__ __forceinline__ void store_row16(__nv_bfloat16* p, const float (&v)[16]) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<uint32_t*>(&h); }
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+// eight values, in pairs (0 4) (1 5) (2 6) (3 7) as they are unpacked, to channels 0 .. 7
+__device__ __forceinline__ void store8(__half* p, uint4 v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(prmt(v.x, v.y, 0x5410u), prmt(v.z, v.w, 0x5410u), prmt(v.x, v.y, 0x7632u), prmt(v.z, v.w, 0x7632u));
 }
-__device__ __forceinline__ void store_row16(__half* p, const float (&v)[16]) {
-  uint32_t w[8];
+__device__ __forceinline__ void floats8(uint4 v, float2 (&f)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<uint32_t*>(&h); }
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
 }
-__device__ __forceinline__ void store_row16(float* p, const float (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+__device__ __forceinline__ void store8(__nv_bfloat16* p, uint4 v) {
+  float2 f[4];
+  floats8(v, f);
+  const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(f[0].x, f[1].x), __floats2bfloat162_rn(f[2].x, f[3].x), __floats2bfloat162_rn(f[0].y, f[1].y),
+                               __floats2bfloat162_rn(f[2].y, f[3].y)};
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(h);
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void dequant16(uint2 c, float s, float (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = (float)((int)(c.x << (28 - 4 * i)) >> 28) * s;
-    v[8 + i] = (float)((int)(c.y << (28 - 4 * i)) >> 28) * s;
-  }
+__device__ __forceinline__ void store8(float* p, uint4 v) {
+  float2 f[4];
+  floats8(v, f);
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0].x, f[1].x, f[2].x, f[3].x);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[0].y, f[1].y, f[2].y, f[3].y);
 }
 
 template <typename T>
@@ -252,24 +259,25 @@ read_kernel(const uint8_t* __restrict__ pages, int64_t num_slots, int page_shift
             T* __restrict__ k, T* __restrict__ v) {
   const int lane = threadIdx.x & 31, sub = lane & 7;
   const int64_t rows = (int64_t)n * H, step = (int64_t)gridDim.x * 32;
+  const Unpack u = unpack_masks();
   for (int64_t r = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); r < rows; r += step) {
     const int t = (int)((uint32_t)r / (uint32_t)H), h = (int)(r - (int64_t)t * H);
     const int64_t slot = __ldg(slots + t);
-    uint2 ck = make_uint2(0u, 0u), cv = ck;
+    uint32_t c[4] = {0u, 0u, 0u, 0u};
     float ks = 0.f, vs = 0.f;
     if (slot >= 0 && slot < num_slots) {
       const uint8_t* block = pages + block_offset(slot, h, H, page_shift);
       const int row = (int)(slot & (kTok - 1));
-      ck = __ldg(reinterpret_cast<const uint2*>(block + row * 64) + sub);
-      cv = __ldg(reinterpret_cast<const uint2*>(block + kVOff + row * 64) + sub);
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(block + row * 64) + sub;
+      c[0] = __ldg(from); c[1] = __ldg(from + 8); c[2] = __ldg(from + kVOff / 4); c[3] = __ldg(from + kVOff / 4 + 8);
       ks = __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(block + kKsOff) + row) << 16);
       vs = __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(block + kVsOff) + row) << 16);
     }
-    float x[16];
-    dequant16(ck, ks, x);
-    store_row16(k + r * 128 + sub * 16, x);
-    dequant16(cv, vs, x);
-    store_row16(v + r * 128 + sub * 16, x);
+    const __half2 k2 = __float2half2_rn(ks), v2 = __float2half2_rn(vs);
+    T* kr = k + r * 128 + 8 * sub;
+    T* vr = v + r * 128 + 8 * sub;
+    store8(kr, values8(u, c[0], k2)); store8(kr + 64, values8(u, c[1], k2));
+    store8(vr, values8(u, c[2], v2)); store8(vr + 64, values8(u, c[3], v2));
   }
 }
 
@@ -310,8 +318,18 @@ extern "C" int hq_page_advance(const hq_page_advance_args* a, void* stream) {
     HQ_CUDA(cudaFuncSetAttribute(advance_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kAdvMostR + 3) * (int)sizeof(int)));
     attr_dev = dev;
   }
-  advance_kernel<<<1, kAdvThreads, smem, (cudaStream_t)stream>>>(p, 1);
-  HQ_CUDA(cudaGetLastError());
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a->T >= kAdvMany ? kAdvBlocks : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(attr.val.clusterDim.x);
+  cfg.blockDim = dim3(kAdvThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  HQ_CUDA(cudaLaunchKernelEx(&cfg, advance_kernel, p, (int)attr.val.clusterDim.x));
   return HQ_OK;
 }
 

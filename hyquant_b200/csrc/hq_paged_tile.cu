@@ -174,20 +174,6 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
   return out;
 }
 
-// Eight codes -> eight values in the order 0 4 1 5 2 6 3 7.  Nibbles in the low mantissa bits are 1024 + 8 + code, or 1024 + 16 (8 + code)
-// four bits up; the code is taken out exactly and its product with the scale is an fp16 number.
-struct Unpack { uint32_t lo, hi, lo8, hi8; };
-__device__ __forceinline__ uint4 values8(const Unpack& k, uint32_t w, __half2 s) {
-  const uint32_t w8 = w >> 8;
-  auto h2 = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
-  auto u32 = [](__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); };
-  const __half2 c1032 = h2(0xE408E408u), c16th = h2(0x2C002C00u), c72 = h2(0xD480D480u);       // -1032, 1 / 16, -72
-  return make_uint4(u32(__hmul2(__hadd2(h2(lop3_and_xor(w, k.lo, k.lo8)), c1032), s)),
-                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w, k.hi, k.hi8)), c16th, c72), s)),
-                    u32(__hmul2(__hadd2(h2(lop3_and_xor(w8, k.lo, k.lo8)), c1032), s)),
-                    u32(__hmul2(__hfma2(h2(lop3_and_xor(w8, k.hi, k.hi8)), c16th, c72), s)));
-}
-
 __device__ __forceinline__ void halves_meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the eight softmax warps
 
 template <bool kBf16>
@@ -369,11 +355,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
     // Lane: row lane / 4 of a group of eight keys, channels 32 (lane % 4) ..  A warp reads 512 bytes in one piece; the lanes of the
     // upper channels take their words two apart, so that no two of eight lanes write to the same banks either.
     const int w = warp - 8, rowl = lane >> 2, quarter = lane & 3, turn = quarter & 2;
-    Unpack uk;                                   // kept in registers: as constants they are loaded again beside every use
-    asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(uk.lo));
-    asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(uk.hi));
-    asm volatile("mov.b32 %0, 0x64086408;" : "=r"(uk.lo8));
-    asm volatile("mov.b32 %0, 0x64806480;" : "=r"(uk.hi8));
+    const Unpack uk = unpack_masks();
     int n_all = 0;
     while (pc.take(p)) { n_all += pc.t1 - pc.t0; pc.done(p); }
     int ks = 0, vs = 0;

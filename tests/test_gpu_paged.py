@@ -90,6 +90,29 @@ def test_advance_pages_pass_from_one_request_to_another_in_one_step():
     assert s.step([0, 3, 64, 0], [0, 61, 0, 0], 70, True) == 0
 
 
+@pytest.mark.parametrize("R,T", [(1, 12287), (1, 12288), (3, 16385), (400, 70000)])
+def test_advance_many_tokens(R, T):
+    """The sizes around which one block's work becomes eight blocks', with pages that pass from request to request."""
+    rng = random.Random(T)
+    s = State(R, 16, 2 * T // 16 // R + 8, 2 * T // 16 + 2 * R)
+    assert s.step([T // R] * R, None, T, False) == 0
+    keep = [rng.randint(0, n) for n in s.book.lens]
+    assert s.step([rng.randint(0, n - k) for n, k in zip(s.book.lens, keep)], keep, T, True) == 0
+    s.step([T] * R, None, T, True)                                          # one request has room for them, several have not
+    s.step([1] * R, None, T, False)
+
+
+def test_advance_length_past_32_bits():
+    pages = 2 ** 24 + 4                                                     # rows of more tokens than a position holds
+    n = 2 ** 31 - 100
+    table = torch.zeros(1, pages, dtype=torch.int32, device=DEV)
+    got = hq.page_advance(ints([n]), ints([2 ** 24]), ints([200]), table, ints([0] * 8), ints([8]), page_size=128, max_tokens=200)
+    assert int(got.status) == 2 and got.kv_lens.tolist() == [n] and got.slots.tolist() == [-1] * 200
+    got = hq.page_advance(ints([n]), ints([2 ** 24]), ints([99]), table, ints([0] * 8), ints([8]), page_size=128, max_tokens=99)
+    assert int(got.status) == 0 and got.kv_lens.tolist() == [2 ** 31 - 1] and got.positions.tolist() == list(range(n, 2 ** 31 - 1))
+    assert int(got.free_count) == 8
+
+
 # ---------------------------------------------------------------------------------------------- rows in, rows out
 
 def special_rows(dtype):
