@@ -37,6 +37,11 @@ struct AttnParams {
   float* ws;
 };
 
+// positions that the tile kernel gives a key tile of 64 that both halves of its softmax work on, one that a half has to itself, and a
+// query tile beside them: about 400 clocks each
+constexpr int kFullCost = 5, kSplitCost = 4, kItemCost = 30;
+constexpr double kTilePerKey = kFullCost / 64., kTilePerItem = kItemCost + kFullCost;
+
 int64_t decode_workspace(const AttnParams& p);                 // bytes; hq_paged_decode.cu
 int decode_launch(const AttnParams& p, cudaStream_t st);
 int64_t tile_workspace(const AttnParams& p);                   // hq_paged_tile.cu
@@ -155,6 +160,10 @@ struct Cuts {
   }
 };
 
+// Sums of weights stop at 2^31 - 1.  Starts that rise never get there (the entry point sees to that); starts that rise and fall can hand the
+// same rows to many requests, and their positions past that number are left out.
+__device__ __forceinline__ int add_sat(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7FFFFFFFu); }
+
 // The requests' weights in a row.  Up to 64 requests every warp adds them up by itself; more go through shared memory (part: threads + 1
 // words, s_warp: a word per warp), a run of requests per thread.  All threads call the constructor, whole warps `seek`.
 template <int kThreads, class Weight>
@@ -167,7 +176,7 @@ struct Prefix {
   __device__ __forceinline__ static int scan(int x) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x = add_sat(x, y); }
     return x;
   }
   __device__ __forceinline__ Prefix(const AttnParams& pp, Weight w, int* part, int* s_warp) : p(pp), weight(w), s_part(part) {
@@ -176,20 +185,20 @@ struct Prefix {
       w0 = scan(lane < p.R ? weight(request_of(p, lane)) : 0);
       total = __shfl_sync(0xffffffffu, w0, 31);
       if (p.R > 32) {
-        w1 = scan(32 + lane < p.R ? weight(request_of(p, 32 + lane)) : 0) + total;
+        w1 = add_sat(scan(32 + lane < p.R ? weight(request_of(p, 32 + lane)) : 0), total);
         total = __shfl_sync(0xffffffffu, w1, 31);
       }
       return;
     }
     per = (p.R + kThreads - 1) / kThreads;
     int mine = 0;
-    for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine += weight(request_of(p, r));
+    for (int r = tid * per; r < min(p.R, (tid + 1) * per); ++r) mine = add_sat(mine, weight(request_of(p, r)));
     const int x = scan(mine);
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
     const int sums = scan(lane < kThreads / 32 ? s_warp[lane] : 0), before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
     total = __shfl_sync(0xffffffffu, sums, 31);
-    part[tid + 1] = x + (warp ? before : 0);
+    part[tid + 1] = add_sat(x, warp ? before : 0);
     if (tid == 0) part[0] = 0;
     __syncthreads();
   }

@@ -7,6 +7,8 @@ namespace paged {
 
 static int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
 
+static bool few_rows(const hq_paged_attention_args* a) { return (int64_t)a->max_q_len * (a->H_Q / a->H_KV) <= 16; }
+
 static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a != nullptr, HQ_ERR_INVALID, "hq_paged_attention: null argument block");
   HQ_REQUIRE(a->struct_bytes == (int)sizeof(hq_paged_attention_args), HQ_ERR_INVALID, "hq_paged_attention: struct_bytes %d, expected %d",
@@ -26,10 +28,11 @@ static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a->num_pages * a->H_KV <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_paged_attention: %lld pages of %d kv heads", (long long)a->num_pages, a->H_KV);
   HQ_REQUIRE((int64_t)a->T * (a->H_Q / a->H_KV) < (1 << 27), HQ_ERR_UNSUPPORTED, "hq_paged_attention: %d tokens of %d query heads a kv head", a->T,
              a->H_Q / a->H_KV);
-  // places in the row of all requests' keys are 32-bit numbers: a key tile of 64 costs two, or one for each of 32 keys, and every query
-  // tile of 256 rows has its own
-  const double tiles = (double)a->R + (double)a->T * (a->H_Q / a->H_KV) / 256, keys = (double)a->max_pages * a->page_size;
-  HQ_REQUIRE(tiles * a->H_KV * (keys / 32 + 8) < 2147483647.0, HQ_ERR_UNSUPPORTED,
+  // Places in the row of all requests' keys are 32-bit numbers (at most kTilePerKey a cached token and kTilePerItem more for each query tile
+  // of 256 rows, or a unit of 32 tokens and two more for each kv head): tables this long, for this many rows, are refused.
+  const double items = few_rows(a) ? (double)a->R : (double)a->R + (double)a->T * (a->H_Q / a->H_KV) / 256;
+  const double each = (double)a->max_pages * a->page_size * (few_rows(a) ? 1. / 32 : kTilePerKey) + (few_rows(a) ? 2 : kTilePerItem);
+  HQ_REQUIRE(items * a->H_KV * each < 2147483647.0, HQ_ERR_UNSUPPORTED,
              "hq_paged_attention: %d requests, %d tokens and tables of %d pages of %d tokens are too much for one call", a->R, a->T, a->max_pages, a->page_size);
   if (a->R == 0 || a->T == 0) return HQ_OK;
   HQ_REQUIRE(a->q && a->out && a->kv_lens && (a->page_table || a->max_pages == 0) && (a->pages || a->num_pages == 0), HQ_ERR_INVALID,
@@ -54,8 +57,7 @@ static AttnParams params_of(const hq_paged_attention_args* a) {
   p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh; p.dtype = a->dtype;
   return p;
 }
-static bool few_rows(const AttnParams& p) { return (int64_t)p.max_q_len * p.G <= 16; }
-static int64_t workspace_of(const AttnParams& p) { return few_rows(p) ? decode_workspace(p) : tile_workspace(p); }
+static int64_t workspace_of(const hq_paged_attention_args* a, const AttnParams& p) { return few_rows(a) ? decode_workspace(p) : tile_workspace(p); }
 
 }  // namespace paged
 }  // namespace hq
@@ -65,7 +67,7 @@ extern "C" int hq_paged_attention_workspace_bytes(const hq_paged_attention_args*
   if (int rc = paged::check(a)) return rc;
   HQ_REQUIRE(bytes, HQ_ERR_INVALID, "hq_paged_attention_workspace_bytes: null pointer");
   const paged::AttnParams p = paged::params_of(a);
-  *bytes = a->R > 0 && a->T > 0 ? paged::workspace_of(p) : 0;
+  *bytes = a->R > 0 && a->T > 0 ? paged::workspace_of(a, p) : 0;
   return HQ_OK;
 }
 
@@ -75,9 +77,9 @@ extern "C" int hq_paged_attention(const hq_paged_attention_args* a, void* stream
   if (int rc = check(a)) return rc;
   if (a->R == 0 || a->T == 0) return HQ_OK;
   const AttnParams p = params_of(a);
-  const int64_t need = workspace_of(p);
+  const int64_t need = workspace_of(a, p);
   HQ_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), HQ_ERR_WORKSPACE, "hq_paged_attention: %lld bytes of workspace, %lld needed",
              (long long)a->workspace_bytes, (long long)need);
   HQ_REQUIRE(aligned16(a->workspace), HQ_ERR_ALIGNMENT, "hq_paged_attention: the workspace must be 16-byte aligned");
-  return few_rows(p) ? decode_launch(p, (cudaStream_t)stream) : tile_launch(p, (cudaStream_t)stream);
+  return few_rows(a) ? decode_launch(p, (cudaStream_t)stream) : tile_launch(p, (cudaStream_t)stream);
 }

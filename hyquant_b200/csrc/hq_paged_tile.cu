@@ -32,9 +32,6 @@ constexpr int kIssue = 12, kFetch = 14;          // first issuing warp; the fetc
 constexpr int kKStages = 3, kVStages = 4;        // K tiles and V tiles in shared memory
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
-// positions, of about 200 clocks each: a key tile that both halves work on, one that a half has to itself (KEEP clocks against 1950), and
-// what a query tile costs beside them (queries 3500, first reference and masks 2600 each, results 5000)
-constexpr int kFullCost = 10, kSplitCost = 8, kItemCost = 60;
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
 constexpr uint32_t kTPolls = 400000u;
 

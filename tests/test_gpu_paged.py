@@ -348,6 +348,21 @@ def test_starts_that_are_no_starts(new):
     assert (room[0] == 7).all() and (room[-1] == 7).all()
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 1, 3], [90, 3, 200]])
+def test_a_query_that_is_no_number(new, value):
+    """It makes its own row NaN and leaves the others as they are."""
+    lens = [250, 131, 300]
+    q, pages, table, cu = make(lens, new, 8, 2, 64, torch.bfloat16, seed=34)
+    q[1, 2, 77] = value
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    assert got[1, 2].isnan().all()
+    got[1, 2], q[1, 2] = 0, 0
+    want, tol = plain.attention(q, pages, table, lens, cu)
+    want[1, 2] = 0
+    assert ((got.double() - want).abs() <= tol).all()
+
+
 def test_offsets_past_32_bits():
     """A pool of 6 GB whose last pages are the ones in use."""
     page, H = 128, 8

@@ -46,6 +46,16 @@ def test_attention_refusals(fields, code, text):
     assert lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n)) == code
 
 
+@pytest.mark.parametrize("fields", [dict(R=4000, T=4096, H_Q=32, H_KV=8, max_q_len=4096, max_pages=1 << 13, page_size=128, table_stride=1 << 13),
+                                    dict(R=3, T=1 << 20, max_q_len=1 << 20, max_pages=1 << 14, table_stride=1 << 14),
+                                    dict(R=1 << 15, T=1 << 15, H_KV=8, max_q_len=1, max_pages=1 << 14, table_stride=1 << 14)])
+def test_more_positions_than_32_bits_hold(fields):
+    lib, n = _lib.lib(), C.c_int64()
+    a = attention_args(**fields)
+    assert lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n)) == -2 and b"too much" in lib.hq_last_error()
+    assert lib.hq_paged_attention(C.byref(a), None) == -2 and b"too much" in lib.hq_last_error()
+
+
 def test_attention_null_block_and_nothing_to_do():
     lib, n = _lib.lib(), C.c_int64(-1)
     assert lib.hq_paged_attention(None, None) == -1
