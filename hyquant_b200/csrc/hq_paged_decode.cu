@@ -1,11 +1,15 @@
 // Attention of a few new tokens per request over the paged 4-bit cache: calls whose new tokens times query heads per kv head
 // fit 16 rows (one token at every group size, drafts of a few).
 //
-// HBM-bound: 132 bytes a cached token and kv head, read once; at 6.5 TB/s an SM has some 100 clocks for 32 tokens.
+// 132 bytes a cached token and kv head, read once: at 6.5 TB/s an SM has some 100 clocks for 32 tokens, and the 530 instructions that a warp
+// spends on them (unpacking 176, exponentials and sums 60, products 34) take its four schedulers 130 at full rate, 240 as it is.
+// So long batches are bound by issue: 16 requests of up to 32768 tokens, 8 heads, 58 us, 4.0 TB/s.  Short calls are bound by a chain
+// of latencies (finding the part, first copy, queries, one unit, the merges): one request of 517 tokens 8.6 us, of 32768 16.4 us.
+// Nine to sixteen rows a head double the products and exponentials, not the unpacking: 4 requests of up to 131072 tokens, 2 heads, 50 us.
 //
 // Work split.  A kv head of a request is a run of units of 32 tokens and one closing unit, so that heads without tokens cost
-// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one of 16 warps per SM, and a block's
-// part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
+// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one of 16 warps per SM (12 for more than eight rows, which
+// take more registers), and a block's part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
 // barrier inside, and a run that lies within one warp's part is written out by that warp.  Runs that several warps share are
 // merged through shared memory at the block's end, runs that several blocks share by the merge kernel.  Everything goes by
 // position, nothing by arrival: results do not depend on timing, and no counter has to be zero beforehand.
@@ -610,8 +614,9 @@ merge_kernel(const AttnParams p, int grid) {
 
 static int tiles_of(const AttnParams& p) { return p.max_q_len * p.G <= 8 ? 1 : 2; }
 
-// Short tables and no more runs than SMs: a block per run, nothing to merge across blocks, one launch and no workspace.  Longer
-// ones gain more from every SM's share of the bandwidth: KEEP
+// Short tables and no more runs than SMs: a block per run, nothing to merge across blocks, one launch and no workspace.  Against the cut
+// over all SMs: one request of 8 heads, 512 tokens 8.0 us and 10.6, 1024 9.8 and 11.4, 2048 13.3 and 11.3; eight requests 8.2 and
+// 10.9, 10.0 and 11.0, 13.7 and 12.7; sixteen rows a head 14.0 and 18.7, 17.0 and 17.7, 22.9 and 17.8.
 static bool block_per_run(const AttnParams& p) {
   return ((int64_t)p.max_pages << p.page_shift) <= 1024 && (int64_t)p.R * p.H_KV <= sm_count();
 }
