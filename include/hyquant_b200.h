@@ -466,7 +466,7 @@ int hq_prefill_vertical_gather_v_fp8(const int32_t* vidx_asc, int B, int H_Q, in
  *   kv_lens, held (pages in the row), add, keep  int32 [R]; page_table int32 [R, max_pages] with row stride table_stride;
  *   free_pages int32 [free_cap]; free_count int32 [1]; cu_q int32 [R + 1]; slots int64 [T]; positions int32 [T]
  *   status int32 [1]: 0, or why nothing was changed (cu_q is then 0 throughout, slots -1): bit 0 too few free pages, bit 1 a
- *   request longer than max_pages, bit 2 more than T new tokens, bit 3 arguments that do not fit (keep > kv_lens, a negative
+ *   request longer than max_pages or than 2^31 - 1 tokens, bit 2 more than T new tokens, bit 3 arguments that do not fit (keep > kv_lens, a negative
  *   number, held outside [ceil(kv_lens / page_size), max_pages], a full stack).  The word is written by every call. */
 typedef struct hq_page_advance_args {
   int32_t struct_bytes;
@@ -494,7 +494,9 @@ int hq_paged_read(const void* pages, int64_t num_pages, int page_size, const int
  * (null: token r) and kv_lens[r] cached tokens with them; its token i of n sees keys 0 .. kv_lens[r] - n + i:
  *   out[t, h] = sum_j softmax_j(sm_scale q[t, h] . k_j) v_j;   a token that sees no key gets zeros.
  * max_q_len: no request has more tokens (those beyond are not computed).  Rows of out behind the last token are not written.
- * Lengths past the table and pages outside the pool are treated as absent keys. */
+ * Lengths past the table and pages outside the pool are treated as absent keys.  Refused (HQ_ERR_UNSUPPORTED): 2^27 rows (tokens
+ * times query heads per kv head) or more, tables and rows whose 32-token units, or 64-token tiles times 256-row query tiles, pass the
+ * kernels' 32-bit positions.  A device wait that runs out makes the rows concerned NaN. */
 typedef struct hq_paged_attention_args {
   int32_t struct_bytes;
   int32_t R, T, H_Q, H_KV, head_dim;          /* H_Q / H_KV 1..16, head_dim 128 */
