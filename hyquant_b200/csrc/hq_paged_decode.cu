@@ -31,7 +31,7 @@ constexpr int kRowPad = 132;                    // floats of a row of a piece
 constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9): at most 2^10 when a reference is set, 2^15 before it moves
 constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
 constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ that lets it stay
-__host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 16 : 12; }
+__host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 12 : 8; }
 __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
