@@ -2,14 +2,15 @@
 // fit 16 rows (one token at every group size, drafts of a few).
 //
 // 132 bytes a cached token and kv head, read once: at 6.5 TB/s an SM has some 100 clocks for 32 tokens, and the 530 instructions that a warp
-// spends on them (unpacking 176, exponentials and sums 60, products 34) take its four schedulers 130 at full rate, 240 as it is.
+// spends on them (unpacking 176, exponentials and sums 60, products 34) take its four schedulers 130 at full rate; half of them are for the
+// ALU pipe, which takes one every other clock.  It is 240 as it is.
 // So long batches are bound by issue: 16 requests of up to 32768 tokens, 8 heads, 58 us, 4.0 TB/s.  Short calls are bound by a chain
-// of latencies (finding the part, first copy, queries, one unit, the merges): one request of 517 tokens 8.6 us, of 32768 16.4 us.
-// Nine to sixteen rows a head double the products and exponentials, not the unpacking: 4 requests of up to 131072 tokens, 2 heads, 50 us.
+// of latencies (finding the part, first copy, queries, one unit, the merges): one request of 517 tokens 7.7 us, of 32768 15.7 us.
+// Nine to sixteen rows a head double the products and exponentials, not the unpacking: 4 requests of up to 131072 tokens, 2 heads, 47 us.
+// O += P V beside the next unit's scores in one stretch of code, in order or interleaved, gave nothing (61 us where the batch takes 58).
 //
 // Work split.  A kv head of a request is a run of units of 32 tokens and one closing unit, so that heads without tokens cost
-// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one of 16 warps per SM (12 for more than eight rows, which
-// take more registers), and a block's part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
+// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one per SM, and a block's part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
 // barrier inside, and a run that lies within one warp's part is written out by that warp.  Runs that several warps share are
 // merged through shared memory at the block's end, runs that several blocks share by the merge kernel.  Everything goes by
 // position, nothing by arrival: results do not depend on timing, and no counter has to be zero beforehand.
@@ -31,6 +32,9 @@ constexpr int kRowPad = 132;                    // floats of a row of a piece
 constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9): at most 2^10 when a reference is set, 2^15 before it moves
 constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
 constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ that lets it stay
+// Warps of a block: few enough for their registers (168 and 234 without spills), and as many on every scheduler.  The 32768 tokens, the batch
+// and 200 short requests: 16 warps 16.6, 57.8, 28.7 us, 14 17.3, 62.8, 29.3, 12 15.7, 57.8, 25.5, 11 17.1, 63.4, 26.1, 8 17.1, 68.4, 28.1.
+// More than eight rows: 12 warps 49.6 us, 11 51.1, 10 54.4, 8 47.0.
 __host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 12 : 8; }
 __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
 
@@ -459,7 +463,7 @@ decode_kernel(const AttnParams p, bool whole) {
   __syncthreads();
   bool inside = start_u > 0;                                 // the run in hand began before this part
   // the first unit is asked for before anything else, the others of the ring behind the queries: a copy takes the SM's copy engine some
-  // 25 ns, 16 warps' rings 1.2 us
+  // 25 ns, 12 warps' rings 0.9 us
   if (left > 0) { ask_q(request_of(p, c.r), 0); fetch(); ++ahead; }
 #pragma unroll 1
   while (left > 0) {
@@ -615,8 +619,8 @@ merge_kernel(const AttnParams p, int grid) {
 static int tiles_of(const AttnParams& p) { return p.max_q_len * p.G <= 8 ? 1 : 2; }
 
 // Short tables and no more runs than SMs: a block per run, nothing to merge across blocks, one launch and no workspace.  Against the cut
-// over all SMs: one request of 8 heads, 512 tokens 8.0 us and 10.6, 1024 9.8 and 11.4, 2048 13.3 and 11.3; eight requests 8.2 and
-// 10.9, 10.0 and 11.0, 13.7 and 12.7; sixteen rows a head 14.0 and 18.7, 17.0 and 17.7, 22.9 and 17.8.
+// over all SMs: one request of 8 heads, 512 tokens 7.3 us and 10.3, 1024 9.4 and 9.7, 2048 13.1 and 9.9; eight requests 7.5 and
+// 10.5, 9.7 and 10.9, 13.7 and 12.7; four of 2 heads with sixteen rows 11.8 and 15.1, 14.9 and 15.3, 21.2 and 15.2.
 static bool block_per_run(const AttnParams& p) {
   return ((int64_t)p.max_pages << p.page_shift) <= 1024 && (int64_t)p.R * p.H_KV <= sm_count();
 }
