@@ -11,7 +11,7 @@ cache's values without rounding them again.  Values beyond +-65408 saturate; a N
 
 A step is: :func:`page_advance` (block tables, slots, positions - once for all layers), then per layer :func:`paged_append`
 and :func:`paged_attention`.  All of it stays on the device, allocates only its outputs (and attention its scratch) and
-can be captured in a CUDA graph.  :class:`PagedKVCache` keeps the state of a whole model.
+can be captured in a CUDA graph.  Nothing here has gradients.  :class:`PagedKVCache` keeps the state of a whole model.
 """
 
 from __future__ import annotations

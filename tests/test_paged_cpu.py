@@ -1,6 +1,8 @@
 """The paged cache's checks of arguments, and its entry points in the C ABI; nothing here reaches a GPU."""
 
 import ctypes as C
+import os
+import re
 
 import pytest
 import torch
@@ -36,6 +38,7 @@ def attention_args(**fields):
     (dict(sm_scale=-1.0), -1, b"sm_scale"), (dict(sm_scale=float("nan")), -1, b"sm_scale"), (dict(sm_scale=float("inf")), -1, b"sm_scale"),
     (dict(cu_q=None), -1, b"cu_q"), (dict(q=None), -1, b"null"), (dict(out=None), -1, b"null"), (dict(kv_lens=None), -1, b"null"),
     (dict(page_table=None), -1, b"null"), (dict(pages=None), -1, b"null"), (dict(table_stride=9), -1, b"overlap"),
+    (dict(o_st=0), -1, b"overlap"), (dict(o_sh=64), -1, b"overlap"),
     (dict(q=FAKE + 8), -3, b"aligned"), (dict(out=FAKE + 2), -3, b"aligned"), (dict(pages=FAKE + 4), -3, b"aligned"),
     (dict(q_st=1028), -3, b"aligned"), (dict(o_sh=129), -3, b"aligned"),
 ])
@@ -149,3 +152,13 @@ def test_argument_blocks_as_bytes():
 def test_format_constants():
     assert paged_kv.BLOCK_BYTES == 2 * paged_kv.BLOCK * 64 + 2 * paged_kv.BLOCK * 2
     assert [f[0] for f in _lib.PagedAttentionArgs._fields_][-2:] == ["workspace", "workspace_bytes"] and C.sizeof(_lib.PagedAttentionArgs) == 160
+
+
+@pytest.mark.parametrize("name,mirror", [("hq_page_advance_args", _lib.PageAdvanceArgs), ("hq_paged_attention_args", _lib.PagedAttentionArgs)])
+def test_the_listed_argument_blocks_are_the_bound_ones(name, mirror):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "INTEGRATION.md")).read()
+    fields = eval(re.search(r"class %s\(C\.Structure\):\n    _fields_ = (\[.*?\)\])\n" % name, text, re.S).group(1), {"C": C})
+    listed = type("Listed", (C.Structure,), {"_fields_": fields})
+    assert [f[0] for f in fields] == [f[0] for f in mirror._fields_] and C.sizeof(listed) == C.sizeof(mirror)
+    assert all(getattr(listed, f[0]).offset == getattr(mirror, f[0]).offset for f in fields)
