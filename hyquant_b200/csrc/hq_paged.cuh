@@ -39,7 +39,7 @@ struct AttnParams {
 
 // positions that the tile kernel gives a key tile of 64 that both halves of its softmax work on, one that a half has to itself, and a
 // query tile beside them, in 400 clocks: 1930, 1300 to 1500, and queries 3500, first reference and masks 2600 each, results 5000.
-// With nothing for the query tiles chunks of 1 to 512 tokens took 238 us, with this 145.
+// With nothing for the query tiles six chunks of 1 to 700 tokens took 238 us, with this 145 at that time.
 constexpr int kFullCost = 5, kSplitCost = 4, kItemCost = 30;
 constexpr double kTilePerKey = kFullCost / 64., kTilePerItem = kItemCost + kFullCost;
 
