@@ -38,7 +38,7 @@ struct AttnParams {
 };
 
 // positions that the tile kernel gives a key tile of 64 that both halves of its softmax work on, one that a half has to itself, and a
-// query tile beside them, in 400 clocks: 1930, 1300 to 1500, and queries 3500, first reference and masks 2600 each, results 5000.
+// query tile beside them, in 400 clocks: 1930, 1300 to 1500, and some 12000 for queries, first reference, masks and results.
 // With nothing for the query tiles six chunks of 1 to 700 tokens took 238 us, with this 145 at that time.
 constexpr int kFullCost = 5, kSplitCost = 4, kItemCost = 30;
 constexpr double kTilePerKey = kFullCost / 64., kTilePerItem = kItemCost + kFullCost;

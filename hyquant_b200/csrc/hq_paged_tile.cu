@@ -5,7 +5,7 @@
 // group size; keys come in tiles of 64.  The two halves of the softmax take 128 rows each, or, where a query tile has no more than
 // 128 rows, the same rows and every other key tile, and join their states at the end.  A key tile of 256 rows is 8.4 MFLOP and 16384
 // exponentials, some 1024 clocks of an SM each at their nominal rates; the products' operands and the unpacked tiles pass through
-// shared memory in some 1600.  It takes 1930: a prompt of 2048 tokens over 32768 cached ones, 32 heads over 8, 906 us, 1.18 PFLOP/s.
+// shared memory in some 1600.  It takes 1930: a prompt of 2048 tokens over 32768 cached ones, 32 heads over 8, 890 us, 1.20 PFLOP/s.
 // Exponentials moved to the FMA pipe (an eighth to a half of them, by polynomial) gave nothing, key tiles of 128 lost the second
 // buffer of scores and took 1236 us where 64 took 1052.
 //

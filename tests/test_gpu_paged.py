@@ -515,3 +515,32 @@ def test_two_graphs_and_an_eager_call_at_once():
     torch.cuda.synchronize()
     for a, b in (*outs, again):
         assert torch.equal(a, want) and torch.equal(b, want3)
+
+
+def test_a_prompt_step_in_a_cuda_graph():
+    """Bookkeeping by several blocks, rows and reading back, one behind the other in a graph: as the same calls made eagerly."""
+    T, R = 12500, 7
+    caches = [hq.PagedKVCache(1, 3 * T // 16 + 2 * R, 2, max_requests=R, max_pages_per_request=3 * T // 16 + 1, page_size=16) for _ in range(2)]
+    add, keep = torch.zeros(R, dtype=torch.int32, device=DEV), torch.zeros(R, dtype=torch.int32, device=DEV)
+    k = torch.randn(T, 2, 128, device=DEV).to(torch.float16)
+
+    def step(cache):
+        made = cache.advance(add, max_tokens=T, keep=keep)
+        cache.append(0, k, -k)
+        return made.slots, made.positions, made.status, *cache.read(0, made.slots, torch.float32)
+
+    step(caches[1])                                                         # nothing to add yet: the lazy parts are loaded
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[1])
+    rng = random.Random(5)
+    for _ in range(4):
+        lens = caches[0].kv_lens.tolist()
+        kept = [rng.randint(0, n) for n in lens]
+        add.copy_(ints([rng.randint(0, T // R) for _ in range(R)]))
+        keep.copy_(ints(kept))
+        want = step(caches[0])
+        graph.replay()
+        assert int(got[2]) == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(caches[0].kv_lens, caches[1].kv_lens) and torch.equal(caches[0].pages[0], caches[1].pages[0])
+        assert torch.equal(caches[0].free_count, caches[1].free_count)
