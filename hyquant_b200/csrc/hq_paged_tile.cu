@@ -689,7 +689,9 @@ tile_merge_kernel(const AttnParams p, int piece_rows, int grid) {
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = o;
 }
 
-static int piece_rows_of(const AttnParams& p) { return (int)min((int64_t)kRows, (int64_t)p.max_q_len * p.G); }
+// Rows of a piece: as many as a query tile of the call has, an even number: a row is 130 floats, and pieces, which are moved in
+// 16-byte parts, lie one behind the other.
+static int piece_rows_of(const AttnParams& p) { return (int)min((int64_t)kRows, ((int64_t)p.max_q_len * p.G + 1) & ~(int64_t)1); }
 
 int64_t tile_workspace(const AttnParams& p) {
   const int64_t grid = sm_count();

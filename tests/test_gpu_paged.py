@@ -544,3 +544,13 @@ def test_a_prompt_step_in_a_cuda_graph():
         assert int(got[2]) == 0 and all(torch.equal(a, b) for a, b in zip(got, want))
         assert torch.equal(caches[0].kv_lens, caches[1].kv_lens) and torch.equal(caches[0].pages[0], caches[1].pages[0])
         assert torch.equal(caches[0].free_count, caches[1].free_count)
+
+
+@pytest.mark.parametrize("heads,new", [((7, 1), [3, 1]), ((7, 1), [5, 2]), ((28, 4), [3, 3, 1]), ((1, 1), [17]), ((1, 1), [255, 31]), ((3, 3), [21, 85]),
+                                       ((11, 1), [23])])
+def test_shared_query_tiles_of_odd_numbers_of_rows(heads, new):
+    """Contexts long enough that several blocks share a query tile: its pieces go through the workspace."""
+    lens = [9000, 4100, 2500][:len(new)]
+    q, pages, table, cu = make(lens, new, *heads, 64, torch.bfloat16, seed=sum(new))
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+    verify(got, q, pages, table, lens, cu)

@@ -162,3 +162,21 @@ def test_the_listed_argument_blocks_are_the_bound_ones(name, mirror):
     listed = type("Listed", (C.Structure,), {"_fields_": fields})
     assert [f[0] for f in fields] == [f[0] for f in mirror._fields_] and C.sizeof(listed) == C.sizeof(mirror)
     assert all(getattr(listed, f[0]).offset == getattr(mirror, f[0]).offset for f in fields)
+
+
+def test_pieces_of_query_tiles_begin_on_16_bytes():
+    """A query tile's piece in the workspace (its rows of 128 sums, a maximum and a sum each) is read and written in 16-byte pieces,
+    two of them one behind the other per block and 32 bytes of a merge's order: whatever the rows, odd numbers of them too."""
+    lib, n = _lib.lib(), C.c_int64()
+
+    def workspace(G, most):
+        a = attention_args(H_Q=G, H_KV=1, max_q_len=most)
+        assert lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n)) == 0
+        return n.value
+    full = 2 * 256 * 130 * 4 + 32
+    blocks = workspace(1, 256) // full
+    assert blocks >= 1 and workspace(1, 256) == blocks * full
+    for G in range(1, 17):
+        for most in range(16 // G + 1, 260):
+            per, rest = divmod(workspace(G, most), blocks)
+            assert rest == 0 and (per - 32) % 32 == 0 and (per - 32) // 2 >= min(256, most * G) * 130 * 4, (G, most)
