@@ -182,6 +182,7 @@ decode_kernel(const AttnParams p, bool whole) {
   uint32_t parity = 0;
   Walk f = c;                                                // the unit that is fetched next
   int f_left = left, tab_r = -1, tab_u = 0;                  // pages of the units tab_u .. + 31 of request tab_r are at hand
+  bool lost = false;                                         // a copy never came: from there on the part's rows are NaN
   auto fetch = [&]() {                                       // asks for the next unit, if there is one; all lanes
     while (f_left > 0 && f.u >= f.units) { if (--f_left > 0) next_run(p, f); }
     if (f_left <= 0) return;
@@ -311,7 +312,7 @@ decode_kernel(const AttnParams p, bool whole) {
   const int tau = (g >> 1) + 4 * (g & 1);                    // token of score row g (and + 8): the four tokens of a V fragment's
                                                              // load are neighbours then, on both halves of the banks
   auto unit = [&](bool fresh) {                              // fresh: the run's first one here
-    const bool ok = mbar_wait_bounded(bar + slot, parity);
+    const bool late = lost || !mbar_wait_bounded(bar + slot, parity);
     const uint8_t* u0 = ring + slot * kUnitBytes;
     const int there = s_live[warp * kSlots + slot];
     float S[NT][2][4];
@@ -402,7 +403,15 @@ decode_kernel(const AttnParams p, bool whole) {
       }
       return !(most <= 32768.f) || !fits;
     };
-    if (__builtin_expect(__any_sync(0xffffffffu, form(fresh)), 0)) {
+    if (__builtin_expect(__any_sync(0xffffffffu, form(fresh) || late), 0)) {
+      if (!lost && __any_sync(0xffffffffu, late)) {
+        // Barriers of slots that are asked for again would be a phase behind: nothing more is fetched or waited for, only what is
+        // under way, once more, since its places are used for other things later.
+        lost = true;
+        f_left = 0;
+        for (int i = 0; i < ahead; ++i)
+          mbar_wait_bounded(bar + (slot + i >= kSlots ? slot + i - kSlots : slot + i), slot + i >= kSlots ? parity ^ 1u : parity, 1u << 16);
+      }
       const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
       // 2^-e for the largest scale's power of two e, kept in the range of normal numbers; smaller than before unless nothing was before
       const int e = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23), 1), 253);
@@ -431,7 +440,7 @@ decode_kernel(const AttnParams p, bool whole) {
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) { P[nt][cb][0] = movmatrix(P[nt][cb][0]); P[nt][cb][1] = movmatrix(P[nt][cb][1]); }
     }
-    if (!ok) {                                               // a copy that never came: the rows are NaN
+    if (lost) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) l[nt] = make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000));
     }
