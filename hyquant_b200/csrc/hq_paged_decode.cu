@@ -20,8 +20,9 @@
 // subnormals (one logic operation for two of them): the nibble + 8 as mantissa bits is (code + 8) 2^-24, or 2^-20 for a nibble four
 // bits up.  The power of two goes into the query operand and the epilogue, the 8 into the accumulators' start (K) and the row sum
 // of P (V, one more product against ones).  Queries are scaled by a power of two of their own so that fp16 holds them
-// exactly.  P v_scale is rounded to fp16, 11 bits against bf16's 8: relative to the largest v_scale so far, whose power of two moves like
-// the maximum does.
+// exactly.  P v_scale is rounded to fp16, 11 bits against bf16's 8, relative to the row's largest product so far: a row's one reference is
+// the maximum of score and log2 of v_scale together, so that a key with all the weight and a small value keeps its bits beside large
+// values without weight.  The row sum of P, in 32 bits, is relative to it too.
 #include "hq_paged.cuh"
 
 namespace hq {
@@ -29,9 +30,9 @@ namespace paged {
 
 constexpr int kUnit = 32, kUnitBytes = 2 * kBlockBytes, kSlots = 3;
 constexpr int kRowPad = 132;                    // floats of a row of a piece
-constexpr float kShift = 9.0f;                  // P~ = 2^(s - m + 9): at most 2^10 when a reference is set, 2^15 before it moves
+constexpr float kShift = 9.0f;                  // P~ v_scale = 2^(s - m + 9) v_scale: at most 2^10 when a reference is set, 2^15 before it moves
 constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
-constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ that lets it stay
+constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ v_scale that lets it stay
 // Warps of a block: few enough for their registers (168 and 234 without spills), and as many on every scheduler.  The 32768 tokens, the batch
 // and 200 short requests: 16 warps 16.6, 57.8, 28.7 us, 14 17.3, 62.8, 29.3, 12 15.7, 57.8, 25.5, 11 17.1, 63.4, 26.1, 8 17.1, 68.4, 28.1.
 // More than eight rows: 12 warps 49.6 us, 11 51.1, 10 54.4, 8 47.0.
@@ -220,7 +221,6 @@ decode_kernel(const AttnParams p, bool whole) {
   float2 l[NT], shift[NT];                                   // P = 2^(score + shift); kNone: no key so far
   const Masks km = masks();
   float O[NT][8][4], Ls[NT][4];
-  float vback = 1.f;                                         // V scales are taken times this power of two
   int lim0 = 0;                                              // keys that the run's first token sees
   auto ask_q = [&](const Request& q, int nt) {
     const int n = 8 * nt + g, i = token_of(p, n);
@@ -271,17 +271,16 @@ decode_kernel(const AttnParams p, bool whole) {
       fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
     }
   };
-  // The run's rows so far: the 8 of the codes taken off, the powers of two put back.  To the output (piece == nullptr) or as a piece.
+  // The run's rows so far: the 8 of the codes taken off, their powers of two put back.  To the output (piece == nullptr) or as a piece.
   auto finish = [&](float* piece, int at_piece, const Request& q) {
     const int rows = q.nq * p.G;
-    const float back = 1.f / vback;                          // a power of two, exact
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float ls[2] = {over_g(l[nt].x, false), over_g(l[nt].y, false)};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int n = 8 * nt + 2 * t4 + j;
-        const float f = piece ? back : ls[j] == 0.f ? 0.f : back / ls[j], eight = -8.f * Ls[nt][j] * f, f24 = f * 0x1p24f, f20 = f * 0x1p20f;
+        const float f = piece ? 1.f : ls[j] == 0.f ? 0.f : 1.f / ls[j], eight = -8.f * Ls[nt][j] * f, f24 = f * 0x1p24f, f20 = f * 0x1p20f;
         float v[16];
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
@@ -368,10 +367,9 @@ decode_kernel(const AttnParams p, bool whole) {
               if (!here || tok >= lim0 + min(token_of(p, 8 * nt + 2 * t4 + j), q.nq - 1)) S[nt][cb][2 * i + j] = -INFINITY;
         }
     }
-    // P against the references as they stand: a row's reference maximum, the power of two of the V scales.  Nothing is compared
-    // beforehand: a term that fp16 could not hold shows in the sum of the terms.  Only then the maxima are taken, the references
-    // move and the unit's P is formed again.  A run's first unit is tried with a reference of 2^kFirst and scales as they are, which fits
-    // if every row's sum comes out large enough for fp16's lower end, too.
+    // P v_scale against the rows' references as they stand.  Nothing is compared beforehand: a term that fp16 could not hold shows
+    // in the sum of the terms.  Only then the maxima are taken, the references move and the unit's P is formed again.  A run's first unit is
+    // tried with a reference of kFirst, which fits if every row's sum comes out large enough for fp16's lower end, too.
     uint32_t P[NT][2][2];
     float2 le[NT];
     auto form = [&](bool first) {                            // true where the references do not fit
@@ -388,8 +386,7 @@ decode_kernel(const AttnParams p, bool whole) {
             const float2 y = fadd2(make_float2(S[nt][cb][2 * i], S[nt][cb][2 * i + 1]), shift[nt]);
             const float2 e = make_float2(ex2f(y.x), ex2f(y.y));
             le[nt] = fadd2(le[nt], e);
-            const float sv = vs[cb][i] * vback;
-            const float2 pv = fmul2(e, make_float2(sv, sv));
+            const float2 pv = fmul2(e, make_float2(vs[cb][i], vs[cb][i]));
             sum = fadd2(sum, pv);
             const __half2 hh = __floats2half2_rn(pv.x, pv.y);
             P[nt][cb][i] = *reinterpret_cast<const uint32_t*>(&hh);
@@ -412,24 +409,24 @@ decode_kernel(const AttnParams p, bool whole) {
         for (int i = 0; i < ahead; ++i)
           mbar_wait_bounded(bar + (slot + i >= kSlots ? slot + i - kSlots : slot + i), slot + i >= kSlots ? parity ^ 1u : parity, 1u << 16);
       }
-      const float vtop = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])), 0.f);
-      // 2^-e for the largest scale's power of two e, kept in the range of normal numbers; smaller than before unless nothing was before
-      const int e = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23), 1), 253);
-      const float nb = __uint_as_float((uint32_t)(254 - e) << 23), vnew = fresh ? nb : fminf(vback, nb), vscale = fresh ? 0.f : vnew / vback;
-      vback = vnew;
+      float ve[2][2];                                        // exponents of the V scales; a row that was never written (0) counts like the least scale
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ve[cb][i] = (float)((int)max(__float_as_uint(vs[cb][i]) >> 23, 127u - 17u) - 127);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float x0 = over_g(fmaxf(fmaxf(S[nt][0][0], S[nt][0][2]), fmaxf(S[nt][1][0], S[nt][1][2])), true);
-        const float x1 = over_g(fmaxf(fmaxf(S[nt][0][1], S[nt][0][3]), fmaxf(S[nt][1][1], S[nt][1][3])), true);
+        auto top = [&](int j) {
+          return over_g(fmaxf(fmaxf(S[nt][0][j] + ve[0][0], S[nt][0][2 + j] + ve[0][1]), fmaxf(S[nt][1][j] + ve[1][0], S[nt][1][2 + j] + ve[1][1])), true);
+        };
         // the reference rises to the maximum, or falls to it if there was none; P so far is of 2^(new - old)
         const float2 old = fresh ? make_float2(kNone, kNone) : shift[nt];
-        const float2 ns = make_float2(fminf(old.x, kShift - x0), fminf(old.y, kShift - x1));
+        const float2 ns = make_float2(fminf(old.x, kShift - top(0)), fminf(old.y, kShift - top(1)));
         const float2 al = make_float2(old.x == kNone ? 0.f : ex2f(ns.x - old.x), old.y == kNone ? 0.f : ex2f(ns.y - old.y));
         l[nt] = fmul2(l[nt], al);
-        const float2 av = make_float2(al.x * vscale, al.y * vscale);
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) { O[nt][mt][0] *= av.x; O[nt][mt][1] *= av.y; O[nt][mt][2] *= av.x; O[nt][mt][3] *= av.y; }
-        Ls[nt][0] *= av.x; Ls[nt][1] *= av.y; Ls[nt][2] *= av.x; Ls[nt][3] *= av.y;
+        for (int mt = 0; mt < 8; ++mt) { O[nt][mt][0] *= al.x; O[nt][mt][1] *= al.y; O[nt][mt][2] *= al.x; O[nt][mt][3] *= al.y; }
+        Ls[nt][0] *= al.x; Ls[nt][1] *= al.y; Ls[nt][2] *= al.x; Ls[nt][3] *= al.y;
         shift[nt] = ns;
       }
       form(false);
@@ -487,7 +484,6 @@ decode_kernel(const AttnParams p, bool whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) O[nt][mt][i] = 0.f;
     }
-    vback = 1.f;
     const int n = min(c.units - c.u, left);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {

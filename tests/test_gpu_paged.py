@@ -554,3 +554,32 @@ def test_shared_query_tiles_of_odd_numbers_of_rows(heads, new):
     q, pages, table, cu = make(lens, new, *heads, 64, torch.bfloat16, seed=sum(new))
     got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
     verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("L,at,heads,n", [(40, 0, 4, 1), (600, 0, 4, 1), (600, 599, 8, 1), (20000, 7000, 4, 1), (600, 300, 16, 1), (9000, 64, 16, 1),
+                                          (600, 0, 4, 4), (600, 31, 4, 70)])
+def test_a_heavy_key_with_a_small_value(L, at, heads, n, dtype):
+    """One key has all the weight and values 2^-28 of the others': its own precision counts, not that of the largest value.
+
+    The row is that key's value, so the others' share is left out of the bound but for what they may come to: 2^-40 of it (asserted).
+    The key's own term: P~ to fp16 2^-11, 2^-16 for exponential, sums and quotient, 2^-13 p v_scale for codes below the normal
+    numbers (as in `attention`), half a step of the output.  The others' terms, nearest fp16 numbers of almost nothing: 2^-25 each in units of
+    which the largest term is 8 at least, times a nibble of 15 at most."""
+    g = torch.Generator(device=DEV).manual_seed(L + heads)
+    q = torch.randn(1, 1, 128, generator=g, device=DEV).to(dtype).expand(n, heads, 128).contiguous()
+    k = torch.randn(L, 1, 128, generator=g, device=DEV) * 0.3
+    v = torch.randn(L, 1, 128, generator=g, device=DEV) * 20000
+    k[at, 0], v[at] = 8 * q[0, 0].float(), v[at] * (1e-4 / 20000)
+    pages, slots = hq.paged_pages(-(-L // 64), 1, 64), torch.arange(L, device=DEV)
+    plain.store(pages, slots, k, v)
+    table = torch.arange(-(-L // 64), device=DEV, dtype=torch.int32)[None]
+    got = hq.paged_attention(q, pages, table, ints([L]), cu_q=ints([0, n]), max_q_len=n).double()
+    kk, vv = plain.values(pages, slots)
+    s = (kk[:, 0] @ q[0, 0].double()) * 128 ** -0.5
+    p = torch.softmax(s, 0)
+    want, vs = p @ vv[:, 0], plain.scales(pages, slots)[at, 0]
+    assert p[at] > 0.999 and ((p @ vv[:, 0].abs()) - p[at] * vv[at, 0].abs() <= 2.0 ** -40 * vs).all()
+    eps = torch.finfo(dtype).eps / 2
+    tol = (eps * 1.01 + 2.0 ** -11 + 2.0 ** -16) * want.abs() + (2.0 ** -13 + 15 * L * 2.0 ** -28) * vs + torch.finfo(dtype).smallest_normal * eps
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
