@@ -18,8 +18,12 @@
 // Per warp a ring of three units in shared memory, each one bulk copy (two for pages of sixteen tokens).  Products on mma.sync
 // m16n8k16 in fp16: S^T = K Q^T, tokens on M and the rows (token, head of the group) on N, then O^T = V^T P^T.  Codes enter as fp16
 // subnormals (one logic operation for two of them): the nibble + 8 as mantissa bits is (code + 8) 2^-24, or 2^-20 for a nibble four
-// bits up.  The power of two goes into the query operand and the epilogue, the 8 into the accumulators' start (K) and the row sum
-// of P (V, one more product against ones).  Queries are scaled by a power of two of their own so that fp16 holds them
+// bits up.  The power of two goes into the query operand and the epilogue, the 8 into the accumulators' start (K) and a row sum
+// of P (V, one more product).  The tensor core cuts what does not fit 24 bits beside its largest term off towards zero, and all terms of
+// P (code + 8) are positive: summed in its accumulators over a part's length they came out 1.2e-5 v_scale too small for 16 requests of 32768
+// tokens, 3e-5 for 64 of 16384, where flat attention is 0.02 of it.  So a unit's products start at zero and are added outside, rounded
+// to nearest, and the row sum is formed of eights of the codes' own two kinds, which lose what they lose: the errors are those of
+// P's and the output's rounding now, at every length (batch 16: 60.2 -> 61.2 us, sixteen rows 47.5 -> 49.1).  Queries are scaled by a power of two of their own so that fp16 holds them
 // exactly.  P v_scale is rounded to fp16, 11 bits against bf16's 8, relative to the row's largest product so far: a row's one reference is
 // the maximum of score and log2 of v_scale together, so that a key with all the weight and a small value keeps its bits beside large
 // values without weight.  The row sum of P, in 32 bits, is relative to it too.
@@ -42,6 +46,10 @@ __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void add4(float (&a)[4], const float (&b)[4]) {
+  const float2 x = fadd2(make_float2(a[0], a[1]), make_float2(b[0], b[1])), y = fadd2(make_float2(a[2], a[3]), make_float2(b[2], b[3]));
+  a[0] = x.x; a[1] = x.y; a[2] = y.x; a[3] = y.y;
 }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
@@ -280,12 +288,12 @@ decode_kernel(const AttnParams p, bool whole) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int n = 8 * nt + 2 * t4 + j;
-        const float f = piece ? 1.f : ls[j] == 0.f ? 0.f : 1.f / ls[j], eight = -8.f * Ls[nt][j] * f, f24 = f * 0x1p24f, f20 = f * 0x1p20f;
+        const float f = piece ? 1.f : ls[j] == 0.f ? 0.f : 1.f / ls[j], f24 = f * 0x1p24f, f20 = f * 0x1p20f, eight = -Ls[nt][j] * f24, eight20 = -Ls[nt][2 + j] * f20;
         float v[16];
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          v[4 * q4] = fmaf(O[nt][2 * q4][j], f24, eight); v[4 * q4 + 1] = fmaf(O[nt][2 * q4 + 1][j], f20, eight);
-          v[4 * q4 + 2] = fmaf(O[nt][2 * q4][2 + j], f24, eight); v[4 * q4 + 3] = fmaf(O[nt][2 * q4 + 1][2 + j], f20, eight);
+          v[4 * q4] = fmaf(O[nt][2 * q4][j], f24, eight); v[4 * q4 + 1] = fmaf(O[nt][2 * q4 + 1][j], f20, eight20);
+          v[4 * q4 + 2] = fmaf(O[nt][2 * q4][2 + j], f24, eight); v[4 * q4 + 3] = fmaf(O[nt][2 * q4 + 1][2 + j], f20, eight20);
         }
         if (n >= rows) continue;
         if (piece) {
@@ -441,25 +449,42 @@ decode_kernel(const AttnParams p, bool whole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) l[nt] = make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000));
     }
+    uint2 vw[2][4];
 #pragma unroll
-    for (int cb = 0; cb < 2; ++cb) {
-      const uint8_t* b = u0 + cb * kBlockBytes + kVOff + 8 * g;
-      const uint2 v0 = *reinterpret_cast<const uint2*>(b + t4 * 64), v1 = *reinterpret_cast<const uint2*>(b + (t4 + 4) * 64);
-      const uint2 v2 = *reinterpret_cast<const uint2*>(b + (t4 + 8) * 64), v3 = *reinterpret_cast<const uint2*>(b + (t4 + 12) * 64);
+    for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {                       // channels 16 g + 4 q4 .. + 3: a 16-bit half of each token's word
-        const uint32_t sel = q4 & 1 ? 0x7632u : 0x5410u;
+      for (int i = 0; i < 4; ++i) vw[cb][i] = *reinterpret_cast<const uint2*>(u0 + cb * kBlockBytes + kVOff + 8 * g + (t4 + 4 * i) * 64);
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {                         // channels 16 g + 4 q4 .. + 3: a 16-bit half of each token's word
+      const uint32_t sel = q4 & 1 ? 0x7632u : 0x5410u;
+      float d[NT][2][4];                                     // the unit's own products
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
         uint32_t ha[4], hb[4];
-        nibbles(km, prmt(q4 < 2 ? v0.x : v0.y, q4 < 2 ? v1.x : v1.y, sel), ha);
-        nibbles(km, prmt(q4 < 2 ? v2.x : v2.y, q4 < 2 ? v3.x : v3.y, sel), hb);
+        nibbles(km, prmt(q4 < 2 ? vw[cb][0].x : vw[cb][0].y, q4 < 2 ? vw[cb][1].x : vw[cb][1].y, sel), ha);
+        nibbles(km, prmt(q4 < 2 ? vw[cb][2].x : vw[cb][2].y, q4 < 2 ? vw[cb][3].x : vw[cb][3].y, sel), hb);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma16816(O[nt][2 * q4], ha[0], ha[2], hb[0], hb[2], P[nt][cb][0], P[nt][cb][1]);
-          mma16816(O[nt][2 * q4 + 1], ha[1], ha[3], hb[1], hb[3], P[nt][cb][0], P[nt][cb][1]);
+          if (cb == 0) {
+            mma16816_from(d[nt][0], ha[0], ha[2], hb[0], hb[2], P[nt][0][0], P[nt][0][1], make_float2(0.f, 0.f));
+            mma16816_from(d[nt][1], ha[1], ha[3], hb[1], hb[3], P[nt][0][0], P[nt][0][1], make_float2(0.f, 0.f));
+          } else {
+            mma16816(d[nt][0], ha[0], ha[2], hb[0], hb[2], P[nt][1][0], P[nt][1][1]);
+            mma16816(d[nt][1], ha[1], ha[3], hb[1], hb[3], P[nt][1][0], P[nt][1][1]);
+          }
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma16816(Ls[nt], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, P[nt][cb][0], P[nt][cb][1]);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) add4(O[nt][2 * q4 + k], d[nt][k]);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {                        // 8 P in the units of nibbles 0 and 2 (the first two sums), of 1 and 3
+      float d[4];
+      mma16816_from(d, km.lo8, km.hi8, km.lo8, km.hi8, P[nt][0][0], P[nt][0][1], make_float2(0.f, 0.f));
+      mma16816(d, km.lo8, km.hi8, km.lo8, km.hi8, P[nt][1][0], P[nt][1][1]);
+      add4(Ls[nt], d);
     }
     __syncwarp();
     if (++slot == kSlots) { slot = 0; parity ^= 1u; }

@@ -583,3 +583,33 @@ def test_a_heavy_key_with_a_small_value(L, at, heads, n, dtype):
     eps = torch.finfo(dtype).eps / 2
     tol = (eps * 1.01 + 2.0 ** -11 + 2.0 ** -16) * want.abs() + (2.0 ** -13 + 15 * L * 2.0 ** -28) * vs + torch.finfo(dtype).smallest_normal * eps
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("R,L,heads", [(16, 32768, (32, 8)), (64, 16384, (32, 8)), (4, 131072, (32, 2))])
+@pytest.mark.parametrize("spread", [0.3, 1.0])
+def test_long_flat_attention_keeps_its_bits(R, L, heads, spread):
+    """Almost flat scores over long contexts: outputs are small beside the values, and what sums lose in one direction would show.
+
+    fp16 outputs.  What there is to be off by at random: the output's own rounding (taken from the exact output), and P~ v_scale rounded
+    to fp16: at most 2^-11 of a term, 2^-11 / sqrt(3) in the root mean square, terms independent of each other.  Everything else (32-bit
+    sums, exponentials: 2^-23 of terms) is far less, so the whole error's root mean square stays within these two."""
+    g = torch.Generator(device=DEV).manual_seed(R)
+    hq_, H = heads
+    pages, slots = hq.paged_pages(L // 128, H, 128), torch.arange(L, device=DEV)
+    for at in range(0, L, 16384):
+        hq.paged_append(pages, *(torch.randn(16384, H, 128, generator=g, device=DEV) for _ in range(2)), slots[at:at + 16384])
+    table = torch.arange(L // 128, dtype=torch.int32, device=DEV).repeat(R, 1)          # all requests read the same pages
+    q = (torch.randn(R, hq_, 128, generator=g, device=DEV) * spread).to(torch.float16)
+    got = hq.paged_attention(q, pages, table, ints([L] * R)).double()
+    k, v = plain.values(pages, slots)
+    vs = plain.scales(pages, slots)
+    G, off, rounding, terms = hq_ // H, 0.0, 0.0, 0.0
+    for h in range(H):
+        x = q[:, h * G:h * G + G].reshape(R * G, 128).double()
+        p = torch.softmax(x @ k[:, h].T * 128 ** -0.5, -1)
+        unit = (p @ vs[:, h])[:, None]
+        o = p @ v[:, h]
+        off += ((got[:, h * G:h * G + G].reshape(R * G, 128) - o) / unit).square().mean().item() / H
+        rounding += ((o.to(torch.float16).double() - o) / unit).square().mean().item() / H
+        terms += ((p.square() @ v[:, h].square()) / unit.square()).mean().item() / H
+    assert off <= rounding + terms * 2.0 ** -22 / 3, (off ** 0.5, rounding ** 0.5, terms ** 0.5)
