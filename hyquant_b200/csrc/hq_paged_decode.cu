@@ -275,7 +275,8 @@ decode_kernel(const AttnParams p, bool whole) {
       for (int w = 0; w < 8; ++w) mma16816(zero, km.lo8, km.lo8, km.hi8, km.hi8, qf[nt][2 * w], qf[nt][2 * w + 1]);
       start[nt] = make_float2(-zero[0], -zero[1]);
       shift[nt] = make_float2(kShift - kFirst, kShift - kFirst);
-      const float back = p.sml * __uint_as_float((uint32_t)min(127 + 24 - up, 255) << 23);       // sml 2^24 / scale
+      // sml 2^24 / scale.  Where that is no number (queries from 2^117 on) the largest one serves: scores are 2^60 apart then, or equal.
+      const float back = fminf(p.sml * __uint_as_float((uint32_t)min(127 + 24 - up, 254) << 23), 0x1.fffffep127f);
       fac[nt] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t4), __shfl_sync(0xffffffffu, back, 8 * t4 + 4));
     }
   };

@@ -613,3 +613,33 @@ def test_long_flat_attention_keeps_its_bits(R, L, heads, spread):
         rounding += ((o.to(torch.float16).double() - o) / unit).square().mean().item() / H
         terms += ((p.square() @ v[:, h].square()) / unit.square()).mean().item() / H
     assert off <= rounding + terms * 2.0 ** -22 / 3, (off ** 0.5, rounding ** 0.5, terms ** 0.5)
+
+
+@pytest.mark.parametrize("power", [60, 116, 117, 121, 127])
+@pytest.mark.parametrize("new", [1, 3])
+def test_queries_near_the_end_of_bf16(power, new):
+    """Finite queries whose scores are so far apart that a row is the value of the keys with the largest one, and no other row is touched.
+    The bound of such a row is that of its terms: P~ to fp16 2^-11, 2^-16 for the sums and the quotient, 2^-13 of a V scale, half a
+    step of the output."""
+    L = 300
+    g = torch.Generator(device=DEV).manual_seed(power)
+    k, v = (torch.randn(L, 1, 128, generator=g, device=DEV) for _ in range(2))
+    k *= 0.1
+    k[:, 0, 3] = 0.7 + 0.7 * torch.randperm(L, generator=g, device=DEV) / L                 # a row's largest: code 7 times its scale
+    pages, slots = hq.paged_pages(5, 1, 64), torch.arange(L, device=DEV)
+    plain.store(pages, slots, k, v)
+    table = torch.arange(5, dtype=torch.int32, device=DEV)[None]
+    q = torch.randn(new, 4, 128, generator=g, device=DEV).to(torch.bfloat16)
+    q[:, 1] = 0.0
+    q[:, 1, 3] = 2.0 ** power if power < 127 else 3e38
+    got = hq.paged_attention(q, pages, table, ints([L]), cu_q=ints([0, new]), max_q_len=new).double()
+    want, tol = plain.attention(q, pages, table, [L], [0, new])
+    kk, vv = plain.values(pages, slots)
+    vs = plain.scales(pages, slots)[:, 0]
+    for i in range(new):
+        n = L - new + 1 + i
+        top = kk[:n, 0, 3] == kk[:n, 0, 3].max()
+        p = top.double() / top.sum()
+        assert (want[i, 1] - p @ vv[:n, 0]).abs().max() < 1e-12
+        tol[i, 1] = (torch.finfo(torch.bfloat16).eps / 2 * 1.01 + 2.0 ** -11 + 2.0 ** -16) * (p @ vv[:n, 0].abs()) + 2.0 ** -13 * (p @ vs[:n])
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
