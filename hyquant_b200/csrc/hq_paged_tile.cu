@@ -35,6 +35,7 @@ constexpr int kKStages = 3, kVStages = 4;        // K tiles and V tiles in share
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
+constexpr float kTFar = 8192.0f;                 // scores (log2) up to which a rounded reference will do: it is off by 2^-12 of a power of two at most
 constexpr uint32_t kTPolls = 400000u;
 
 struct TileSmem {
@@ -106,9 +107,10 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 
 struct SlowState { float m, l; bool ok; };
 
-// A tile that needs masks or a new reference: the scores are read again, the maximum taken, O rescaled where a row's reference
+// A tile that needs masks or a new reference: the products are read again, the maximum taken, O rescaled where a row's reference
 // moves (where the maximum passes it by `slack`), P formed.  `lim`: keys of the tile that the row sees; bad: blocks of sixteen keys that are
-// not there.
+// not there.  A row's reference m is a product of the tensor core, its score m f.  Differences are taken before the factor here: equal scores
+// have equal weights, whatever their size.
 __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, int lim, uint32_t bad, float slack, float m, float l,
                                             uint64_t* pv_bar, uint32_t pv_parity, volatile int* abort_flag) {
   SlowState out{m, l, true};
@@ -128,11 +130,11 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
     tc::tmem_wait_ld();
     const uint32_t mask = c ? see[1] : see[0];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (mask >> e) & 1u ? x[e] * f : -INFINITY);
+    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, (mask >> e) & 1u ? x[e] : -INFINITY);
   }
-  const bool grow = mx > m + slack;
+  const bool grow = m == -INFINITY ? mx > m : (mx - m) * f > slack;
   if (__any_sync(0xffffffffu, grow)) {
-    const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2f(m - mx);
+    const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2f((m - mx) * f);
     if (pv_bar != nullptr) {                     // O must be quiescent
       if (!wait_warp(pv_bar, pv_parity, abort_flag)) { out.ok = false; return out; }
       tc::fence_after_sync();
@@ -150,7 +152,7 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
     out.l *= alpha;
     if (grow) out.m = mx;
   }
-  const float shift = out.m == -INFINITY ? 0.f : kTShift - out.m;
+  const float base = out.m == -INFINITY ? 0.f : out.m;
   float sum = 0.f;
 #pragma unroll 1
   for (int c = 0; c < 2; ++c) {                  // P of columns 32 c .. lands in columns 16 c .., which have been read
@@ -161,7 +163,7 @@ __device__ __noinline__ SlowState slow_tile(uint32_t tS, uint32_t tO, float f, i
     uint32_t pk[16];
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
-      const float p0 = ex2f(((mask >> e) & 1u ? x[e] * f : -INFINITY) + shift), p1 = ex2f(((mask >> (e + 1)) & 1u ? x[e + 1] * f : -INFINITY) + shift);
+      const float p0 = (mask >> e) & 1u ? ex2f(fmaf(x[e] - base, f, kTShift)) : 0.f, p1 = (mask >> (e + 1)) & 1u ? ex2f(fmaf(x[e + 1] - base, f, kTShift)) : 0.f;
       sum += p0 + p1;
       const __half2 hh = __floats2half2_rn(p0, p1);
       pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&hh);
@@ -478,7 +480,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
         };
         const float top = value(max(top2 & 0xFFFFu, top2 >> 16), 0);
         const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 255 ? 0 : 140 - max(ex, 14);       // largest magnitude to [2^13, 2^14)
-        const float scale = __uint_as_float((uint32_t)(127 + up) << 23), f = p.sml * __uint_as_float((uint32_t)(127 - up) << 23);
+        const float scale = __uint_as_float((uint32_t)(127 + up) << 23), f = fminf(p.sml * __uint_as_float((uint32_t)(127 - up) << 23), 0x1.fffffep127f);
         const float2 scale2 = make_float2(scale, scale);
 #pragma unroll 4
         for (int c = 0; c < 16; ++c) {
@@ -497,6 +499,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
         tc::mbar_arrive(q_full + half);
         const int lim = r < rows ? min(q.len, q.past + 1 + i) : 0x7FFFFFFF;      // rows that are none see everything: finite, not written
         float shift = INFINITY;
+        bool far = true;                         // no reference yet, or one whose rounding a weight would show: slow_tile
         const float2 f2 = make_float2(f, f);
 #pragma unroll 1
         for (int t = 0; t < n; ++t, ++tile) {
@@ -508,7 +511,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
           const int at = first + step * t;
           const uint32_t bad = bads[(all + (uint32_t)at) & 15u];
           const int see = lim - (pc.t0 + at) * kKeys;
-          const bool masks = __any_sync(0xffffffffu, see < kKeys || bad != 0u);
+          const bool masks = __any_sync(0xffffffffu, see < kKeys || bad != 0u || far);
           bool need = false;
           uint32_t pk[32];
           float sum = 0.f;
@@ -537,7 +540,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
             ok = x2.ok;
             if (!ok) break;
             m = x2.m; l = x2.l;
-            shift = m == -INFINITY ? INFINITY : kTShift - m;
+            far = m == -INFINITY || fabsf(m) * f > kTFar;
+            shift = kTShift - m * f;
           } else {
             l += sum;
             tc::tmem_st32(tS, pk);
@@ -547,6 +551,7 @@ tile_kernel(const AttnParams p, int piece_rows) {
           tc::mbar_arrive(p_ready + 2 * half + slot);
         }
         if (ok) ok = wait_warp(pv_done + 2 * half + ((tile - 1u) & 1u), ((tile - 1u) >> 1) & 1u, abort_flag);
+        if (m != -INFINITY) m *= f;              // the score, for the other half and other blocks
       }
       all += (uint32_t)n_all;
       if (!ok) { m = 0.f; l = __int_as_float(0x7FC00000); }            // gave up: the rows are NaN

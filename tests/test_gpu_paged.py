@@ -616,7 +616,7 @@ def test_long_flat_attention_keeps_its_bits(R, L, heads, spread):
 
 
 @pytest.mark.parametrize("power", [60, 116, 117, 121, 127])
-@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("new", [1, 3, 70])
 def test_queries_near_the_end_of_bf16(power, new):
     """Finite queries whose scores are so far apart that a row is the value of the keys with the largest one, and no other row is touched.
     The bound of such a row is that of its terms: P~ to fp16 2^-11, 2^-16 for the sums and the quotient, 2^-13 of a V scale, half a
