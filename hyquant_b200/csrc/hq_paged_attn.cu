@@ -12,6 +12,17 @@ static int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 3
 
 static bool few_rows(const hq_paged_attention_args* a) { return (int64_t)a->max_q_len * (a->H_Q / a->H_KV) <= 16; }
 
+// Rows of 128 at i * si + j * sj that share nothing: one index's rows all lie within a step of the other.  (Strides below 2^56: no
+// overflow in what is compared; an index of one value has no stride.)
+static bool rows_apart(int64_t ni, int64_t si, int64_t nj, int64_t sj) {
+  constexpr int64_t kMost = (int64_t)1 << 56;
+  if (ni == 1) si = 128;
+  if (nj == 1) sj = 128;
+  if (si < 128 || sj < 128 || si > kMost || sj > kMost) return false;
+  auto within = [](int64_t n, int64_t s, int64_t step) { return n == 1 || (step - 128) / s >= n - 1; };
+  return ni == 1 || nj == 1 || within(nj, sj, si) || within(ni, si, sj);
+}
+
 static int check(const hq_paged_attention_args* a) {
   HQ_REQUIRE(a != nullptr, HQ_ERR_INVALID, "hq_paged_attention: null argument block");
   HQ_REQUIRE(a->struct_bytes == (int)sizeof(hq_paged_attention_args), HQ_ERR_INVALID, "hq_paged_attention: struct_bytes %d, expected %d",
@@ -42,10 +53,10 @@ static int check(const hq_paged_attention_args* a) {
              "hq_paged_attention: null pointer");
   HQ_REQUIRE(a->table_stride >= a->max_pages, HQ_ERR_INVALID, "hq_paged_attention: table rows of %d pages overlap at stride %lld", a->max_pages,
              (long long)a->table_stride);
-  HQ_REQUIRE((a->T == 1 || a->o_st >= 128) && (a->H_Q == 1 || a->o_sh >= 128), HQ_ERR_INVALID,
-             "hq_paged_attention: rows of out overlap at strides %lld and %lld", (long long)a->o_st, (long long)a->o_sh);
   HQ_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->pages) && (a->q_st | a->q_sh | a->o_st | a->o_sh) % 8 == 0, HQ_ERR_ALIGNMENT,
              "hq_paged_attention: q, out and pages must be 16-byte aligned, strides multiples of 8 elements");
+  HQ_REQUIRE(rows_apart(a->T, a->o_st, a->H_Q, a->o_sh), HQ_ERR_INVALID, "hq_paged_attention: rows of out overlap at strides %lld and %lld",
+             (long long)a->o_st, (long long)a->o_sh);
   return HQ_OK;
 }
 

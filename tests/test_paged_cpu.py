@@ -170,7 +170,7 @@ def test_pieces_of_query_tiles_begin_on_16_bytes():
     lib, n = _lib.lib(), C.c_int64()
 
     def workspace(G, most):
-        a = attention_args(H_Q=G, H_KV=1, max_q_len=most)
+        a = attention_args(H_Q=G, H_KV=1, max_q_len=most, o_st=G * 128)
         assert lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n)) == 0
         return n.value
     full = 2 * 256 * 130 * 4 + 32
@@ -180,3 +180,21 @@ def test_pieces_of_query_tiles_begin_on_16_bytes():
         for most in range(16 // G + 1, 260):
             per, rest = divmod(workspace(G, most), blocks)
             assert rest == 0 and (per - 32) % 32 == 0 and (per - 32) // 2 >= min(256, most * G) * 130 * 4, (G, most)
+
+
+@pytest.mark.parametrize("fields,apart", [
+    (dict(), True), (dict(o_st=128, o_sh=128), False), (dict(o_st=512, o_sh=128), False), (dict(o_st=1016, o_sh=128), False), (dict(o_st=128, o_sh=640), True),
+    (dict(o_st=128, o_sh=632), False), (dict(o_st=136, o_sh=672), True), (dict(o_st=136, o_sh=664), False), (dict(o_st=1080, o_sh=136), True),
+    (dict(o_st=1072, o_sh=136), False), (dict(T=1, R=1, o_st=0, o_sh=128), True), (dict(T=1, R=1, o_st=0, o_sh=120), False),
+    (dict(H_Q=1, H_KV=1, o_sh=0, o_st=128), True), (dict(H_Q=1, H_KV=1, o_sh=0, o_st=120), False), (dict(o_st=-1024), False), (dict(o_sh=-128), False),
+    (dict(o_st=1 << 60, o_sh=1 << 58), False), (dict(o_st=1 << 40), True)])
+def test_rows_of_the_output_lie_apart(fields, apart):
+    """Five tokens of eight heads: every pair of strides that puts two rows on the same elements is refused."""
+    lib, n = _lib.lib(), C.c_int64()
+    a = attention_args(**fields)
+    rc = lib.hq_paged_attention_workspace_bytes(C.byref(a), C.byref(n))
+    assert rc == 0 if apart else rc == -1 and b"overlap" in lib.hq_last_error()
+    if abs(a.o_st) < 1 << 20 and abs(a.o_sh) < 1 << 20:
+        at = [t * a.o_st + h * a.o_sh + c for t in range(a.T) for h in range(a.H_Q) for c in range(128)]
+        assert not apart or len(set(at)) == len(at)
+        assert apart or len(set(at)) < len(at) or min(at) < 0
