@@ -53,7 +53,8 @@ static int check(const hq_paged_attention_args* a) {
              "hq_paged_attention: null pointer");
   HQ_REQUIRE(a->table_stride >= a->max_pages, HQ_ERR_INVALID, "hq_paged_attention: table rows of %d pages overlap at stride %lld", a->max_pages,
              (long long)a->table_stride);
-  HQ_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->pages) && (a->q_st | a->q_sh | a->o_st | a->o_sh) % 8 == 0, HQ_ERR_ALIGNMENT,
+  const int64_t strides = (a->T > 1 ? a->q_st | a->o_st : 0) | (a->H_Q > 1 ? a->q_sh | a->o_sh : 0);
+  HQ_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->pages) && strides % 8 == 0, HQ_ERR_ALIGNMENT,
              "hq_paged_attention: q, out and pages must be 16-byte aligned, strides multiples of 8 elements");
   HQ_REQUIRE(rows_apart(a->T, a->o_st, a->H_Q, a->o_sh), HQ_ERR_INVALID, "hq_paged_attention: rows of out overlap at strides %lld and %lld",
              (long long)a->o_st, (long long)a->o_sh);

@@ -171,8 +171,12 @@ def _rows(x: torch.Tensor):
     address = x.data_ptr()
     if sd == 1 and not (st | sh) & 7 and not address & 15:
         return x, address, st, sh
-    x = x.contiguous()
-    return x, x.data_ptr(), x.stride(0), x.stride(1)
+    T, H, _ = x.shape
+    st, sh = st if T > 1 else 0, sh if H > 1 else 0                        # an index of one value has no stride
+    if sd != 1 or (st | sh) & 7 or address & 15:
+        x = x.clone(memory_format=torch.contiguous_format)                 # (contiguous() would give back one that lies at an odd offset)
+        address, st, sh = x.data_ptr(), H * 128, 128
+    return x, address, st, sh
 
 
 def paged_read(pages: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:

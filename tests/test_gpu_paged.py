@@ -643,3 +643,24 @@ def test_queries_near_the_end_of_bf16(power, new):
         assert (want[i, 1] - p @ vv[:n, 0]).abs().max() < 1e-12
         tol[i, 1] = (torch.finfo(torch.bfloat16).eps / 2 * 1.01 + 2.0 ** -11 + 2.0 ** -16) * (p @ vv[:n, 0].abs()) + 2.0 ** -13 * (p @ vs[:n])
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+def test_contiguous_rows_at_an_odd_offset():
+    """Contiguous views that begin off 16 bytes, and single rows with strides of any number: as copies of them."""
+    lens, new = [250, 131], [30, 90]
+    q, pages, table, cu = make(lens, new, 8, 2, 64, torch.float16, seed=37)
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape)
+    odd.copy_(q)
+    want = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=90)
+    assert torch.equal(hq.paged_attention(odd, pages, table, ints(lens), cu_q=ints(cu), max_q_len=90), want)
+    one, room = (torch.zeros(2, 1200, dtype=q.dtype, device=DEV).as_strided((1, 8, 128), (1197, 128, 1)) for _ in range(2))
+    one.copy_(q[:1])
+    want = hq.paged_attention(q[:1].clone(), pages, table[:1], ints(lens[:1]))
+    assert torch.equal(hq.paged_attention(one, pages, table[:1], ints(lens[:1]), out=room), want) and torch.equal(room, want)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.randn(5 * 2 * 128 + 1, device=DEV).to(dtype)[1:].view(5, 2, 128)
+        pages, expect = hq.paged_pages(2, 2, 16), hq.paged_pages(2, 2, 16)
+        slots = torch.arange(5, device=DEV)
+        hq.paged_append(pages, x, x, slots)
+        plain.store(expect, slots, x, x)
+        assert torch.equal(pages, expect)

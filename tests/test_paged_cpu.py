@@ -198,3 +198,27 @@ def test_rows_of_the_output_lie_apart(fields, apart):
         at = [t * a.o_st + h * a.o_sh + c for t in range(a.T) for h in range(a.H_Q) for c in range(128)]
         assert not apart or len(set(at)) == len(at)
         assert apart or len(set(at)) < len(at) or min(at) < 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,H,offset,st,sh,copied", [
+    (5, 2, 0, 256, 128, False), (5, 2, 1, 256, 128, True), (5, 2, 4, 256, 128, None), (5, 2, 8, 256, 128, False), (5, 2, 0, 257, 128, True), (5, 2, 0, 384, 132, True),
+    (5, 2, 0, 0, 128, False), (1, 2, 0, 257, 128, False), (1, 2, 3, 257, 128, True), (5, 1, 0, 136, 3, False), (1, 1, 0, 7, 5, False), (1, 1, 1, 7, 5, True),
+    (0, 2, 1, 256, 128, None)])
+def test_rows_the_kernels_cannot_read_as_they_lie_are_copied(T, H, offset, st, sh, copied, dtype):
+    """Views at every offset and with every stride, contiguous ones at an odd offset among them; an index of one value has no stride."""
+    flat = torch.arange(3000, dtype=torch.float32).remainder(251).to(dtype)
+    x = flat.as_strided((T, H, 128), (st, sh, 1), offset)
+    y, address, y_st, y_sh = paged_kv._rows(x)
+    assert address == y.data_ptr() and address % 16 == 0 and (y_st | y_sh) % 8 == 0
+    assert torch.equal(y, x) and (copied is None or (y is not x) == copied)
+    size = y.element_size()
+    for t in range(T):
+        for h in range(H):
+            assert address + (t * y_st + h * y_sh) * size == y[t, h].data_ptr()
+
+
+def test_strides_of_a_single_token_and_of_a_single_head_do_not_count():
+    lib, n = _lib.lib(), C.c_int64()
+    for fields in (dict(T=1, R=1, q_st=3, o_st=5), dict(H_Q=1, H_KV=1, q_sh=1, o_sh=1, q_st=128, o_st=128)):
+        assert lib.hq_paged_attention_workspace_bytes(C.byref(attention_args(**fields)), C.byref(n)) == 0
