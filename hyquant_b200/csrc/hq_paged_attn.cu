@@ -56,6 +56,8 @@ static int check(const hq_paged_attention_args* a) {
   const int64_t strides = (a->T > 1 ? a->q_st | a->o_st : 0) | (a->H_Q > 1 ? a->q_sh | a->o_sh : 0);
   HQ_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->pages) && strides % 8 == 0, HQ_ERR_ALIGNMENT,
              "hq_paged_attention: q, out and pages must be 16-byte aligned, strides multiples of 8 elements");
+  HQ_REQUIRE(((uintptr_t)a->page_table | (uintptr_t)a->kv_lens | (uintptr_t)a->cu_q) % 4 == 0, HQ_ERR_ALIGNMENT,
+             "hq_paged_attention: page_table, kv_lens and cu_q must be 4-byte aligned");
   HQ_REQUIRE(rows_apart(a->T, a->o_st, a->H_Q, a->o_sh), HQ_ERR_INVALID, "hq_paged_attention: rows of out overlap at strides %lld and %lld",
              (long long)a->o_st, (long long)a->o_sh);
   return HQ_OK;

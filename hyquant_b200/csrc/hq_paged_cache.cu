@@ -330,6 +330,10 @@ extern "C" int hq_page_advance(const hq_page_advance_args* a, void* stream) {
   HQ_REQUIRE((int64_t)a->R * a->max_pages <= 0x7FFFFFFF, HQ_ERR_UNSUPPORTED, "hq_page_advance: %d requests of %d pages", a->R, a->max_pages);
   HQ_REQUIRE(a->table_stride >= a->max_pages, HQ_ERR_INVALID, "hq_page_advance: table rows of %d pages overlap at stride %lld", a->max_pages,
              (long long)a->table_stride);
+  const auto bits = [](auto*... p) { return (... | (uintptr_t)p); };
+  HQ_REQUIRE(bits(a->kv_lens, a->held, a->add, a->keep, a->page_table, a->free_pages, a->free_count, a->kv_lens_out, a->held_out, a->free_count_out,
+                  a->cu_q, a->positions, a->status) % 4 == 0 && (uintptr_t)a->slots % 8 == 0, HQ_ERR_ALIGNMENT,
+             "hq_page_advance: slots must be 8-byte, the other arrays 4-byte aligned");
   const AdvanceParams p{a->kv_lens, a->held, a->add, a->keep, a->R, a->page_table, a->table_stride, a->max_pages, a->free_pages, a->free_cap,
                         a->free_count, shift_of(a->page_size), a->T, a->kv_lens_out, a->held_out, a->free_count_out, a->cu_q, a->slots,
                         a->positions, a->status};

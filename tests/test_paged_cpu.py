@@ -222,3 +222,14 @@ def test_strides_of_a_single_token_and_of_a_single_head_do_not_count():
     lib, n = _lib.lib(), C.c_int64()
     for fields in (dict(T=1, R=1, q_st=3, o_st=5), dict(H_Q=1, H_KV=1, q_sh=1, o_sh=1, q_st=128, o_st=128)):
         assert lib.hq_paged_attention_workspace_bytes(C.byref(attention_args(**fields)), C.byref(n)) == 0
+
+
+@pytest.mark.parametrize("name", [n for n, kind in _lib.PageAdvanceArgs._fields_ if kind is C.c_void_p])
+def test_advance_refuses_misaligned_arrays(name):
+    assert advance(**{name: FAKE + (4 if name == "slots" else 2)}) == -3 and b"aligned" in _lib.lib().hq_last_error()
+
+
+@pytest.mark.parametrize("name", ["page_table", "kv_lens", "cu_q"])
+def test_attention_refuses_misaligned_arrays(name):
+    a = attention_args(**{name: FAKE + 2})
+    assert _lib.lib().hq_paged_attention(C.byref(a), None) == -3 and b"aligned" in _lib.lib().hq_last_error()
