@@ -53,8 +53,8 @@ advance_kernel(const AdvanceParams p, int blocks) {
   const int page = 1 << p.page_shift;
   const bool cluster = blocks > 1;
   if (tid == 0) s_bad = 0;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
   const int free_count = *p.free_count;
   const int per = (R + kAdvThreads - 1) / kAdvThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
@@ -290,8 +290,9 @@ read_kernel(const uint8_t* __restrict__ pages, int64_t num_slots, int page_shift
 static int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
 
 // A launch that the kernel before it in the stream lets begin early: the kernels wait for it (griddepcontrol.wait) before they touch
-// memory, but their launch is over by then (rows of 16 tokens in and out 3.8 -> 3.4 us).  Only page_advance lets the next one begin
-// early in turn: blocks of read_kernel that wait beside append_kernel's took 29.3 us for a prompt's rows, not 24.8.
+// memory, but their launch is over by then (rows of 16 tokens in and out 3.8 -> 3.4 us).  Of these only page_advance lets the next one
+// begin early in turn, as attention does, and behind its own wait: what comes next may rely on every kernel but the one just before it
+// (hq_decode_splitk does, which fetches older rows of its cache at once).  Blocks of read_kernel that wait beside append_kernel's took 29.3 us for a prompt's rows, not 24.8.
 template <typename... P, typename... A>
 static cudaError_t launch_early(void (*kernel)(P...), int grid, int cluster, int threads, int smem, cudaStream_t st, A... a) {
   cudaLaunchAttribute attr[2]{};

@@ -148,8 +148,8 @@ decode_kernel(const AttnParams p, bool whole) {
   __shared__ float s_max[8 * NT][32], s_sum[8 * NT][32];     // (log2) maximum and sum of a piece's rows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   if (tid < kWarps * kSlots) { mbar_init(bars + tid, 1); fence_mbar_init(); }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- where this warp's part lies
   const int block = blockIdx.x;

@@ -213,8 +213,8 @@ tile_kernel(const AttnParams p, int piece_rows) {
     __syncwarp();
     tc::tmem_alloc(tmem_slot, 512);
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- where this block's part lies
   auto weight = [&](const Request& q) {

@@ -664,3 +664,39 @@ def test_contiguous_rows_at_an_odd_offset():
         hq.paged_append(pages, x, x, slots)
         plain.store(expect, slots, x, x)
         assert torch.equal(pages, expect)
+
+
+@pytest.mark.parametrize("between", ["advance", "attention", "chunk"])
+def test_an_overlapped_decode_call_behind_a_paged_one(between):
+    """The four-segment decode call may fetch older rows before the kernel just before it has ended.  A paged call there that ended its own
+    wait late would let it begin beside the kernel before that, which writes those rows."""
+    from hyquant_b200.decode_d_stage import DecodePlan, quantize_per_token_into
+    N, H, R = 32768, 8, 4
+    q, pages, table, cu = make([700], [1], 32, 8, 64, torch.bfloat16, seed=3)
+    wide, cu_wide = q.repeat(80, 1, 1), ints([0, 80])
+    lens, zero, free, count = ints([700]), ints([0]), ints([0] * 4), ints([4])
+    g = torch.Generator(device=DEV).manual_seed(8)
+    packed = [torch.zeros(H, N, 64, dtype=torch.int8, device=DEV) for _ in range(2)]
+    scale = [torch.zeros(H, N, dtype=torch.float16, device=DEV) for _ in range(2)]
+    window = torch.randn(2, H, 64, 128, generator=g, device=DEV).to(torch.bfloat16)
+    none = window[0, :, :0]
+    qd = q[0].contiguous()
+
+    def call(overlap):
+        plan = DecodePlan(qd, packed[0], packed[1], scale[0], scale[1], none, none, none, none, window[0], window[1], R, None, overlap_previous=overlap)
+        return plan.run(qd)
+    for _ in range(6):
+        rows = [torch.randn(H, N, 128, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2)]
+        call(False)
+        torch.cuda.synchronize()
+        for x, p, s in zip(rows, packed, scale):
+            quantize_per_token_into(x, p, s, 0, nbits=4)
+        if between == "advance":
+            hq.page_advance(lens, ints([11]), zero, table, free, count, page_size=64, max_tokens=4)
+        elif between == "attention":
+            hq.paged_attention(q, pages, table, lens)
+        else:
+            hq.paged_attention(wide, pages, table, lens, cu_q=cu_wide, max_q_len=80)
+        got = call(True)
+        torch.cuda.synchronize()
+        assert torch.equal(got, call(False))
