@@ -700,3 +700,105 @@ def test_an_overlapped_decode_call_behind_a_paged_one(between):
         got = call(True)
         torch.cuda.synchronize()
         assert torch.equal(got, call(False))
+
+
+@pytest.mark.parametrize("R", [31, 32, 33, 63, 64, 65, 100, 500])
+@pytest.mark.parametrize("kind", ["one", "few", "mixed", "chunks"])
+def test_numbers_of_requests(R, kind):
+    """The ways in which a request is found from a position (up to 32 requests, 64, more) in both forms, requests without tokens or keys
+    among them; one chunk beside many single tokens."""
+    rng = random.Random(R)
+    new = [1] * R if kind == "one" else [rng.choice([0, 1, 2, 4]) for _ in range(R)] if kind == "few" else \
+        [rng.choice([0, 1, 1, 1]) for _ in range(R)] if kind == "mixed" else [rng.choice([0, 1, 7, rng.randint(1, 90)]) for _ in range(R)]
+    if kind == "mixed":
+        new[rng.randrange(R)] = 200
+    most = 4 if kind == "few" else max(new)
+    lens = [rng.choice([0, n, n + rng.randint(0, 40), n + rng.randint(0, 500)]) for n in new]
+    q, pages, table, cu = make(lens, new, 4, 1, 32, torch.float16, seed=R)
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=most)
+    verify(got, q, pages, table, lens, cu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,heads", [(1, 4), (1, 16), (70, 4)])
+@pytest.mark.parametrize("weight", [1.0, 2.0, 4.0])
+@pytest.mark.parametrize("at", [0, 17000])
+def test_terms_that_vanish_beside_a_heavy_key(weight, at, n, heads, dtype):
+    """30000 keys whose scores lie 11, 22 and 45 below one key's: what their terms may be off by is counted term by term.
+
+    A term p v_scale (code + 8) is off by 15 * 2^-28 of the row's largest p v_scale, or by itself if that is less (it becomes 0, or the nearest
+    fp16 number); scores are off by delta as in `attention`, which moves the heavy key's weight by what the others weigh only."""
+    L = 30000
+    g = torch.Generator(device=DEV).manual_seed(int(weight) + at)
+    q = torch.randn(1, 1, 128, generator=g, device=DEV).to(dtype).expand(n, heads, 128).contiguous()
+    k, v = (torch.randn(L, 1, 128, generator=g, device=DEV) for _ in range(2))
+    k *= 0.2
+    k[at, 0] = weight * q[0, 0].float()
+    pages, slots = hq.paged_pages(-(-L // 128), 1, 128), torch.arange(L, device=DEV)
+    plain.store(pages, slots, k, v)
+    table = torch.arange(-(-L // 128), device=DEV, dtype=torch.int32)[None]
+    got = hq.paged_attention(q, pages, table, ints([L]), cu_q=ints([0, n]), max_q_len=n).double()
+    kk, vv = (x[:, 0] for x in plain.values(pages, slots))
+    vs = plain.scales(pages, slots)[:, 0]
+    s, x = (kk @ q[0, 0].double()) * 128 ** -0.5, q[0, 0].double().abs() * 128 ** -0.5
+    delta = 2.0 ** -16 * (kk.abs() @ x).max()
+    eps = torch.finfo(dtype).eps / 2
+    for i in (range(n) if n < 8 else (0, 1, 33, n - 1)):
+        m = L - n + 1 + i
+        p = torch.softmax(s[:m], 0)
+        want = p @ vv[:m]
+        others = p.clone()
+        others[at] = 0
+        tol = eps * 1.01 * want.abs() + (2.0 ** -11 + 2.0 ** -16) * (p @ vv[:m].abs()) + 2.0 ** -13 * (p @ vs[:m]) + \
+            2 * delta * (others @ vv[:m].abs() + others.sum() * vv[at].abs()) + 15 * torch.minimum(p * vs[:m], 2.0 ** -28 * (p * vs[:m]).max()).sum()
+        assert ((got[i] - want).abs() <= tol).all(), float(((got[i] - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("new,most", [([5, 2, 1], 3), ([60, 3, 25], 20), ([400, 1, 300], 130)])
+def test_tokens_beyond_the_most_of_a_request(new, most):
+    """They are not computed; the others see what they see without the limit, and nothing else is written."""
+    lens = [700, 129, 333]
+    q, pages, table, cu = make(lens, new, 8, 2, 32, torch.bfloat16, seed=most)
+    room = torch.full_like(q, 7.0)
+    got = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=most, out=room)
+    want, tol = plain.attention(q, pages, table, lens, cu)
+    for r, n in enumerate(new):
+        first = slice(cu[r], cu[r] + min(n, most))
+        assert ((got[first].double() - want[first]).abs() <= tol[first]).all()
+        assert (got[first.stop:cu[r + 1]] == 7).all()
+
+
+def test_the_other_calls_of_a_refused_step_do_nothing():
+    cache = hq.PagedKVCache(1, 6, 2, max_requests=3, max_pages_per_request=5, page_size=16)
+    k = torch.randn(90, 2, 128, device=DEV).to(torch.bfloat16)
+    cache.advance(ints([20, 16, 0]), max_tokens=90)
+    cache.append(0, k, k)
+    cache.check()
+    before, lens = cache.pages[0].clone(), cache.kv_lens.clone()
+    for add, why in (([0, 0, 80], "free pages"), ([70, 0, 0], "table row"), ([40, 40, 40], "max_tokens")):
+        cache.advance(ints(add), max_tokens=90)
+        cache.append(0, k, -k)
+        out = cache.attention(0, torch.randn(90, 8, 128, device=DEV).to(torch.bfloat16), max_q_len=80, out=torch.full((90, 8, 128), 7.0, device=DEV, dtype=torch.bfloat16))
+        with pytest.raises(hq.HyQuantError, match=why):
+            cache.check()
+        assert torch.equal(cache.pages[0], before) and torch.equal(cache.kv_lens, lens) and (out == 7).all()
+    cache.advance(ints([0, 0, 48]), max_tokens=90)
+    cache.check()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [3, 9], [40, 150]])
+def test_no_requests_no_tokens_no_pages(new):
+    lens = [250, 131]
+    q, pages, table, cu = make(lens, new, 8, 2, 64, torch.float16, seed=35)
+    most = max(new)
+    room = torch.full_like(q, 7.0)
+    hq.paged_attention(q, pages, table[:0], ints([]), cu_q=ints([0]), max_q_len=most, out=room)
+    hq.paged_attention(q, pages, table, ints(lens), cu_q=ints([0, 0, 0]), max_q_len=most, out=room)
+    assert (room == 7).all()
+    assert hq.paged_attention(q[:0], pages, table, ints(lens), cu_q=ints([0, 0, 0]), max_q_len=most).shape == (0, 8, 128)
+    got = hq.paged_attention(q, pages[:0], table, ints(lens), cu_q=ints(cu), max_q_len=most, out=room)
+    assert (got == 0).all()
+    hq.paged_append(pages, q[:0, :2], q[:0, :2], torch.zeros(0, dtype=torch.int64, device=DEV))
+    assert hq.paged_read(pages, torch.zeros(0, dtype=torch.int64, device=DEV))[0].shape == (0, 2, 128)
+    step = hq.page_advance(ints([]), ints([]), ints([]), table[:0], ints([]), ints([0]), page_size=64, max_tokens=3)
+    assert step.cu_q.tolist() == [0] and step.slots.tolist() == [-1] * 3 and int(step.status) == 0
