@@ -1,8 +1,9 @@
 // Attention over the paged 4-bit cache: the entry points.  Calls whose new tokens times query heads per kv head fit 16 rows go to the
 // split kernel on mma.sync (hq_paged_decode.cu), longer ones to the tile kernel on tcgen05 (hq_paged_tile.cu), whose query tiles
 // have 256 rows whatever they are filled with.  Both at the rule's border and below it, split kernel and tile kernel: one request of 512
-// tokens, four rows 10.2 and 14.9 us; of 32768 16.6 and 39.6; 16 of 16384, eight rows 67 and 179; 4 of 65536, sixteen rows
-// 38 and 61; sixteen rows, 2 of 20000 30 and 42, 16 of 4096 41 and 60, 64 of 512 37 and 60.
+// tokens, four rows 7.2 and 16.0 us; of 32768 16.7 and 40.2; 16 of 16384, eight rows 70 and 177; 4 of 65536, sixteen rows
+// 39 and 62; sixteen rows, 2 of 20000 20 and 34, 16 of 4096 22 and 26, 64 of 512 13 and 23.  The rule goes by the call's longest request: one
+// that passes it takes the others along, which then cost what the second figures say.
 #include "hq_paged.cuh"
 
 namespace hq {

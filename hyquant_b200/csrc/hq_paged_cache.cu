@@ -179,7 +179,8 @@ advance_kernel(const AdvanceParams p, int blocks) {
 // HBM-bound: 256 bytes a 16-bit row read, 66 written, or the other way round.  Eight lanes take the K row and the V row of one token
 // and head, so that two rows' loads are in flight per lane; a lane has channels 8 sub .. + 7 and 64 + 8 sub .. + 7, so that an
 // instruction moves whole lines (thirty-two bytes a lane in one piece: every line took two instructions, 17.1 and 19.9 us below).
-// 12289 tokens of eight heads in fp16, rows in and out: 24.8 us for the two, where their 127 MB at a copy's rate take 19.4.
+// 12289 tokens of eight heads, in and out: bf16 and fp16 14.2 and 9.9 us, fp32 19.1 and 30.2; one behind the other in fp16 24.7, where
+// their 127 MB at a copy's rate take 19.4.
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
   const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
   const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -292,7 +293,8 @@ static int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 3
 // A launch that the kernel before it in the stream lets begin early: the kernels wait for it (griddepcontrol.wait) before they touch
 // memory, but their launch is over by then (rows of 16 tokens in and out 3.8 -> 3.4 us).  Of these only page_advance lets the next one
 // begin early in turn, as attention does, and behind its own wait: what comes next may rely on every kernel but the one just before it
-// (hq_decode_splitk does, which fetches older rows of its cache at once).  Blocks of read_kernel that wait beside append_kernel's took 29.3 us for a prompt's rows, not 24.8.
+// (hq_decode_splitk does, which fetches older rows of its cache at once).  Blocks of read_kernel that wait beside append_kernel's took
+// 29.3 us for a prompt's rows, not 24.8.
 template <typename... P, typename... A>
 static cudaError_t launch_early(void (*kernel)(P...), int grid, int cluster, int threads, int smem, cudaStream_t st, A... a) {
   cudaLaunchAttribute attr[2]{};

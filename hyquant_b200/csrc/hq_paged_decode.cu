@@ -1,17 +1,18 @@
 // Attention of a few new tokens per request over the paged 4-bit cache: calls whose new tokens times query heads per kv head
 // fit 16 rows (one token at every group size, drafts of a few).
 //
-// 132 bytes a cached token and kv head, read once: at 6.5 TB/s an SM has some 100 clocks for 32 tokens, and the 530 instructions that a warp
-// spends on them (unpacking 176, exponentials and sums 60, products 34) take its four schedulers 130 at full rate; half of them are for the
-// ALU pipe, which takes one every other clock.  It is 240 as it is.
-// So long batches are bound by issue: 16 requests of up to 32768 tokens, 8 heads, 58 us, 4.0 TB/s.  Short calls are bound by a chain
-// of latencies (finding the part, first copy, queries, one unit, the merges): one request of 517 tokens 7.7 us, of 32768 15.7 us.
-// Nine to sixteen rows a head double the products and exponentials, not the unpacking: 4 requests of up to 131072 tokens, 2 heads, 47 us.
-// O += P V beside the next unit's scores in one stretch of code, in order or interleaved, gave nothing (61 us where the batch takes 58).
+// 132 bytes a cached token and kv head, read once: 32 tokens are 4224 bytes, 95 ns of an SM's share of 6.54 TB/s.  A unit of them takes an SM
+// 131 ns (16 requests of 4096 to 65536 tokens, 64 query heads over 8), and a call takes 12 us beside its units: finding the part, first copy,
+// queries, the merges, the merge kernel.  16 requests of up to 32768 tokens 61 us, 3.8 TB/s; one request of 517 tokens 8.0 us, of 32768
+// 16.4.  Counters of the long batch: 547 instructions a unit with all that runs once, issue slots 50 %, ALU pipe 49 % (unpacking, masks),
+// warps wait for a math pipe (0.88 of every issue) and for an instruction's result (1.58) more than for data (0.29).
+// Nine to sixteen rows a head double the products and exponentials, not the unpacking: 213 ns a unit and 16 us; 4 requests of up to 131072
+// tokens, 2 heads, 49 us, issue slots 37 %.
+// O += P V beside the next unit's scores in one stretch of code, in order or interleaved, gave nothing (61 us where the batch took 58).
 //
 // Work split.  A kv head of a request is a run of units of 32 tokens and one closing unit, so that heads without tokens cost
-// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one per SM, and a block's part evenly over its warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no
-// barrier inside, and a run that lies within one warp's part is written out by that warp.  Runs that several warps share are
+// something too; all runs in a row (requests, then heads) are cut evenly over the blocks, one per SM, and a block's part evenly over its
+// warps, whatever the lengths are: they are only known on the device.  A warp walks its part alone: no barrier inside, and a run that lies within one warp's part is written out by that warp.  Runs that several warps share are
 // merged through shared memory at the block's end, runs that several blocks share by the merge kernel.  Everything goes by
 // position, nothing by arrival: results do not depend on timing, and no counter has to be zero beforehand.
 //
@@ -37,9 +38,9 @@ constexpr int kRowPad = 132;                    // floats of a row of a piece
 constexpr float kShift = 9.0f;                  // P~ v_scale = 2^(s - m + 9) v_scale: at most 2^10 when a reference is set, 2^15 before it moves
 constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
 constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ v_scale that lets it stay
-// Warps of a block: few enough for their registers (168 and 234 without spills), and as many on every scheduler.  The 32768 tokens, the batch
-// and 200 short requests: 16 warps 16.6, 57.8, 28.7 us, 14 17.3, 62.8, 29.3, 12 15.7, 57.8, 25.5, 11 17.1, 63.4, 26.1, 8 17.1, 68.4, 28.1.
-// More than eight rows: 12 warps 49.6 us, 11 51.1, 10 54.4, 8 47.0.
+// Warps of a block: few enough for their registers (167; more than eight rows 255, with 20 bytes spilled), and as many on every scheduler.
+// The 32768 tokens, the batch and 200 short requests: 16 warps 17.3, 62.2, 29.6 us, 14 18.1, 67.2, 30.3, 12 16.4, 61.1, 25.9, 11 17.7, 66.3,
+// 26.0, 8 17.8, 72.3, 28.4.  More than eight rows: 12 warps 51.9 us, 11 53.7, 10 57.1, 8 49.1.
 __host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 12 : 8; }
 __host__ __device__ constexpr int piece_floats(int NT) { return 8 * NT * kRowPad + 16 * NT; }
 
@@ -650,8 +651,9 @@ merge_kernel(const AttnParams p, int grid) {
 static int tiles_of(const AttnParams& p) { return p.max_q_len * p.G <= 8 ? 1 : 2; }
 
 // Short tables and no more runs than SMs: a block per run, nothing to merge across blocks, one launch and no workspace.  Against the cut
-// over all SMs: one request of 8 heads, 512 tokens 7.3 us and 10.3, 1024 9.4 and 9.7, 2048 13.1 and 9.9; eight requests 7.5 and
-// 10.5, 9.7 and 10.9, 13.7 and 12.7; four of 2 heads with sixteen rows 11.8 and 15.1, 14.9 and 15.3, 21.2 and 15.2.
+// over all SMs: one request of 8 heads, 512 tokens 7.2 us and 10.1, 1024 9.5 and 9.5, 2048 13.4 and 9.8; eight requests 7.6 and
+// 10.4, 10.4 and 11.3, 14.5 and 13.4; four of 2 heads with sixteen rows 11.5 and 15.1, 14.9 and 15.1, 21.6 and 15.1.  The rule asks the
+// table's width, since lengths are only known on the device: a wide table takes the cut whatever is in it.
 static bool block_per_run(const AttnParams& p) {
   return ((int64_t)p.max_pages << p.page_shift) <= 1024 && (int64_t)p.R * p.H_KV <= sm_count();
 }

@@ -5,7 +5,9 @@
 // group size; keys come in tiles of 64.  The two halves of the softmax take 128 rows each, or, where a query tile has no more than
 // 128 rows, the same rows and every other key tile, and join their states at the end.  A key tile of 256 rows is 8.4 MFLOP and 16384
 // exponentials, some 1024 clocks of an SM each at their nominal rates; the products' operands and the unpacked tiles pass through
-// shared memory in some 1600.  It takes 1930: a prompt of 2048 tokens over 32768 cached ones, 32 heads over 8, 890 us, 1.20 PFLOP/s.
+// shared memory in some 1600.  It takes 1850 with all that runs once (1.59 M clocks for 859 key tiles an SM): a prompt of 2048 tokens over
+// 32768 cached ones, 32 heads over 8, 910 us in a short run, 1.17 PFLOP/s, 1024 in a long one at the power cap's clock.  Counters: tensor
+// pipe 55 %, issue slots 53 %, ALU pipe 34 %.
 // Exponentials moved to the FMA pipe (an eighth to a half of them, by polynomial) gave nothing, key tiles of 128 lost the second
 // buffer of scores and took 1236 us where 64 took 1052.
 //
@@ -18,7 +20,8 @@
 //   14         fetches the codes: a tile is four blocks of sixteen tokens, a bulk copy each, some tiles ahead
 // Channels stand in the order in which the unpacking produces them (0 4 1 5 2 6 3 7 in every eight), in Q, K and V alike; the rows that
 // are written put them back.  What runs once per query tile is written as loops: straight-line code that is met cold costs more
-// for its instructions' way to the SM than for their execution (results 10800 -> 5000 clocks).
+// for its instructions' way to the SM than for their execution (results 10800 -> 5000 clocks).  480 threads leave 128 registers each, and 60
+// bytes are spilled; registers moved between the roles took longer.
 //
 // All query tiles' keys in a row (requests, heads, query tiles) are cut evenly over the blocks, by position: lengths are only known
 // on the device, and no block is left with a long tile at the end.  A query tile that several blocks share leaves softmax states,
@@ -35,7 +38,9 @@ constexpr int kKStages = 3, kVStages = 4;        // K tiles and V tiles in share
 constexpr int kAhead = 4;                        // tiles of codes in shared memory
 constexpr int kCodeBytes = kKeys / kTok * kBlockBytes;
 constexpr float kTShift = 9.0f, kTMost = 32768.0f;        // P~ = 2^(s - m + 9); a tile's row sum that calls for a new reference
-constexpr float kTFar = 8192.0f;                 // scores (log2) up to which a rounded reference will do: it is off by 2^-12 of a power of two at most
+// Scores (log2) up to which a rounded reference will do: it is off by 2^-12 of a power of two at most.  Exact differences in every tile took 930
+// us where the prompt takes 910.
+constexpr float kTFar = 8192.0f;
 constexpr uint32_t kTPolls = 400000u;
 
 struct TileSmem {

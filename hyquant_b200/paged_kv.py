@@ -198,9 +198,10 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
     """Attention of new tokens ``q`` [T, H_Q, 128] (bf16 or fp16) over the cache, which holds them already -> [T, H_Q, 128].
 
     Request r has the rows ``cu_q[r] .. cu_q[r + 1]`` of ``q`` (without ``cu_q``: row r, one each) and ``kv_lens[r]`` cached tokens
-    with them; its token i of n sees the first ``kv_lens[r] - n + i + 1`` of them, and gets zeros if there is none.
+    with them; its token i of n sees the first ``kv_lens[r] - n + i + 1`` of them, and gets zeros if there is none.  A length past the
+    table counts as the table's.
     ``max_q_len`` is the most tokens of a request (tokens beyond it are not computed).  ``sm_scale`` is 128 ** -0.5 by default.
-    Rows of ``out`` behind the last token stay as they are (without ``out`` they are not initialised)."""
+    Rows of ``out`` do not overlap; those behind the last token stay as they are (without ``out`` they are not initialised)."""
     num_pages, H, page_size = _pool(pages)
     dev, dtype, shape = pages.device, q.dtype, q.shape
     if len(shape) != 3 or shape[2] != 128 or q.device != dev:
