@@ -38,7 +38,7 @@ constexpr int kRowPad = 132;                    // floats of a row of a piece
 constexpr float kShift = 9.0f;                  // P~ v_scale = 2^(s - m + 9) v_scale: at most 2^10 when a reference is set, 2^15 before it moves
 constexpr float kNone = 1e30f;                  // a shift under which nothing is 0 and any key calls for a reference
 constexpr float kFirst = 3.0f, kLeast = 256.0f; // the reference that a run's first unit is tried with, and the least sum of 32 P~ v_scale that lets it stay
-// Warps of a block: few enough for their registers (167; more than eight rows 255, with 20 bytes spilled), and as many on every scheduler.
+// Warps of a block: few enough for their registers (167; more than eight rows 255, with 16 bytes spilled), and as many on every scheduler.
 // The 32768 tokens, the batch and 200 short requests: 16 warps 17.3, 62.2, 29.6 us, 14 18.1, 67.2, 30.3, 12 16.4, 61.1, 25.9, 11 17.7, 66.3,
 // 26.0, 8 17.8, 72.3, 28.4.  More than eight rows: 12 warps 51.9 us, 11 53.7, 10 57.1, 8 49.1.
 __host__ __device__ constexpr int warps_of(int NT) { return NT == 1 ? 12 : 8; }
@@ -236,7 +236,7 @@ decode_kernel(const AttnParams p, bool whole) {
     const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (int64_t)(q.q0 + i) * p.q_st +
                                                      (int64_t)(c.h * p.G + n - i * p.G) * p.q_sh + 32 * t4);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) raw[w] = n < q.nq * p.G ? __ldg(at + w) : make_uint4(0u, 0u, 0u, 0u);
+    for (int w = 0; w < 4; ++w) raw[w] = n < q.nq * p.G ? at[w] : make_uint4(0u, 0u, 0u, 0u);      // (not __ldg: out may be q)
     lim0 = q.past + 1;
   };
   auto open = [&]() {

@@ -6,7 +6,7 @@
 // 128 rows, the same rows and every other key tile, and join their states at the end.  A key tile of 256 rows is 8.4 MFLOP and 16384
 // exponentials, some 1024 clocks of an SM each at their nominal rates; the products' operands and the unpacked tiles pass through
 // shared memory in some 1600.  It takes 1850 with all that runs once (1.59 M clocks for 859 key tiles an SM): a prompt of 2048 tokens over
-// 32768 cached ones, 32 heads over 8, 910 us in a short run, 1.17 PFLOP/s, 1024 in a long one at the power cap's clock.  Counters: tensor
+// 32768 cached ones, 32 heads over 8, 894 to 915 us in a short run, 1.18 PFLOP/s, 1024 in a long one at the power cap's clock.  Counters: tensor
 // pipe 55 %, issue slots 53 %, ALU pipe 34 %.
 // Exponentials moved to the FMA pipe (an eighth to a half of them, by polynomial) gave nothing, key tiles of 128 lost the second
 // buffer of scores and took 1236 us where 64 took 1052.

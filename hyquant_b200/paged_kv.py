@@ -200,8 +200,9 @@ def paged_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tens
     Request r has the rows ``cu_q[r] .. cu_q[r + 1]`` of ``q`` (without ``cu_q``: row r, one each) and ``kv_lens[r]`` cached tokens
     with them; its token i of n sees the first ``kv_lens[r] - n + i + 1`` of them, and gets zeros if there is none.  A length past the
     table counts as the table's.
-    ``max_q_len`` is the most tokens of a request (tokens beyond it are not computed).  ``sm_scale`` is 128 ** -0.5 by default.
-    Rows of ``out`` do not overlap; those behind the last token stay as they are (without ``out`` they are not initialised)."""
+    ``max_q_len`` is the most tokens of a request (tokens beyond it are not computed).  ``sm_scale`` (0 or more) is 128 ** -0.5 by default.
+    ``out`` may be ``q`` and shares nothing else with the arguments; its rows do not overlap, and those behind the last token stay
+    as they are (without ``out`` they are not initialised)."""
     num_pages, H, page_size = _pool(pages)
     dev, dtype, shape = pages.device, q.dtype, q.shape
     if len(shape) != 3 or shape[2] != 128 or q.device != dev:

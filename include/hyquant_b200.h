@@ -494,7 +494,8 @@ int hq_paged_read(const void* pages, int64_t num_pages, int page_size, const int
  * (null: token r) and kv_lens[r] cached tokens with them; its token i of n sees keys 0 .. kv_lens[r] - n + i:
  *   out[t, h] = sum_j softmax_j(sm_scale q[t, h] . k_j) v_j;   a token that sees no key gets zeros.
  * max_q_len: no request has more tokens (those beyond are not computed).  Rows of out behind the last token are not written.
- * A length past the table counts as the table's; pages outside the pool hold absent keys.  Rows of out do not overlap.  Refused (HQ_ERR_UNSUPPORTED): 2^27 rows (tokens
+ * A length past the table counts as the table's; pages outside the pool hold absent keys.  Rows of out do not overlap; out may be q,
+ * row for row, and shares nothing else with the arguments.  Refused (HQ_ERR_UNSUPPORTED): 2^27 rows (tokens
  * times query heads per kv head) or more, tables and rows whose 32-token units, or 64-token tiles times 256-row query tiles, pass the
  * kernels' 32-bit positions.  A device wait that runs out makes the rows concerned NaN. */
 typedef struct hq_paged_attention_args {

@@ -802,3 +802,14 @@ def test_no_requests_no_tokens_no_pages(new):
     assert hq.paged_read(pages, torch.zeros(0, dtype=torch.int64, device=DEV))[0].shape == (0, 2, 128)
     step = hq.page_advance(ints([]), ints([]), ints([]), table[:0], ints([]), ints([0]), page_size=64, max_tokens=3)
     assert step.cu_q.tolist() == [0] and step.slots.tolist() == [-1] * 3 and int(step.status) == 0
+
+
+@pytest.mark.parametrize("lens,new", [([517], [1]), ([9000, 1, 20000, 300], [1, 1, 1, 1]), ([9000, 4100, 40], [4, 2, 1]), ([9000, 4100], [40, 300])])
+def test_the_output_in_place_of_the_queries(lens, new):
+    """``out`` may be ``q``: short tables and long ones, runs and query tiles of one block and of several."""
+    q, pages, table, cu = make(lens, new, 8, 2, 16, torch.bfloat16, seed=len(lens))
+    for _ in range(5):
+        want = hq.paged_attention(q, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new))
+        x = q.clone()
+        assert hq.paged_attention(x, pages, table, ints(lens), cu_q=ints(cu), max_q_len=max(new), out=x) is x
+        assert torch.equal(x, want)
